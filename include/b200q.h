@@ -248,6 +248,66 @@ int b200q_reduce_slots(const float* slots, int n_slots, int64_t rows, int64_t n,
  * out[i] = bit pattern of scale[i % scale_len] in the low word, upper word 0. */
 int b200q_trans_quant_param(const float* scale, int64_t scale_len, int64_t* out, int64_t out_len, void* stream);
 
+/* Tokens sorted by expert (npu_moe_init_routing_v2, npu_moe_token_permute).
+ * Assignment i = (token i / topk, slot i % topk) of expert expert_idx[i]; its row is its place in a stable sort of the
+ * assignments by expert.  An expert outside [expert_begin, expert_end) (-1 for a padded token) has no row.
+ *   quantise == 0: out[row] = x[i / topk] as it is (any dtype); a token's scale [tokens] f32 goes along to out_scale.
+ *   quantise == 1: xs = x * smooth (smooth [scale_rows, hidden], one row or one for each expert, or NULL), then int8 and
+ *                  out_scale as b200q_dynamic_quant.
+ * Rows past the last expert's are zero (their out_scale too). */
+typedef struct {
+  const void* x;            /* [tokens, hidden] bf16, f16; without quantisation also f32, i32, i8           */
+  int x_dtype;
+  const void* expert_idx;   /* [tokens, topk] i32 or i64                                                    */
+  int idx_dtype;
+  int64_t tokens, topk, hidden;
+  int64_t expert_begin, expert_end;   /* at most 1024 experts                                               */
+  int quantise;
+  const void* scale;        /* see above; may be NULL                                                       */
+  int scale_dtype;
+  int64_t scale_rows;
+  void* out;                /* [out_rows, hidden]; x's dtype, or int8 when quantised                        */
+  int64_t out_rows;         /* tokens * topk, or fewer without quantisation: rows from there on are dropped */
+  float* out_scale;         /* [out_rows], or NULL when nothing goes there                                  */
+  int32_t* row_idx;         /* [tokens * topk]: the assignment's row, -1 where it has none                  */
+  int32_t* row_src;         /* [tokens * topk] or NULL: the row's assignment, -1 where it has none          */
+  int64_t* expert_tokens;   /* [expert_end - expert_begin] or NULL: rows of each expert                     */
+  int cumulative;           /* expert_tokens counts the rows of all experts up to this one                  */
+  int strict;               /* an index of expert_end or more is an error (device error code 0x202)         */
+  void* workspace;          /* >= b200q_moe_route_workspace_bytes(), 256-byte aligned                       */
+  size_t workspace_bytes;
+} b200q_moe_route_args;
+
+size_t b200q_moe_route_workspace_bytes(int64_t assignments, int quantise);
+int b200q_moe_route(const b200q_moe_route_args* args, void* stream);
+
+/* The way back (npu_moe_token_unpermute): out[t] = sum over k of weights[t,k] * rows[row_idx[t,k]], added in fp32 in
+ * the order of k and rounded once.  rows [num_rows, hidden] and out [tokens, hidden] in bf16, f16 or f32; weights
+ * [tokens, topk] in any of them, or NULL for ones.  A row index outside [0, num_rows) adds nothing. */
+int b200q_moe_combine(const void* rows, int dtype, int64_t num_rows, const int32_t* row_idx, const void* weights,
+                      int weight_dtype, void* out, int64_t tokens, int64_t topk, int64_t hidden, void* stream);
+
+/* Gradient of b200q_moe_combine: drows[row_idx[t,k]] = weights[t,k] * dy[t], zero for rows that nothing names;
+ * dweights[t,k] = <rows[row_idx[t,k]], dy[t]> (fp32 sum), zero where there is no row.  A row that is named twice is
+ * recorded as device error 0x203 (its gradient would be a sum). */
+typedef struct {
+  const void* dy;           /* [tokens, hidden]                                                             */
+  int dtype;                /* of dy, rows and drows                                                        */
+  const void* rows;         /* [num_rows, hidden]; read for dweights only                                   */
+  int64_t num_rows;
+  const int32_t* row_idx;   /* [tokens, topk]                                                               */
+  const void* weights;      /* [tokens, topk] or NULL for ones                                              */
+  int weight_dtype;         /* of weights and dweights                                                      */
+  int64_t tokens, topk, hidden;
+  void* drows;              /* [num_rows, hidden]                                                           */
+  void* dweights;           /* [tokens, topk] or NULL                                                       */
+  void* workspace;          /* >= b200q_moe_combine_grad_workspace_bytes(), 256-byte aligned                */
+  size_t workspace_bytes;
+} b200q_moe_combine_grad_args;
+
+size_t b200q_moe_combine_grad_workspace_bytes(int64_t num_rows);
+int b200q_moe_combine_grad(const b200q_moe_combine_grad_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,72 @@
+"""Plain 64-bit CPU implementations of the mixture-of-experts block operators: the definitions the kernels are tested
+against.  Integers (rows, counts) are exact; floating results come back in float64, not rounded to the output type."""
+from __future__ import annotations
+
+import numpy as np
+import torch
+
+from . import quant_oracle
+
+F64 = torch.float64
+
+
+def sorted_rows(expert_idx: torch.Tensor, begin: int, end: int):
+    """``(row of every assignment or -1, assignment of every row or -1, rows of each expert)`` of a stable sort by
+    expert; an expert outside ``[begin, end)`` has no row."""
+    flat = expert_idx.reshape(-1).to(torch.int64).numpy()
+    live = (flat >= begin) & (flat < end)
+    order = np.argsort(np.where(live, flat, end), kind="stable")[:int(live.sum())]
+    row = np.full(flat.size, -1, dtype=np.int32)
+    row[order] = np.arange(order.size, dtype=np.int32)
+    src = np.full(flat.size, -1, dtype=np.int32)
+    src[:order.size] = order
+    counts = np.bincount(flat[live] - begin, minlength=end - begin).astype(np.int64)
+    return torch.from_numpy(row), torch.from_numpy(src), torch.from_numpy(counts)
+
+
+def gather_rows(x: torch.Tensor, row_src: torch.Tensor, topk: int) -> torch.Tensor:
+    """``x[assignment // topk]`` for every row, zero for rows without one; x's dtype."""
+    out = torch.zeros((row_src.numel(), x.shape[1]), dtype=x.dtype)
+    live = row_src >= 0
+    out[live] = x[(row_src[live] // topk).long()]
+    return out
+
+
+def route_quantised(x: torch.Tensor, expert_idx: torch.Tensor, smooth: torch.Tensor | None, begin: int, end: int):
+    """int8 rows and their scales, as ``quant_oracle.dynamic_quant`` of the gathered rows with each expert's smooth row."""
+    _, src, counts = sorted_rows(expert_idx, begin, end)
+    n = int(counts.sum())
+    q = torch.zeros((src.numel(), x.shape[1]), dtype=torch.int8)
+    scale = torch.zeros((src.numel(),), dtype=torch.float32)
+    if n:
+        rows = gather_rows(x, src, expert_idx.shape[1])[:n]
+        if smooth is None or smooth.shape[0] == 1:
+            q[:n], scale[:n] = quant_oracle.dynamic_quant(rows, None if smooth is None else smooth[0])
+        else:
+            q[:n], scale[:n] = quant_oracle.dynamic_quant(rows, smooth, torch.cumsum(counts, 0).to(torch.int32))
+    return q, scale
+
+
+def combine(rows: torch.Tensor, row_idx: torch.Tensor, weights: torch.Tensor | None, tokens: int, topk: int):
+    """``(sum over k of weights[t,k] * rows[row_idx[t,k]], sum of the magnitudes)``; a row index out of range adds nothing."""
+    idx = row_idx.reshape(tokens, topk).long()
+    live = (idx >= 0) & (idx < rows.shape[0])
+    parts = torch.zeros((tokens, topk, rows.shape[1]), dtype=F64)
+    parts[live] = rows.to(F64)[idx[live]]
+    if weights is not None:
+        parts = parts * torch.where(live, weights.to(F64), torch.zeros((), dtype=F64))[:, :, None]
+    return parts.sum(1), parts.abs().sum(1)
+
+
+def combine_grad(dy: torch.Tensor, rows: torch.Tensor, row_idx: torch.Tensor, weights: torch.Tensor | None, tokens: int, topk: int):
+    """``(drows, dweights, bound on the magnitude of dweights' terms)``."""
+    idx = row_idx.reshape(tokens, topk).long()
+    live = (idx >= 0) & (idx < rows.shape[0])
+    t, k = torch.nonzero(live, as_tuple=True)
+    w = torch.ones((tokens, topk), dtype=F64) if weights is None else weights.to(F64)
+    drows = torch.zeros(rows.shape, dtype=F64)
+    drows[idx[t, k]] = dy.to(F64)[t] * w[t, k][:, None]
+    dw, size = torch.zeros((tokens, topk), dtype=F64), torch.zeros((tokens, topk), dtype=F64)
+    terms = rows.to(F64)[idx[t, k]] * dy.to(F64)[t]
+    dw[t, k], size[t, k] = terms.sum(1), terms.abs().sum(1)
+    return drows, dw, size

@@ -29,6 +29,11 @@ OPS = (
     "npu_mm_reduce_scatter_base",
     "npu_all_gather_base_mm",
     "npu_mm_all_reduce_base",
+    "npu_moe_init_routing_v2",
+    "npu_moe_token_permute",
+    "npu_moe_token_permute_grad",
+    "npu_moe_token_unpermute",
+    "npu_moe_token_unpermute_grad",
 )
 
 
@@ -50,6 +55,11 @@ npu_trans_quant_param = _torch.ops.npu.npu_trans_quant_param
 npu_dynamic_quant_asymmetric = _torch.ops.npu.npu_dynamic_quant_asymmetric
 npu_anti_quant = _torch.ops.npu.npu_anti_quant
 npu_swiglu_quant = _torch.ops.npu.npu_swiglu_quant
+npu_moe_init_routing_v2 = _torch.ops.npu.npu_moe_init_routing_v2
+npu_moe_token_permute = _torch.ops.npu.npu_moe_token_permute
+npu_moe_token_permute_grad = _torch.ops.npu.npu_moe_token_permute_grad
+npu_moe_token_unpermute = _torch.ops.npu.npu_moe_token_unpermute
+npu_moe_token_unpermute_grad = _torch.ops.npu.npu_moe_token_unpermute_grad
 
 from . import collective_ops  # noqa: E402,F401  (defines the three collective-fused operators in torch.ops.npu)
 

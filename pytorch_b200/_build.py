@@ -69,14 +69,15 @@ def build_torch_ext(force: bool = False) -> str:
     from torch.utils import cpp_extension
 
     build_cabi(force)
-    src = os.path.join(CSRC, "register.cpp")
-    if force or _stale(TORCH_LIB, [src, os.path.join(ROOT, "include", "b200q.h"), CABI_LIB]):
+    src = [os.path.join(CSRC, f) for f in sorted(os.listdir(CSRC)) if f.endswith(".cpp")]
+    headers = [os.path.join(CSRC, "register_common.h"), os.path.join(ROOT, "include", "b200q.h")]
+    if force or _stale(TORCH_LIB, [*src, *headers, CABI_LIB]):
         tlib = os.path.join(os.path.dirname(torch.__file__), "lib")
         inc = [f"-I{p}" for p in cpp_extension.include_paths()] + [
             f"-I{os.path.join(_cuda_home(), 'include')}", f"-I{os.path.join(ROOT, 'include')}"]
         abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
         cmd = ["g++", "-O2", "-std=c++17", "-shared", "-fPIC", f"-D_GLIBCXX_USE_CXX11_ABI={abi}",
-               "-DTORCH_API_INCLUDE_EXTENSION_H", *inc, src, "-o", TORCH_LIB,
+               "-DTORCH_API_INCLUDE_EXTENSION_H", *inc, *src, "-o", TORCH_LIB,
                f"-L{LIBDIR}", "-lb200q", f"-L{tlib}", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-lc10",
                "-lc10_cuda", f"-L{os.path.join(_cuda_home(), 'lib64')}", "-lcudart",
                "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{tlib}"]

@@ -28,6 +28,8 @@ EXPORTS = (
     "b200q_trans_quant_param", "b200q_scatter_columns", "b200q_dynamic_quant_ext", "b200q_anti_quant",
     "b200q_swiglu_quant", "b200q_enable_host_error_word", "b200q_peek_device_error", "b200q_selftest_expire_wait",
     "b200q_peer_barrier", "b200q_reduce_slots", "b200q_copy_columns",
+    "b200q_moe_route_workspace_bytes", "b200q_moe_route", "b200q_moe_combine",
+    "b200q_moe_combine_grad_workspace_bytes", "b200q_moe_combine_grad",
 )
 
 
@@ -57,6 +59,33 @@ class WeightQuantMatmulArgs(C.Structure):
         ("group_size", C.c_int64),
         ("bias", C.c_void_p),
         ("out", C.c_void_p),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
+    ]
+
+
+class MoeRouteArgs(C.Structure):
+    _fields_ = [
+        ("x", C.c_void_p), ("x_dtype", C.c_int),
+        ("expert_idx", C.c_void_p), ("idx_dtype", C.c_int),
+        ("tokens", C.c_int64), ("topk", C.c_int64), ("hidden", C.c_int64),
+        ("expert_begin", C.c_int64), ("expert_end", C.c_int64),
+        ("quantise", C.c_int),
+        ("scale", C.c_void_p), ("scale_dtype", C.c_int), ("scale_rows", C.c_int64),
+        ("out", C.c_void_p), ("out_rows", C.c_int64),
+        ("out_scale", C.c_void_p), ("row_idx", C.c_void_p), ("row_src", C.c_void_p), ("expert_tokens", C.c_void_p),
+        ("cumulative", C.c_int), ("strict", C.c_int),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
+    ]
+
+
+class MoeCombineGradArgs(C.Structure):
+    _fields_ = [
+        ("dy", C.c_void_p), ("dtype", C.c_int),
+        ("rows", C.c_void_p), ("num_rows", C.c_int64),
+        ("row_idx", C.c_void_p),
+        ("weights", C.c_void_p), ("weight_dtype", C.c_int),
+        ("tokens", C.c_int64), ("topk", C.c_int64), ("hidden", C.c_int64),
+        ("drows", C.c_void_p), ("dweights", C.c_void_p),
         ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
     ]
 
@@ -110,6 +139,14 @@ def lib() -> C.CDLL:
         l.b200q_scatter_columns.argtypes = [C.c_void_p, C.POINTER(C.c_void_p), C.c_int, C.c_int64, C.c_int64, C.c_int64,
                                             C.c_int64, C.c_void_p]
         l.b200q_copy_columns.argtypes = l.b200q_scatter_columns.argtypes
+        l.b200q_moe_route_workspace_bytes.restype = C.c_size_t
+        l.b200q_moe_route_workspace_bytes.argtypes = [C.c_int64, C.c_int]
+        l.b200q_moe_route.argtypes = [C.POINTER(MoeRouteArgs), C.c_void_p]
+        l.b200q_moe_combine.argtypes = [C.c_void_p, C.c_int, C.c_int64, C.c_void_p, C.c_void_p, C.c_int, C.c_void_p,
+                                        C.c_int64, C.c_int64, C.c_int64, C.c_void_p]
+        l.b200q_moe_combine_grad_workspace_bytes.restype = C.c_size_t
+        l.b200q_moe_combine_grad_workspace_bytes.argtypes = [C.c_int64]
+        l.b200q_moe_combine_grad.argtypes = [C.POINTER(MoeCombineGradArgs), C.c_void_p]
         _lib = l
     return _lib
 

@@ -10,3 +10,4 @@
 #include "w8a8_gemm.cu"
 #include "w4a16_gemm.cu"
 #include "peer_scatter.cu"
+#include "moe_routing.cu"

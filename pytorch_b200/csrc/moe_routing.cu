@@ -1,0 +1,907 @@
+// Tokens to experts and back: the data movement of a mixture-of-experts layer.
+//
+//   n = tokens * topk assignments, assignment i = (token i / topk, slot i % topk), expert e_i
+//   row of i      #{j : e_j < e_i, or e_j = e_i and j < i}        (a stable sort by expert)
+//   route         out[row_i] = x[i / topk], optionally times the expert's smooth scales and quantised to int8
+//   combine       y[t] = sum_k w[t,k] * rows[row of (t,k)]        (fp32 sum in the order of k, rounded once)
+//   combine grad  drows[row of (t,k)] = w[t,k] * dy[t],  dw[t,k] = <rows[row of (t,k)], dy[t]>
+//
+// An expert outside the layer's range (-1 for a padded token) has no row: its row index is -1, its place in
+// `combine` adds nothing and is not read, and the rows past the last expert's are zero.
+//
+// Everything here is bound by HBM (or, for a decode step, by the latency of a launch), so each op touches its big
+// operands once and uses few launches: up to kDirectIds assignments every CTA finds its own rows by comparing
+// with all indices (one launch); more are sorted first by one cluster of CTAs in shared memory.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <initializer_list>
+#include <type_traits>
+
+#include "common.cuh"
+#include "ptx.cuh"
+
+namespace b200q {
+namespace {
+
+constexpr int kMaxExperts = 1024;
+constexpr int kDirectIds = 2048;          // assignments up to which every CTA counts for itself
+constexpr int kKeyShift = 12;             // (expert, assignment) in one word on that path: 1025 keys x 4096 places
+static_assert(kDirectIds <= (1 << kKeyShift), "an assignment's number fits below the expert");
+constexpr int kNoExpert = -1;
+
+// Expert of assignment i relative to the range [begin, begin + experts), or kNoExpert.
+template <typename IdT>
+__device__ __forceinline__ int expert_of(const IdT* __restrict__ ids, int64_t i, int64_t begin, int experts) {
+  const int64_t e = static_cast<int64_t>(ids[i]) - begin;
+  return (e >= 0 && e < experts) ? static_cast<int>(e) : kNoExpert;
+}
+
+// ------------------------------------------------------------------------------------------------ sorting
+// Stable counting sort of up to 2^31 indices by one cluster of CTAs.  Warp w of CTA c owns a contiguous piece of
+// the indices, so (c, w, position) is the order of the assignments.  Pass 1 counts every warp's experts in shared
+// memory, 32 indices a step (the lanes that hold the same expert find one another with match.any, one of them
+// adds); a prefix over warps, over the CTAs of the cluster (through distributed shared memory) and over the
+// experts turns the counts into first rows; pass 2 walks the indices again and hands the rows out.  No global
+// scratch, no atomics, no waiting but the cluster's barrier.
+constexpr int kSortThreads = 1024;
+constexpr int kSortWarps = kSortThreads / 32;
+
+template <typename IdT>
+__global__ void __launch_bounds__(kSortThreads)
+moe_sort_kernel(const IdT* __restrict__ ids, int64_t n, int64_t begin, int experts, int strict_limit,
+                int32_t* __restrict__ row_idx, int32_t* __restrict__ row_src, int64_t* __restrict__ expert_tokens,
+                int cumulative, int32_t* __restrict__ valid_rows) {
+  extern __shared__ int sort_smem[];
+  int* hist = sort_smem;                                   // [kSortWarps][experts]
+  int* total = hist + kSortWarps * experts;                // [experts] this CTA's counts
+  __shared__ int warp_sums[32];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = (int)cluster_ctarank(), ctas = (int)cluster_nctarank();
+  for (int i = threadIdx.x; i < kSortWarps * experts; i += kSortThreads) hist[i] = 0;
+  __syncthreads();
+
+  const int64_t steps = (n + 31) >> 5;                     // groups of 32 indices, dealt out in contiguous pieces
+  const int64_t piece = rank * (int64_t)kSortWarps + warp, pieces = (int64_t)ctas * kSortWarps;
+  const int64_t s0 = steps * piece / pieces, s1 = steps * (piece + 1) / pieces;
+  int* mine = hist + warp * experts;
+  for (int64_t s = s0; s < s1; ++s) {
+    const int64_t i = s * 32 + lane;
+    int e = kNoExpert;
+    if (i < n) {
+      e = expert_of(ids, i, begin, experts);
+      if (strict_limit && static_cast<int64_t>(ids[i]) >= strict_limit) record_device_error(kDevExpertRange);
+    }
+    const unsigned same = __match_any_sync(0xffffffffu, e);
+    if (e >= 0 && lane == __ffs(same) - 1) mine[e] += __popc(same);
+    __syncwarp();
+  }
+  __syncthreads();
+  for (int e = threadIdx.x; e < experts; e += kSortThreads) {
+    int run = 0;
+    for (int w = 0; w < kSortWarps; ++w) {
+      const int c = hist[w * experts + e];
+      hist[w * experts + e] = run;
+      run += c;
+    }
+    total[e] = run;
+  }
+  if (ctas > 1) cluster_sync_all(); else __syncthreads();
+
+  // One expert a thread: rows of that expert in the lower CTAs and in all, then an exclusive scan over the experts.
+  const int e = threadIdx.x;
+  int lower = 0, all = 0;
+  if (e < experts) {
+    for (int c = 0; c < ctas; ++c) {
+      const int v = ctas > 1 ? (int)ld_shared_cluster_u32(map_to_cta(smem_u32(total + e), c)) : total[e];
+      if (c < rank) lower += v;
+      all += v;
+    }
+  }
+  int incl = all;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int v = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += v;
+  }
+  if (lane == 31) warp_sums[warp] = incl;
+  __syncthreads();
+  if (warp == 0) {
+    int v = warp_sums[lane];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int u = __shfl_up_sync(0xffffffffu, v, o);
+      if (lane >= o) v += u;
+    }
+    warp_sums[lane] = v;
+  }
+  __syncthreads();
+  if (warp > 0) incl += warp_sums[warp - 1];
+  const int valid = warp_sums[31];
+  if (e < experts) {
+    const int first = incl - all + lower;
+    for (int w = 0; w < kSortWarps; ++w) hist[w * experts + e] += first;
+    if (rank == 0 && expert_tokens != nullptr) expert_tokens[e] = cumulative ? incl : all;
+  }
+  if (rank == 0 && threadIdx.x == 0 && valid_rows != nullptr) *valid_rows = valid;
+  if (row_src != nullptr)                                  // rows that no assignment owns
+    for (int64_t r = valid + (int64_t)rank * kSortThreads + threadIdx.x; r < n; r += (int64_t)ctas * kSortThreads) row_src[r] = -1;
+  __syncthreads();
+
+  for (int64_t s = s0; s < s1; ++s) {
+    const int64_t i = s * 32 + lane;
+    const int x = i < n ? expert_of(ids, i, begin, experts) : kNoExpert;
+    const unsigned same = __match_any_sync(0xffffffffu, x);
+    const int row = x >= 0 ? mine[x] + __popc(same & ((1u << lane) - 1)) : -1;
+    __syncwarp();
+    if (x >= 0 && lane == __ffs(same) - 1) mine[x] += __popc(same);
+    __syncwarp();
+    if (i < n) row_idx[i] = row;
+    if (x >= 0 && row_src != nullptr) row_src[row] = (int32_t)i;
+  }
+  if (ctas > 1) cluster_sync_all();                        // nobody leaves while its counts may still be read
+}
+
+// ------------------------------------------------------------------------------------------------ direct counting
+// The word that orders the assignments: expert, then number; padded ones behind every expert.
+template <typename IdT>
+__device__ __forceinline__ int direct_key(const IdT* __restrict__ ids, int i, int64_t begin, int experts) {
+  const int e = expert_of(ids, i, begin, experts);
+  return ((e < 0 ? experts : e) << kKeyShift) | i;
+}
+
+// Rows of the COUNT assignments first, first + 1, ... (those below n), by the whole CTA: how many keys are smaller.
+template <int COUNT, typename IdT>
+__device__ __forceinline__ void direct_rows(const IdT* __restrict__ ids, int n, int64_t begin, int experts, int first,
+                                            int (&red)[COUNT][32], int (&rows)[COUNT]) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, nwarps = blockDim.x >> 5;
+  int key[COUNT], cnt[COUNT];
+#pragma unroll
+  for (int k = 0; k < COUNT; ++k) {
+    key[k] = direct_key(ids, min(first + k, n - 1), begin, experts);
+    cnt[k] = 0;
+  }
+  for (int j = threadIdx.x; j < n; j += blockDim.x) {
+    const int other = direct_key(ids, j, begin, experts);
+#pragma unroll
+    for (int k = 0; k < COUNT; ++k) cnt[k] += other < key[k];
+  }
+  __syncthreads();                                         // `red` may still be read from an earlier round
+#pragma unroll
+  for (int k = 0; k < COUNT; ++k) {
+    const int c = __reduce_add_sync(0xffffffffu, cnt[k]);
+    if (lane == 0) red[k][warp] = c;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < COUNT; ++k) rows[k] = __reduce_add_sync(0xffffffffu, lane < nwarps ? red[k][lane] : 0);
+}
+
+// Rows of every expert (cumulative or not), by one CTA, for the direct path.
+template <typename IdT>
+__device__ __forceinline__ void direct_expert_tokens(const IdT* __restrict__ ids, int n, int64_t begin, int experts, int strict_limit,
+                                                     int64_t* __restrict__ expert_tokens, int cumulative) {
+  __shared__ int count[kMaxExperts];
+  for (int e = threadIdx.x; e < experts; e += blockDim.x) count[e] = 0;
+  __syncthreads();
+  for (int j = threadIdx.x; j < n; j += blockDim.x) {
+    const int e = expert_of(ids, j, begin, experts);
+    if (e >= 0) atomicAdd(&count[e], 1);                   // integers: the same sum in any order
+    if (strict_limit && static_cast<int64_t>(ids[j]) >= strict_limit) record_device_error(kDevExpertRange);
+  }
+  __syncthreads();
+  if (expert_tokens == nullptr || threadIdx.x >= 32) return;
+  int run = 0;
+  for (int e0 = 0; e0 < experts; e0 += 32) {
+    const int e = e0 + threadIdx.x;
+    const int c = e < experts ? count[e] : 0;
+    int incl = c;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, incl, o);
+      if ((int)threadIdx.x >= o) incl += v;
+    }
+    if (e < experts) expert_tokens[e] = cumulative ? run + incl : c;
+    run += __shfl_sync(0xffffffffu, incl, 31);
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ rows as bytes
+template <int BYTES> struct Chunk;
+template <> struct Chunk<16> { using type = uint4; };
+template <> struct Chunk<8> { using type = uint2; };
+template <> struct Chunk<4> { using type = uint32_t; };
+template <> struct Chunk<2> { using type = uint16_t; };
+template <> struct Chunk<1> { using type = uint8_t; };
+
+struct RouteIds {
+  const void* ids;
+  int64_t n;                 // tokens * topk
+  int64_t begin;
+  int experts, topk;
+  int strict_limit;          // indices from here on are an error (0: they are merely outside the range)
+};
+
+// Copy, few assignments: one CTA a token finds the rows of its topk slots and copies the token there; one more CTA
+// counts the experts' rows.
+template <typename IdT, typename VT>
+__global__ void __launch_bounds__(256)
+moe_copy_direct_kernel(const RouteIds r, const VT* __restrict__ x, VT* __restrict__ out, int nvec, int64_t out_rows,
+                       const float* __restrict__ token_scale, float* __restrict__ out_scale, int32_t* __restrict__ row_idx,
+                       int32_t* __restrict__ row_src, int64_t* __restrict__ expert_tokens, int cumulative) {
+  const IdT* ids = static_cast<const IdT*>(r.ids);
+  const int n = (int)r.n, tokens = n / r.topk;
+  if ((int)blockIdx.x == tokens) {
+    direct_expert_tokens(ids, n, r.begin, r.experts, r.strict_limit, expert_tokens, cumulative);
+    return;
+  }
+  constexpr int KC = 8;
+  __shared__ int red[KC][32];
+  const int t = blockIdx.x;
+  for (int k0 = 0; k0 < r.topk; k0 += KC) {
+    int rows[KC];
+    direct_rows(ids, n, r.begin, r.experts, t * r.topk + k0, red, rows);
+    const int kc = min(KC, r.topk - k0);
+    bool live[KC];
+#pragma unroll
+    for (int k = 0; k < KC; ++k) {
+      const int i = t * r.topk + k0 + k;
+      live[k] = k < kc && expert_of(ids, min(i, n - 1), r.begin, r.experts) >= 0;
+      if (k < kc && threadIdx.x == 0) {
+        row_idx[i] = live[k] ? rows[k] : -1;
+        if (row_src != nullptr) row_src[rows[k]] = live[k] ? i : -1;
+        if (out_scale != nullptr && rows[k] < out_rows) out_scale[rows[k]] = live[k] ? token_scale[t] : 0.0f;
+      }
+    }
+    for (int v = threadIdx.x; v < nvec; v += blockDim.x) {
+      const VT val = x[(int64_t)t * nvec + v];
+#pragma unroll
+      for (int k = 0; k < KC; ++k)
+        if (k < kc && rows[k] < out_rows) out[(int64_t)rows[k] * nvec + v] = live[k] ? val : VT{};
+    }
+  }
+}
+
+// Copy, many assignments: a warp takes 32 * U vectors of one token, reads them once and writes them to the token's
+// rows.  The blocks past the last token clear the rows that no assignment owns.
+template <typename VT, int U>
+__global__ void __launch_bounds__(256)
+moe_copy_kernel(const VT* __restrict__ x, VT* __restrict__ out, int64_t tokens, int topk, int64_t nvec, int segs, int64_t out_rows,
+                const float* __restrict__ token_scale, float* __restrict__ out_scale, const int32_t* __restrict__ row_idx,
+                const int32_t* __restrict__ valid_rows, int64_t move_blocks) {
+  const int lane = threadIdx.x & 31;
+  if ((int64_t)blockIdx.x >= move_blocks) {
+    const int64_t zb = blockIdx.x - move_blocks, zn = gridDim.x - move_blocks;
+    for (int64_t row = *valid_rows + zb; row < out_rows; row += zn) {
+      for (int64_t v = threadIdx.x; v < nvec; v += blockDim.x) out[row * nvec + v] = VT{};
+      if (out_scale != nullptr && threadIdx.x == 0) out_scale[row] = 0.0f;
+    }
+    return;
+  }
+  const int64_t unit = (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
+  const int64_t t = unit / segs;
+  if (t >= tokens) return;
+  const int seg = (int)(unit - t * segs);
+  const int64_t v0 = (int64_t)seg * (32 * U) + lane;
+  VT val[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u)
+    if (v0 + 32 * u < nvec) val[u] = x[t * nvec + v0 + 32 * u];
+  for (int k0 = 0; k0 < topk; k0 += 32) {
+    const int mine = k0 + lane < topk ? row_idx[t * topk + k0 + lane] : -1;
+    const int kc = min(32, topk - k0);
+    for (int k = 0; k < kc; ++k) {
+      const int64_t row = __shfl_sync(0xffffffffu, mine, k);
+      if (row < 0 || row >= out_rows) continue;
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (v0 + 32 * u < nvec) out[row * nvec + v0 + 32 * u] = val[u];
+      if (out_scale != nullptr && seg == 0 && lane == 0) out_scale[row] = token_scale[t];
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ routing + int8
+// One row: smooth multiply, row maximum, scale, quantised values, all with the helpers (and bits) of
+// npu_dynamic_quant.  The CTA owns the row; each thread holds ITERS vectors of eight values.
+template <typename T, typename ST, int ITERS>
+__device__ __forceinline__ void quant_row_store(const uint4 (&raw)[ITERS], const ST* __restrict__ smooth, int nvec,
+                                                int8_t* __restrict__ y, float* __restrict__ scale_out, float* red) {
+  float2 f[ITERS][4];
+  float amax = 0.0f;
+#pragma unroll
+  for (int i = 0; i < ITERS; ++i) {
+    const int v = threadIdx.x + i * blockDim.x;
+    float2 sm[4] = {{1.0f, 1.0f}, {1.0f, 1.0f}, {1.0f, 1.0f}, {1.0f, 1.0f}};
+    if (smooth != nullptr && v < nvec) load_smooth8(smooth + (int64_t)v * 8, sm);
+    products8<T, true>(raw[i], sm, f[i], amax);
+  }
+  amax = block_max(amax, red);
+  const float scale = scale_of_amax(amax);
+  if (threadIdx.x == 0) *scale_out = scale;
+  const float inv = quant_inverse(scale);
+  uint2* yr = reinterpret_cast<uint2*>(y) + threadIdx.x;
+#pragma unroll
+  for (int i = 0; i < ITERS; ++i)
+    if (threadIdx.x + i * blockDim.x < nvec)
+      st_stream(yr + i * blockDim.x, inv == inv ? quantize8<false>(f[i], scale, inv) : quantize8<true>(f[i], scale, inv));
+}
+
+// The same for any width and alignment: two passes over the row.
+template <typename T, typename ST>
+__device__ __forceinline__ void quant_row_generic(const T* __restrict__ x, const ST* __restrict__ smooth, int64_t width,
+                                                  int8_t* __restrict__ y, float* __restrict__ scale_out, float* red) {
+  float amax = 0.0f;
+  for (int64_t c = threadIdx.x; c < width; c += blockDim.x) {
+    float f = to_f32<T>(x[c]);
+    if (smooth != nullptr) f = __fmul_rn(f, to_f32<ST>(smooth[c]));
+    amax = fmaxf(amax, fabsf(f));
+  }
+  amax = block_max(amax, red);
+  const float scale = __fdiv_rn(amax, 127.0f);
+  if (threadIdx.x == 0) *scale_out = scale;
+  for (int64_t c = threadIdx.x; c < width; c += blockDim.x) {
+    float f = to_f32<T>(x[c]);
+    if (smooth != nullptr) f = __fmul_rn(f, to_f32<ST>(smooth[c]));
+    int q = 0;
+    if (scale != 0.0f) q = max(-128, min(127, __float2int_rn(__fdiv_rn(f, scale))));
+    y[c] = static_cast<int8_t>(q);
+  }
+}
+
+__device__ __forceinline__ void zero_quant_row(int8_t* __restrict__ y, float* __restrict__ scale_out, int64_t width) {
+  for (int64_t c = threadIdx.x; c < width; c += blockDim.x) y[c] = 0;
+  if (threadIdx.x == 0) *scale_out = 0.0f;
+}
+
+// Few assignments: one CTA an assignment.  ITERS 0: any width and alignment.
+template <typename IdT, typename T, typename ST, int ITERS>
+__global__ void __launch_bounds__(512)
+moe_quant_direct_kernel(const RouteIds r, const T* __restrict__ x, int64_t width, const ST* __restrict__ smooth, int smooth_rows,
+                        int8_t* __restrict__ out, float* __restrict__ out_scale, int32_t* __restrict__ row_idx,
+                        int32_t* __restrict__ row_src, int64_t* __restrict__ expert_tokens, int cumulative) {
+  const IdT* ids = static_cast<const IdT*>(r.ids);
+  const int n = (int)r.n;
+  if ((int)blockIdx.x == n) {
+    direct_expert_tokens(ids, n, r.begin, r.experts, r.strict_limit, expert_tokens, cumulative);
+    return;
+  }
+  __shared__ int red_i[1][32];
+  __shared__ float red[32];
+  const int i = blockIdx.x;
+  const T* xr = x + (int64_t)(i / r.topk) * width;
+  const int nvec = (int)(width >> 3);
+  uint4 raw[ITERS ? ITERS : 1];
+  if constexpr (ITERS > 0) {                               // in flight while the row is being found
+#pragma unroll
+    for (int q = 0; q < ITERS; ++q) {
+      const int v = threadIdx.x + q * blockDim.x;
+      raw[q] = v < nvec ? __ldg(reinterpret_cast<const uint4*>(xr) + v) : make_uint4(0, 0, 0, 0);
+    }
+  }
+  int rows[1];
+  direct_rows(ids, n, r.begin, r.experts, i, red_i, rows);
+  const int64_t row = rows[0];
+  const int e = expert_of(ids, i, r.begin, r.experts);
+  if (threadIdx.x == 0) {
+    row_idx[i] = e >= 0 ? (int)row : -1;
+    if (row_src != nullptr) row_src[row] = e >= 0 ? i : -1;
+  }
+  if (e < 0) {
+    zero_quant_row(out + row * width, out_scale + row, width);
+    return;
+  }
+  const ST* sm = smooth == nullptr ? nullptr : smooth + (smooth_rows > 1 ? (int64_t)e * width : 0);
+  if constexpr (ITERS > 0) quant_row_store<T, ST, ITERS>(raw, sm, nvec, out + row * width, out_scale + row, red);
+  else quant_row_generic<T, ST>(xr, sm, width, out + row * width, out_scale + row, red);
+}
+
+// Many assignments: persistent CTAs take contiguous pieces of the sorted rows (so a piece stays with one expert's
+// smooth scales, which the SM's L1 then holds); the next row is in flight during the arithmetic of this one.
+template <typename IdT, typename T, typename ST, int ITERS>
+__global__ void __launch_bounds__(512)
+moe_quant_kernel(const RouteIds r, const T* __restrict__ x, int64_t width, const ST* __restrict__ smooth, int smooth_rows,
+                 int8_t* __restrict__ out, float* __restrict__ out_scale, const int32_t* __restrict__ row_src) {
+  const IdT* ids = static_cast<const IdT*>(r.ids);
+  __shared__ float red[2][32];
+  const int nvec = (int)(width >> 3);
+  const int64_t r0 = r.n * blockIdx.x / gridDim.x, r1 = r.n * (blockIdx.x + 1) / gridDim.x;
+  uint4 raw[ITERS ? ITERS : 1], nxt[ITERS ? ITERS : 1];
+  auto load = [&](int src, uint4(&to)[ITERS ? ITERS : 1]) {
+    if constexpr (ITERS > 0) {
+      const uint4* xr = reinterpret_cast<const uint4*>(x + (int64_t)(src / r.topk) * width);
+#pragma unroll
+      for (int q = 0; q < ITERS; ++q) {
+        const int v = threadIdx.x + q * blockDim.x;
+        to[q] = v < nvec ? __ldg(xr + v) : make_uint4(0, 0, 0, 0);
+      }
+    }
+  };
+  int src = r0 < r1 ? row_src[r0] : -1;
+  if (src >= 0) load(src, nxt);
+  int after = r0 + 1 < r1 ? row_src[r0 + 1] : -1;
+  int par = 0;
+  for (int64_t row = r0; row < r1; ++row) {
+    if constexpr (ITERS > 0) {
+#pragma unroll
+      for (int q = 0; q < ITERS; ++q) raw[q] = nxt[q];
+      if (after >= 0) load(after, nxt);
+    }
+    const int here = src;
+    src = after;
+    after = row + 2 < r1 ? row_src[row + 2] : -1;
+    if (here < 0) {
+      zero_quant_row(out + row * width, out_scale + row, width);
+      continue;
+    }
+    par ^= 1;                                              // a buffer is written again only behind the other one's barrier
+    const int e = expert_of(ids, here, r.begin, r.experts);
+    const ST* sm = smooth == nullptr ? nullptr : smooth + (smooth_rows > 1 ? (int64_t)e * width : 0);
+    if constexpr (ITERS > 0) {
+      quant_row_store<T, ST, ITERS>(raw, sm, nvec, out + row * width, out_scale + row, red[par]);
+    } else {
+      quant_row_generic<T, ST>(x + (int64_t)(here / r.topk) * width, sm, width, out + row * width, out_scale + row, red[par]);
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ combine
+// Values of one 16-byte vector (or one element) as floats and back.
+template <typename T, bool VEC>
+struct Lanes {
+  static constexpr int N = VEC ? 16 / (int)sizeof(T) : 1;
+  using Raw = typename Chunk<VEC ? 16 : (int)sizeof(T)>::type;
+  static __device__ __forceinline__ void unpack(const Raw& raw, float (&f)[N]) {
+    const T* p = reinterpret_cast<const T*>(&raw);
+#pragma unroll
+    for (int j = 0; j < N; ++j) f[j] = to_f32<T>(p[j]);
+  }
+  static __device__ __forceinline__ Raw pack(const float (&f)[N]) {
+    Raw raw;
+    T* p = reinterpret_cast<T*>(&raw);
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      if constexpr (sizeof(T) == 4) p[j] = f[j];
+      else if constexpr (std::is_same<T, __half>::value) p[j] = __float2half_rn(f[j]);
+      else p[j] = __float2bfloat16_rn(f[j]);
+    }
+    return raw;
+  }
+};
+
+__device__ __forceinline__ float load_as_f32(const void* p, int dtype, int64_t i) {
+  if (dtype == B200Q_F32) return static_cast<const float*>(p)[i];
+  if (dtype == B200Q_BF16) return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
+  return __half2float(static_cast<const __half*>(p)[i]);
+}
+__device__ __forceinline__ void store_from_f32(void* p, int dtype, int64_t i, float v) {
+  if (dtype == B200Q_F32) static_cast<float*>(p)[i] = v;
+  else if (dtype == B200Q_BF16) static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
+  else static_cast<__half*>(p)[i] = __float2half_rn(v);
+}
+
+// A thread owns one vector of one token: the loads of up to KC rows are issued before the first is used, the sum
+// runs in fp32 in the order of the slots.
+template <typename T, bool VEC, int KC>
+__global__ void __launch_bounds__(256)
+moe_combine_kernel(const T* __restrict__ rows, int64_t num_rows, const int32_t* __restrict__ row_idx, const void* __restrict__ weights,
+                   int weight_dtype, T* __restrict__ out, int64_t tokens, int topk, int64_t nvec) {
+  using L = Lanes<T, VEC>;
+  using Raw = typename L::Raw;
+  const int64_t unit = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+  const int64_t t = unit / nvec, v = unit - t * nvec;
+  if (t >= tokens) return;
+  float acc[L::N];
+#pragma unroll
+  for (int j = 0; j < L::N; ++j) acc[j] = 0.0f;
+  for (int k0 = 0; k0 < topk; k0 += KC) {
+    int64_t row[KC];
+    Raw raw[KC];
+#pragma unroll
+    for (int k = 0; k < KC; ++k) {
+      row[k] = k0 + k < topk ? row_idx[t * topk + k0 + k] : -1;
+      if (row[k] >= num_rows) row[k] = -1;
+    }
+#pragma unroll
+    for (int k = 0; k < KC; ++k)
+      if (row[k] >= 0) raw[k] = reinterpret_cast<const Raw*>(rows)[row[k] * nvec + v];
+#pragma unroll
+    for (int k = 0; k < KC; ++k) {
+      if (row[k] < 0) continue;
+      float f[L::N];
+      L::unpack(raw[k], f);
+      const float w = weights != nullptr ? load_as_f32(weights, weight_dtype, t * topk + k0 + k) : 1.0f;
+#pragma unroll
+      for (int j = 0; j < L::N; ++j) acc[j] = fmaf(w, f[j], acc[j]);
+    }
+  }
+  reinterpret_cast<Raw*>(out)[t * nvec + v] = L::pack(acc);
+}
+
+// Gradient of combine: one CTA a token; dy's vector stays in registers while the topk rows pass by, so dy and the
+// rows are read once and drows written once.  `marks` gets a bit for every row that has an owner: a second owner
+// (whose gradient would have to be added) is recorded as an error, and moe_clear_rows_kernel clears the rows
+// without one.
+template <typename T, bool VEC, int KC>
+__global__ void __launch_bounds__(256)
+moe_combine_grad_kernel(const T* __restrict__ dy, const T* __restrict__ rows, int64_t num_rows, const int32_t* __restrict__ row_idx,
+                        const void* __restrict__ weights, int weight_dtype, T* __restrict__ drows, void* __restrict__ dweights,
+                        uint32_t* __restrict__ marks, int topk, int64_t nvec) {
+  using L = Lanes<T, VEC>;
+  using Raw = typename L::Raw;
+  __shared__ float red[KC][8];
+  const int64_t t = blockIdx.x;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, nwarps = blockDim.x >> 5;
+  for (int k0 = 0; k0 < topk; k0 += KC) {
+    int64_t row[KC];
+    float w[KC], dot[KC];
+#pragma unroll
+    for (int k = 0; k < KC; ++k) {
+      row[k] = k0 + k < topk ? row_idx[t * topk + k0 + k] : -1;
+      if (row[k] >= num_rows) row[k] = -1;
+      w[k] = row[k] >= 0 && weights != nullptr ? load_as_f32(weights, weight_dtype, t * topk + k0 + k) : 1.0f;
+      dot[k] = 0.0f;
+    }
+    if (marks != nullptr) {
+#pragma unroll
+      for (int k = 0; k < KC; ++k)
+        if ((int)threadIdx.x == k && row[k] >= 0) {
+          const uint32_t bit = 1u << (row[k] & 31);
+          if (atomicOr(marks + (row[k] >> 5), bit) & bit) record_device_error(kDevRowTwice);
+        }
+    }
+    for (int64_t v = threadIdx.x; v < nvec; v += blockDim.x) {
+      float g[L::N];
+      L::unpack(reinterpret_cast<const Raw*>(dy)[t * nvec + v], g);
+      Raw raw[KC];
+      if (dweights != nullptr) {
+#pragma unroll
+        for (int k = 0; k < KC; ++k)
+          if (row[k] >= 0) raw[k] = reinterpret_cast<const Raw*>(rows)[row[k] * nvec + v];
+      }
+#pragma unroll
+      for (int k = 0; k < KC; ++k) {
+        if (row[k] < 0) continue;
+        float f[L::N];
+        if (dweights != nullptr) {
+          L::unpack(raw[k], f);
+#pragma unroll
+          for (int j = 0; j < L::N; ++j) dot[k] = fmaf(f[j], g[j], dot[k]);
+        }
+#pragma unroll
+        for (int j = 0; j < L::N; ++j) f[j] = w[k] * g[j];
+        reinterpret_cast<Raw*>(drows)[row[k] * nvec + v] = L::pack(f);
+      }
+    }
+    if (dweights == nullptr) continue;
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < KC; ++k) {
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) dot[k] += __shfl_xor_sync(0xffffffffu, dot[k], o);
+      if (lane == 0) red[k][warp] = dot[k];
+    }
+    __syncthreads();
+    if ((int)threadIdx.x < KC && k0 + (int)threadIdx.x < topk) {
+      float s = 0.0f;
+      for (int i = 0; i < nwarps; ++i) s += red[threadIdx.x][i];
+      store_from_f32(dweights, weight_dtype, t * topk + k0 + threadIdx.x, s);   // no row: nothing was added
+    }
+  }
+}
+
+template <typename VT>
+__global__ void __launch_bounds__(256)
+moe_clear_rows_kernel(const uint32_t* __restrict__ marks, VT* __restrict__ drows, int64_t num_rows, int64_t nvec) {
+  const int lane = threadIdx.x & 31;
+  const int64_t warp = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 5, nwarps = ((int64_t)gridDim.x * blockDim.x) >> 5;
+  for (int64_t row = warp; row < num_rows; row += nwarps) {
+    if ((marks[row >> 5] >> (row & 31)) & 1u) continue;
+    for (int64_t v = lane; v < nvec; v += 32) drows[row * nvec + v] = VT{};
+  }
+}
+
+// Widest power of two up to 16 that divides a row of `bytes` bytes and all the addresses.
+inline int chunk_bytes(int64_t bytes, std::initializer_list<const void*> ptrs) {
+  for (int c = 16; c > 1; c >>= 1) {
+    bool ok = bytes % c == 0;
+    for (const void* p : ptrs) ok = ok && aligned(p, c);
+    if (ok) return c;
+  }
+  return 1;
+}
+
+inline int element_bytes(int dtype) {
+  switch (dtype) {
+    case B200Q_BF16: case B200Q_F16: return 2;
+    case B200Q_F32: case B200Q_I32: return 4;
+    case B200Q_I8: return 1;
+    default: return 0;
+  }
+}
+
+// Launches the sort: one cluster whose size grows with the number of indices (a CTA sorts 16384 in a few
+// microseconds; more CTAs than that only add the cluster's barriers).
+template <typename IdT>
+int launch_sort(const RouteIds& r, int32_t* row_idx, int32_t* row_src, int64_t* expert_tokens, int cumulative, int32_t* valid_rows,
+                cudaStream_t st) {
+  const int smem = (kSortWarps + 1) * r.experts * (int)sizeof(int);
+  if (int rc = ensure_dynamic_smem<moe_sort_kernel<IdT>>((kSortWarps + 1) * kMaxExperts * (int)sizeof(int), "moe_route (sort)")) return rc;
+  int ctas = 1;
+  while (ctas < 8 && (int64_t)ctas * 8192 < r.n) ctas *= 2;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(ctas);
+  cfg.blockDim = dim3(kSortThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = ctas;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  cudaError_t err = cudaLaunchKernelEx(&cfg, moe_sort_kernel<IdT>, static_cast<const IdT*>(r.ids), r.n, r.begin, r.experts, r.strict_limit,
+                                       row_idx, row_src, expert_tokens, cumulative, valid_rows);
+  if (err != cudaSuccess) return fail(B200Q_ERR_LAUNCH, "moe_route (sort): %s", cudaGetErrorString(err));
+  return check_launch("moe_route (sort)");
+}
+
+template <typename IdT, int BYTES>
+int launch_copy(const b200q_moe_route_args& a, const RouteIds& r, int64_t row_bytes, int32_t* valid_rows, cudaStream_t st) {
+  using VT = typename Chunk<BYTES>::type;
+  const VT* x = static_cast<const VT*>(a.x);
+  VT* out = static_cast<VT*>(a.out);
+  const float* scale = a.out_scale != nullptr ? static_cast<const float*>(a.scale) : nullptr;
+  const int64_t nvec = row_bytes / BYTES;
+  if (r.n <= kDirectIds) {
+    moe_copy_direct_kernel<IdT, VT><<<(unsigned)(a.tokens + 1), 256, 0, st>>>(r, x, out, (int)nvec, a.out_rows, scale, a.out_scale, a.row_idx,
+                                                                              a.row_src, a.expert_tokens, a.cumulative);
+    return check_launch("moe_route (copy, few tokens)");
+  }
+  if (int rc = launch_sort<IdT>(r, a.row_idx, a.row_src, a.expert_tokens, a.cumulative, valid_rows, st)) return rc;
+  constexpr int U = 4;
+  const int64_t segs = nvec == 0 ? 1 : ceil_div(nvec, 32 * U);
+  const int64_t move_blocks = ceil_div(a.tokens * segs, 8), blocks = move_blocks + 2 * sm_count();
+  B200Q_REQUIRE(blocks <= 0x7fffffffLL, B200Q_ERR_UNSUPPORTED, "moe_route: too many rows");
+  moe_copy_kernel<VT, U><<<(unsigned)blocks, 256, 0, st>>>(x, out, a.tokens, r.topk, nvec, (int)segs, a.out_rows, scale, a.out_scale, a.row_idx,
+                                                           valid_rows, move_blocks);
+  return check_launch("moe_route (copy)");
+}
+
+template <typename IdT, typename T, typename ST, int ITERS>
+int launch_route_quant_iters(const b200q_moe_route_args& a, const RouteIds& r, int threads, int32_t* row_src, int32_t* valid_rows, cudaStream_t st) {
+  const T* x = static_cast<const T*>(a.x);
+  const ST* sm = static_cast<const ST*>(a.scale);
+  int8_t* out = static_cast<int8_t*>(a.out);
+  if (r.n <= kDirectIds) {
+    moe_quant_direct_kernel<IdT, T, ST, ITERS><<<(unsigned)(r.n + 1), threads, 0, st>>>(r, x, a.hidden, sm, (int)a.scale_rows, out, a.out_scale,
+                                                                                        a.row_idx, a.row_src, a.expert_tokens, a.cumulative);
+    return check_launch("moe_route (quantised, few tokens)");
+  }
+  if (int rc = launch_sort<IdT>(r, a.row_idx, row_src, a.expert_tokens, a.cumulative, valid_rows, st)) return rc;
+  int per_sm = 1;
+  cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, moe_quant_kernel<IdT, T, ST, ITERS>, threads, 0);
+  const int64_t cap = (int64_t)sm_count() * (per_sm > 0 ? per_sm : 1);
+  moe_quant_kernel<IdT, T, ST, ITERS><<<(unsigned)(r.n < cap ? r.n : cap), threads, 0, st>>>(r, x, a.hidden, sm, (int)a.scale_rows, out, a.out_scale,
+                                                                                             row_src);
+  return check_launch("moe_route (quantised)");
+}
+
+template <typename IdT, typename T, typename ST>
+int launch_route_quant(const b200q_moe_route_args& a, const RouteIds& r, int32_t* row_src, int32_t* valid_rows, cudaStream_t st) {
+  const bool vec = a.hidden % 8 == 0 && a.hidden > 0 && a.hidden <= 8 * 512 * 4 && aligned(a.x, 16) && aligned(a.out, 8) &&
+                   (a.scale == nullptr || aligned(a.scale, 16));
+  if (!vec) return launch_route_quant_iters<IdT, T, ST, 0>(a, r, 256, row_src, valid_rows, st);
+  const int nvec = (int)(a.hidden / 8);
+  int iters = 1;
+  while (iters < 4 && nvec > iters * 256) iters *= 2;
+  const int threads = (int)ceil_div(ceil_div(nvec, iters), 32) * 32;
+  switch (iters) {
+    case 1: return launch_route_quant_iters<IdT, T, ST, 1>(a, r, threads, row_src, valid_rows, st);
+    case 2: return launch_route_quant_iters<IdT, T, ST, 2>(a, r, threads, row_src, valid_rows, st);
+    default: return launch_route_quant_iters<IdT, T, ST, 4>(a, r, threads, row_src, valid_rows, st);
+  }
+}
+
+template <typename IdT>
+int route(const b200q_moe_route_args& a, const RouteIds& r, int32_t* row_src, int32_t* valid_rows, cudaStream_t st) {
+  if (!a.quantise) {
+    const int64_t bytes = a.hidden * element_bytes(a.x_dtype);
+    switch (chunk_bytes(bytes, {a.x, a.out})) {
+      case 16: return launch_copy<IdT, 16>(a, r, bytes, valid_rows, st);
+      case 8: return launch_copy<IdT, 8>(a, r, bytes, valid_rows, st);
+      case 4: return launch_copy<IdT, 4>(a, r, bytes, valid_rows, st);
+      case 2: return launch_copy<IdT, 2>(a, r, bytes, valid_rows, st);
+      default: return launch_copy<IdT, 1>(a, r, bytes, valid_rows, st);
+    }
+  }
+  const bool f32 = a.scale == nullptr || a.scale_dtype == B200Q_F32;
+  if (a.x_dtype == B200Q_BF16)
+    return f32 ? launch_route_quant<IdT, __nv_bfloat16, float>(a, r, row_src, valid_rows, st)
+               : launch_route_quant<IdT, __nv_bfloat16, __nv_bfloat16>(a, r, row_src, valid_rows, st);
+  return f32 ? launch_route_quant<IdT, __half, float>(a, r, row_src, valid_rows, st)
+             : launch_route_quant<IdT, __half, __half>(a, r, row_src, valid_rows, st);
+}
+
+// [valid rows: 1 word, padded to 256 bytes][row -> assignment: n words, quantised form only]
+size_t route_workspace(int64_t n, int quantise) {
+  if (n <= kDirectIds) return 0;
+  return 256 + (quantise ? (size_t)n * 4 : 0);
+}
+
+template <typename T, bool VEC>
+int launch_combine(const void* rows, int64_t num_rows, const int32_t* row_idx, const void* w, int w_dtype, void* out, int64_t tokens, int topk,
+                   int64_t hidden, cudaStream_t st) {
+  const int64_t nvec = hidden / Lanes<T, VEC>::N, blocks = ceil_div(tokens * nvec, 256);
+  B200Q_REQUIRE(blocks <= 0x7fffffffLL, B200Q_ERR_UNSUPPORTED, "moe_combine: too many tokens");
+  const T* r = static_cast<const T*>(rows);
+  T* o = static_cast<T*>(out);
+#define B200Q_COMBINE(KC) moe_combine_kernel<T, VEC, KC><<<(unsigned)blocks, 256, 0, st>>>(r, num_rows, row_idx, w, w_dtype, o, tokens, topk, nvec)
+  if (topk == 1) B200Q_COMBINE(1);
+  else if (topk == 2) B200Q_COMBINE(2);
+  else if (topk <= 4) B200Q_COMBINE(4);
+  else B200Q_COMBINE(8);
+#undef B200Q_COMBINE
+  return check_launch("moe_combine");
+}
+
+template <typename T>
+int combine(const void* rows, int64_t num_rows, const int32_t* row_idx, const void* w, int w_dtype, void* out, int64_t tokens, int topk,
+            int64_t hidden, cudaStream_t st) {
+  if (chunk_bytes(hidden * (int)sizeof(T), {rows, out}) == 16)
+    return launch_combine<T, true>(rows, num_rows, row_idx, w, w_dtype, out, tokens, topk, hidden, st);
+  return launch_combine<T, false>(rows, num_rows, row_idx, w, w_dtype, out, tokens, topk, hidden, st);
+}
+
+template <typename T, bool VEC>
+int launch_combine_grad(const b200q_moe_combine_grad_args& a, cudaStream_t st) {
+  using L = Lanes<T, VEC>;
+  const int64_t nvec = a.hidden / L::N;
+  const T* dy = static_cast<const T*>(a.dy);
+  const T* rows = static_cast<const T*>(a.rows);
+  T* drows = static_cast<T*>(a.drows);
+  uint32_t* marks = static_cast<uint32_t*>(a.workspace);
+  cudaError_t err = cudaMemsetAsync(marks, 0, (size_t)ceil_div(a.num_rows, 32) * 4, st);
+  if (err != cudaSuccess) return fail(B200Q_ERR_LAUNCH, "moe_combine_grad: memset: %s", cudaGetErrorString(err));
+  if (a.tokens > 0) {
+    const int threads = nvec >= 256 ? 256 : (int)(nvec <= 32 ? 32 : ceil_div(nvec, 32) * 32);
+#define B200Q_COMBINE_GRAD(KC)                                                                                                       \
+  moe_combine_grad_kernel<T, VEC, KC><<<(unsigned)a.tokens, threads, 0, st>>>(dy, rows, a.num_rows, a.row_idx, a.weights, a.weight_dtype, \
+                                                                              drows, a.dweights, marks, (int)a.topk, nvec)
+    if (a.topk == 1) B200Q_COMBINE_GRAD(1);
+    else if (a.topk == 2) B200Q_COMBINE_GRAD(2);
+    else if (a.topk <= 4) B200Q_COMBINE_GRAD(4);
+    else B200Q_COMBINE_GRAD(8);
+#undef B200Q_COMBINE_GRAD
+    if (int rc = check_launch("moe_combine_grad")) return rc;
+  }
+  using VT = typename L::Raw;
+  const int64_t want = ceil_div(a.num_rows, 8), cap = (int64_t)sm_count() * 4;
+  moe_clear_rows_kernel<VT><<<(unsigned)(want < cap ? want : cap), 256, 0, st>>>(marks, static_cast<VT*>(a.drows), a.num_rows, nvec);
+  return check_launch("moe_combine_grad (rows without an owner)");
+}
+
+template <typename T>
+int combine_grad(const b200q_moe_combine_grad_args& a, cudaStream_t st) {
+  const bool rows_ok = a.rows == nullptr || aligned(a.rows, 16);
+  if (rows_ok && chunk_bytes(a.hidden * (int)sizeof(T), {a.dy, a.drows}) == 16) return launch_combine_grad<T, true>(a, st);
+  return launch_combine_grad<T, false>(a, st);
+}
+
+bool float_dtype(int d) { return d == B200Q_BF16 || d == B200Q_F16 || d == B200Q_F32; }
+
+}  // namespace
+}  // namespace b200q
+
+extern "C" size_t b200q_moe_route_workspace_bytes(int64_t assignments, int quantise) {
+  return assignments > 0 ? b200q::route_workspace(assignments, quantise) : 0;
+}
+
+extern "C" int b200q_moe_route(const b200q_moe_route_args* a, void* stream) {
+  using namespace b200q;
+  clear_error();
+  B200Q_REQUIRE(a != nullptr, B200Q_ERR_BAD_ARG, "moe_route: args is NULL");
+  B200Q_REQUIRE(a->tokens >= 0 && a->topk >= 0 && a->hidden >= 0 && a->out_rows >= 0, B200Q_ERR_BAD_ARG, "moe_route: negative size");
+  B200Q_REQUIRE(a->topk <= 1024 && a->tokens <= 0x7fffffffLL && a->tokens * a->topk < 0x7fffffffLL && a->hidden <= (1LL << 28),
+                B200Q_ERR_UNSUPPORTED, "moe_route: more than 2^31-2 assignments, 1024 slots or 2^28 columns");
+  B200Q_REQUIRE(a->idx_dtype == B200Q_I32 || a->idx_dtype == B200Q_I64, B200Q_ERR_UNSUPPORTED, "moe_route: expert indices must be i32 or i64");
+  B200Q_REQUIRE(a->expert_end > a->expert_begin && a->expert_end - a->expert_begin <= kMaxExperts, B200Q_ERR_UNSUPPORTED,
+                "moe_route: the expert range must hold 1 to %d experts", kMaxExperts);
+  const int64_t n = a->tokens * a->topk;
+  if (a->quantise) {
+    B200Q_REQUIRE(a->x_dtype == B200Q_BF16 || a->x_dtype == B200Q_F16, B200Q_ERR_UNSUPPORTED, "moe_route: quantised rows need a bf16 or f16 x");
+    B200Q_REQUIRE(a->scale == nullptr || a->scale_dtype == B200Q_F32 || a->scale_dtype == a->x_dtype, B200Q_ERR_UNSUPPORTED,
+                  "moe_route: smooth scales must be f32 or x's dtype");
+    B200Q_REQUIRE(a->scale == nullptr || a->scale_rows == 1 || a->scale_rows == a->expert_end - a->expert_begin, B200Q_ERR_BAD_ARG,
+                  "moe_route: smooth scales need one row, or one for each expert of the range");
+    B200Q_REQUIRE(a->out_rows == n, B200Q_ERR_BAD_ARG, "moe_route: the quantised form writes every row (out_rows = tokens * topk)");
+  } else {
+    B200Q_REQUIRE(element_bytes(a->x_dtype) != 0, B200Q_ERR_UNSUPPORTED, "moe_route: unsupported dtype of x");
+    B200Q_REQUIRE(a->out_rows <= n, B200Q_ERR_BAD_ARG, "moe_route: out_rows is larger than tokens * topk");
+    B200Q_REQUIRE((a->scale == nullptr) == (a->out_scale == nullptr) && (a->scale == nullptr || a->scale_dtype == B200Q_F32), B200Q_ERR_BAD_ARG,
+                  "moe_route: a token's scale (f32) needs out_scale, and the other way round");
+  }
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (n == 0) {
+    if (a->expert_tokens != nullptr) {
+      cudaError_t e = cudaMemsetAsync(a->expert_tokens, 0, (size_t)(a->expert_end - a->expert_begin) * 8, st);
+      if (e != cudaSuccess) return fail(B200Q_ERR_LAUNCH, "moe_route: %s", cudaGetErrorString(e));
+    }
+    return B200Q_OK;
+  }
+  B200Q_REQUIRE(a->expert_idx != nullptr && a->row_idx != nullptr, B200Q_ERR_BAD_ARG, "moe_route: expert_idx or row_idx is NULL");
+  B200Q_REQUIRE(a->hidden == 0 || (a->x != nullptr && (a->out != nullptr || a->out_rows == 0)), B200Q_ERR_BAD_ARG, "moe_route: x or out is NULL");
+  B200Q_REQUIRE(!a->quantise || a->out_scale != nullptr, B200Q_ERR_BAD_ARG, "moe_route: out_scale is NULL");
+  const int es = a->quantise ? 2 : element_bytes(a->x_dtype);
+  B200Q_REQUIRE(aligned(a->x, es) && aligned(a->out, a->quantise ? 1 : es) && aligned(a->expert_idx, a->idx_dtype == B200Q_I64 ? 8 : 4) &&
+                    aligned(a->row_idx, 4) && aligned(a->row_src, 4) && aligned(a->expert_tokens, 8) && aligned(a->out_scale, 4) &&
+                    aligned(a->scale, a->scale == nullptr || a->scale_dtype == B200Q_F32 ? 4 : 2),
+                B200Q_ERR_BAD_ARG, "moe_route: misaligned buffer");
+  const size_t need = route_workspace(n, a->quantise);
+  B200Q_REQUIRE(need == 0 || (a->workspace != nullptr && a->workspace_bytes >= need && aligned(a->workspace, 256)), B200Q_ERR_WORKSPACE,
+                "moe_route: needs %zu bytes of 256-byte aligned workspace, got %zu", need, a->workspace_bytes);
+  int32_t* valid_rows = static_cast<int32_t*>(a->workspace);
+  int32_t* row_src = a->row_src != nullptr || !a->quantise || need == 0 ? a->row_src
+                                                                         : reinterpret_cast<int32_t*>(static_cast<uint8_t*>(a->workspace) + 256);
+  RouteIds r{a->expert_idx, n, a->expert_begin, (int)(a->expert_end - a->expert_begin), (int)a->topk, a->strict ? (int)a->expert_end : 0};
+  return a->idx_dtype == B200Q_I64 ? route<int64_t>(*a, r, row_src, valid_rows, st) : route<int32_t>(*a, r, row_src, valid_rows, st);
+}
+
+extern "C" int b200q_moe_combine(const void* rows, int dtype, int64_t num_rows, const int32_t* row_idx, const void* weights, int weight_dtype,
+                                 void* out, int64_t tokens, int64_t topk, int64_t hidden, void* stream) {
+  using namespace b200q;
+  clear_error();
+  B200Q_REQUIRE(num_rows >= 0 && tokens >= 0 && topk >= 1 && hidden >= 0, B200Q_ERR_BAD_ARG, "moe_combine: negative size, or no slot");
+  B200Q_REQUIRE(float_dtype(dtype), B200Q_ERR_UNSUPPORTED, "moe_combine: rows must be bf16, f16 or f32 (dtype enum %d)", dtype);
+  B200Q_REQUIRE(weights == nullptr || float_dtype(weight_dtype), B200Q_ERR_UNSUPPORTED, "moe_combine: weights must be bf16, f16 or f32");
+  B200Q_REQUIRE(topk <= 1024 && tokens <= 0x7fffffffLL && num_rows <= 0x7fffffffLL && hidden <= (1LL << 28), B200Q_ERR_UNSUPPORTED,
+                "moe_combine: size out of range");
+  if (tokens == 0 || hidden == 0) return B200Q_OK;
+  B200Q_REQUIRE((rows != nullptr || num_rows == 0) && row_idx != nullptr && out != nullptr, B200Q_ERR_BAD_ARG, "moe_combine: NULL buffer");
+  const int es = element_bytes(dtype);
+  B200Q_REQUIRE(aligned(rows, es) && aligned(out, es) && aligned(row_idx, 4) && (weights == nullptr || aligned(weights, element_bytes(weight_dtype))),
+                B200Q_ERR_BAD_ARG, "moe_combine: misaligned buffer");
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (dtype == B200Q_BF16) return combine<__nv_bfloat16>(rows, num_rows, row_idx, weights, weight_dtype, out, tokens, (int)topk, hidden, st);
+  if (dtype == B200Q_F16) return combine<__half>(rows, num_rows, row_idx, weights, weight_dtype, out, tokens, (int)topk, hidden, st);
+  return combine<float>(rows, num_rows, row_idx, weights, weight_dtype, out, tokens, (int)topk, hidden, st);
+}
+
+extern "C" size_t b200q_moe_combine_grad_workspace_bytes(int64_t num_rows) {
+  return num_rows > 0 ? ((size_t)b200q::ceil_div(num_rows, 32) * 4 + 255) & ~size_t(255) : 0;
+}
+
+extern "C" int b200q_moe_combine_grad(const b200q_moe_combine_grad_args* a, void* stream) {
+  using namespace b200q;
+  clear_error();
+  B200Q_REQUIRE(a != nullptr, B200Q_ERR_BAD_ARG, "moe_combine_grad: args is NULL");
+  B200Q_REQUIRE(a->num_rows >= 0 && a->tokens >= 0 && a->topk >= 1 && a->hidden >= 0, B200Q_ERR_BAD_ARG,
+                "moe_combine_grad: negative size, or no slot");
+  B200Q_REQUIRE(float_dtype(a->dtype), B200Q_ERR_UNSUPPORTED, "moe_combine_grad: rows must be bf16, f16 or f32 (dtype enum %d)", a->dtype);
+  B200Q_REQUIRE((a->weights == nullptr && a->dweights == nullptr) || float_dtype(a->weight_dtype), B200Q_ERR_UNSUPPORTED,
+                "moe_combine_grad: weights must be bf16, f16 or f32");
+  B200Q_REQUIRE(a->topk <= 1024 && a->tokens <= 0x7fffffffLL && a->num_rows <= 0x7fffffffLL && a->hidden <= (1LL << 28), B200Q_ERR_UNSUPPORTED,
+                "moe_combine_grad: size out of range");
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (a->num_rows == 0 || a->hidden == 0) {
+    if (a->dweights != nullptr && a->tokens > 0) {
+      cudaError_t e = cudaMemsetAsync(a->dweights, 0, (size_t)(a->tokens * a->topk) * element_bytes(a->weight_dtype), st);
+      if (e != cudaSuccess) return fail(B200Q_ERR_LAUNCH, "moe_combine_grad: %s", cudaGetErrorString(e));
+    }
+    return B200Q_OK;
+  }
+  B200Q_REQUIRE(a->drows != nullptr && (a->tokens == 0 || (a->dy != nullptr && a->row_idx != nullptr)) &&
+                    (a->dweights == nullptr || a->rows != nullptr || a->tokens == 0),
+                B200Q_ERR_BAD_ARG, "moe_combine_grad: NULL buffer");
+  const int es = element_bytes(a->dtype), ws = element_bytes(a->weight_dtype);
+  B200Q_REQUIRE(aligned(a->dy, es) && aligned(a->rows, es) && aligned(a->drows, es) && aligned(a->row_idx, 4) &&
+                    (ws == 0 || (aligned(a->weights, ws) && aligned(a->dweights, ws))),
+                B200Q_ERR_BAD_ARG, "moe_combine_grad: misaligned buffer");
+  const size_t need = b200q_moe_combine_grad_workspace_bytes(a->num_rows);
+  B200Q_REQUIRE(a->workspace != nullptr && a->workspace_bytes >= need && aligned(a->workspace, 256), B200Q_ERR_WORKSPACE,
+                "moe_combine_grad: needs %zu bytes of 256-byte aligned workspace, got %zu", need, a->workspace_bytes);
+  if (a->dtype == B200Q_BF16) return combine_grad<__nv_bfloat16>(*a, st);
+  if (a->dtype == B200Q_F16) return combine_grad<__half>(*a, st);
+  return combine_grad<float>(*a, st);
+}

@@ -24,6 +24,8 @@ enum DeviceErrorCode : unsigned int {
   kDevTimeoutBarrier = 0x104,    // cross-rank barrier: a peer's flag did not arrive in time
   kDevTimeoutSelfTest = 0x1FF,   // the wait self-test (b200q_selftest_expire_wait) ran out, as it should
   kDevInt4Range = 0x201,         // npu_convert_weight_to_int4pack met a value outside [-8, 7]
+  kDevExpertRange = 0x202,       // npu_moe_token_permute met an expert index of 1024 or more
+  kDevRowTwice = 0x203,          // gradient of npu_moe_token_unpermute: sorted_indices names a row twice
 };
 
 // Records the first error of the device (later ones keep the first code).

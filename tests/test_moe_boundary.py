@@ -1,0 +1,133 @@
+"""Host-side checks of the mixture-of-experts block operators that need no GPU: shape contracts on meta tensors, refusals
+of arguments, and the C ABI's argument checks (every call fails, or has nothing to do, before it touches the device)."""
+import ctypes as C
+
+import pytest
+import torch
+
+from pytorch_b200 import _cabi as cabi
+
+
+@pytest.fixture(scope="module")
+def pkg():
+    import pytorch_b200
+    return pytorch_b200
+
+
+@pytest.fixture(scope="module")
+def lib():
+    return cabi.lib()
+
+
+def meta(*shape, dtype=torch.bfloat16):
+    return torch.empty(*shape, dtype=dtype, device="meta")
+
+
+I32, I64, F32 = torch.int32, torch.int64, torch.float32
+
+
+def test_routing_meta_contract(pkg):
+    q, place, tokens, scale = pkg.npu_moe_init_routing_v2(meta(10, 64), meta(10, 4, dtype=I32), scale=meta(16, 64, dtype=F32), expert_num=16, quant_mode=1)
+    assert q.shape == (40, 64) and q.dtype == torch.int8 and place.shape == (40,) and place.dtype == I32
+    assert tokens.shape == (16,) and tokens.dtype == I64 and scale.shape == (40,) and scale.dtype == F32
+    r, _, tokens, scale = pkg.npu_moe_init_routing_v2(meta(10, 64), meta(10, 4, dtype=I64), expert_num=16, active_expert_range=[4, 10])
+    assert r.shape == (40, 64) and r.dtype == torch.bfloat16 and tokens.shape == (6,) and scale.shape == (0,)
+    for kw, what in [(dict(expert_num=0), "expert_num"), (dict(expert_num=2000), "at most 1024"), (dict(expert_num=8, quant_mode=0), "quant_mode"),
+                     (dict(expert_num=8, drop_pad_mode=1), "drop_pad_mode"), (dict(expert_num=8, expert_tokens_num_type=2), "expert_tokens_num_type"),
+                     (dict(expert_num=8, active_num=7), "active_num"), (dict(expert_num=8, row_idx_type=2), "row_idx_type"),
+                     (dict(expert_num=8, active_expert_range=[3, 9]), "active_expert_range"), (dict(expert_num=8, offset=meta(8)), "offset"),
+                     (dict(expert_num=8, quant_mode=1, scale=meta(7, 64, dtype=F32)), "smooth scales"), (dict(expert_num=8, scale=meta(9, dtype=F32)), "scale must be")]:
+        with pytest.raises(RuntimeError, match=what):
+            pkg.npu_moe_init_routing_v2(meta(10, 64), meta(10, 4, dtype=I32), **kw)
+    with pytest.raises(RuntimeError, match="tokens, topk"):
+        pkg.npu_moe_init_routing_v2(meta(10, 64), meta(9, 4, dtype=I32), expert_num=8)
+    with pytest.raises(RuntimeError, match="int32 or int64"):
+        pkg.npu_moe_init_routing_v2(meta(10, 64), meta(10, 4, dtype=F32), expert_num=8)
+
+
+def test_permute_and_unpermute_meta_contract(pkg):
+    rows, place = pkg.npu_moe_token_permute(meta(10, 64), meta(10, 4, dtype=I64))
+    assert rows.shape == (40, 64) and place.shape == (40,) and place.dtype == I32
+    assert pkg.npu_moe_token_permute(meta(10, 64), meta(10, dtype=I32), 7)[0].shape == (7, 64)
+    assert pkg.npu_moe_token_permute(meta(10, 64), meta(10, 2, dtype=I32), 100)[0].shape == (20, 64)
+    assert pkg.npu_moe_token_permute(meta(10, 64), meta(10, 2, dtype=I32), -3)[0].shape == (17, 64)
+    y = pkg.npu_moe_token_unpermute(rows, place, meta(10, 4, dtype=F32))
+    assert y.shape == (10, 64) and y.dtype == torch.bfloat16
+    assert pkg.npu_moe_token_unpermute(rows, place).shape == (40, 64)
+    d, w = pkg.npu_moe_token_unpermute_grad(rows, y, place, meta(10, 4, dtype=F32))
+    assert d.shape == rows.shape and w.shape == (10, 4) and w.dtype == F32
+    assert pkg.npu_moe_token_permute_grad(meta(10, 64), rows, meta(10, 4, dtype=I64), place).shape == (10, 64)
+    with pytest.raises(RuntimeError, match="padded_mode"):
+        pkg.npu_moe_token_permute(meta(10, 64), meta(10, 4, dtype=I64), None, True)
+    with pytest.raises(RuntimeError, match="num_tokens"):
+        pkg.npu_moe_token_permute(meta(10, 64), meta(11, 4, dtype=I64))
+    with pytest.raises(RuntimeError, match="padded_mode"):
+        pkg.npu_moe_token_unpermute(rows, place, None, False, [10, 64])
+    with pytest.raises(RuntimeError, match="int32"):
+        pkg.npu_moe_token_unpermute(rows, meta(40, dtype=I64))
+    with pytest.raises(RuntimeError, match="do not match"):
+        pkg.npu_moe_token_unpermute(rows, place, meta(10, 3, dtype=F32))
+    with pytest.raises(RuntimeError, match="grad_unpermuted_tokens"):
+        pkg.npu_moe_token_unpermute_grad(rows, meta(10, 32), place, meta(10, 4, dtype=F32))
+    with pytest.raises(NotImplementedError):
+        pkg.npu_moe_token_permute(torch.zeros(2, 8), torch.zeros(2, 1, dtype=I32))
+
+
+def test_route_argument_checks(lib):
+    last = lambda: lib.b200q_last_error().decode()  # noqa: E731
+    assert lib.b200q_moe_route(None, None) == cabi.ERR_BAD_ARG
+    buf = (C.c_uint8 * 4096)()
+    p = C.addressof(buf) + (-C.addressof(buf)) % 256
+
+    def args(**kw):
+        a = cabi.MoeRouteArgs()
+        a.x, a.x_dtype, a.expert_idx, a.idx_dtype, a.tokens, a.topk, a.hidden = p, cabi.BF16, p, cabi.I32, 4, 2, 8
+        a.expert_begin, a.expert_end, a.out, a.out_rows, a.row_idx = 0, 8, p, 8, p
+        for k, v in kw.items():
+            setattr(a, k, v)
+        return C.byref(a)
+
+    for kw, status, what in [
+            (dict(tokens=-1), cabi.ERR_BAD_ARG, "negative"), (dict(topk=2000), cabi.ERR_UNSUPPORTED, "1024 slots"),
+            (dict(tokens=2 ** 31), cabi.ERR_UNSUPPORTED, "assignments"), (dict(idx_dtype=cabi.F32), cabi.ERR_UNSUPPORTED, "i32 or i64"),
+            (dict(expert_end=2000), cabi.ERR_UNSUPPORTED, "1 to 1024"), (dict(expert_end=0), cabi.ERR_UNSUPPORTED, "1 to 1024"),
+            (dict(out_rows=9), cabi.ERR_BAD_ARG, "out_rows"), (dict(x_dtype=cabi.I64), cabi.ERR_UNSUPPORTED, "dtype"),
+            (dict(scale=p, scale_dtype=cabi.F32), cabi.ERR_BAD_ARG, "out_scale"), (dict(expert_idx=None), cabi.ERR_BAD_ARG, "NULL"),
+            (dict(x=None), cabi.ERR_BAD_ARG, "NULL"), (dict(x=p + 1), cabi.ERR_BAD_ARG, "misaligned"), (dict(row_idx=p + 2), cabi.ERR_BAD_ARG, "misaligned"),
+            (dict(quantise=1, x_dtype=cabi.F32), cabi.ERR_UNSUPPORTED, "bf16 or f16"), (dict(quantise=1, out_rows=7, out_scale=p), cabi.ERR_BAD_ARG, "every row"),
+            (dict(quantise=1), cabi.ERR_BAD_ARG, "out_scale"),
+            (dict(quantise=1, out_scale=p, scale=p, scale_dtype=cabi.F32, scale_rows=3), cabi.ERR_BAD_ARG, "one row"),
+            (dict(tokens=2000, out_rows=4000), cabi.ERR_WORKSPACE, "workspace")]:
+        assert lib.b200q_moe_route(args(**kw), None) == status and what in last(), (kw, last())
+    assert lib.b200q_moe_route(args(tokens=0, out_rows=0), None) == cabi.OK
+    assert lib.b200q_moe_route_workspace_bytes(2048, 1) == 0 and lib.b200q_moe_route_workspace_bytes(0, 1) == 0
+    assert lib.b200q_moe_route_workspace_bytes(4096, 1) == 256 + 4 * 4096 and lib.b200q_moe_route_workspace_bytes(4096, 0) == 256
+
+
+def test_combine_argument_checks(lib):
+    last = lambda: lib.b200q_last_error().decode()  # noqa: E731
+    buf = (C.c_uint8 * 4096)()
+    p = C.addressof(buf) + (-C.addressof(buf)) % 256
+
+    def fwd(rows=p, dtype=cabi.BF16, n=4, idx=p, w=None, wd=cabi.NONE, out=p, t=2, k=2, h=8):
+        return lib.b200q_moe_combine(rows, dtype, n, idx, w, wd, out, t, k, h, None)
+
+    assert fwd(dtype=cabi.I8) == cabi.ERR_UNSUPPORTED and fwd(k=0) == cabi.ERR_BAD_ARG and fwd(t=-1) == cabi.ERR_BAD_ARG
+    assert fwd(w=p, wd=cabi.I32) == cabi.ERR_UNSUPPORTED and "weights" in last()
+    assert fwd(k=2000) == cabi.ERR_UNSUPPORTED and fwd(rows=None) == cabi.ERR_BAD_ARG and fwd(out=p + 1) == cabi.ERR_BAD_ARG
+    assert fwd(t=0) == cabi.OK and fwd(h=0) == cabi.OK
+
+    def bwd(**kw):
+        a = cabi.MoeCombineGradArgs()
+        a.dy, a.dtype, a.rows, a.num_rows, a.row_idx, a.weight_dtype = p, cabi.BF16, p, 4, p, cabi.NONE
+        a.tokens, a.topk, a.hidden, a.drows, a.workspace, a.workspace_bytes = 2, 2, 8, p, p, 256
+        for k, v in kw.items():
+            setattr(a, k, v)
+        return lib.b200q_moe_combine_grad(C.byref(a), None)
+
+    assert lib.b200q_moe_combine_grad(None, None) == cabi.ERR_BAD_ARG
+    assert bwd(dtype=cabi.I8) == cabi.ERR_UNSUPPORTED and bwd(topk=0) == cabi.ERR_BAD_ARG
+    assert bwd(dweights=p) == cabi.ERR_UNSUPPORTED and bwd(dweights=p, weight_dtype=cabi.F32, rows=None) == cabi.ERR_BAD_ARG
+    assert bwd(workspace_bytes=0) == cabi.ERR_WORKSPACE and bwd(workspace=p + 16) == cabi.ERR_WORKSPACE
+    assert bwd(drows=None) == cabi.ERR_BAD_ARG and bwd(num_rows=0) == cabi.OK
+    assert lib.b200q_moe_combine_grad_workspace_bytes(33) == 256 and lib.b200q_moe_combine_grad_workspace_bytes(0) == 0
