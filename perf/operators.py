@@ -213,6 +213,8 @@ def prepare(case, seed):
 # ------------------------------------------------------------------------------------------------ one pass
 def run(s):
     case = s["case"]
+    if own:
+        import pytorch_b200  # noqa: F401  (registers torch.ops.npu)
     return (_own if own else _plain)[case["op"]](s, case)
 
 
