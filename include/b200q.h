@@ -308,6 +308,53 @@ typedef struct {
 size_t b200q_moe_combine_grad_workspace_bytes(int64_t num_rows);
 int b200q_moe_combine_grad(const b200q_moe_combine_grad_args* args, void* stream);
 
+/* npu_gated_add_rms_norm: the norm after a block, its gate and residual scale, and the norm before the next block.
+ *   z = x * rsqrt(mean(x^2) + epsilon) * post_gamma   (x itself without post_gamma)
+ *   h = residual_scale * residual + gate * z
+ *   y = h * rsqrt(mean(h^2) + epsilon) * gamma
+ * all in fp32, y and h rounded once.  With `scale` (the _dynamic_quant form) y is int8: y * smooth quantised per row as
+ * b200q_dynamic_quant. */
+typedef struct {
+  const void* x;            /* [rows, width] bf16, f16 or f32; width at most 16384                          */
+  const void* residual;     /* the same                                                                     */
+  int dtype;
+  const void* gamma;        /* [width]                                                                      */
+  int gamma_dtype;
+  const void* post_gamma;   /* [width] or NULL                                                              */
+  int post_gamma_dtype;
+  const void* gate;         /* [ceil(rows / gate_rows), width] (gate_per_row 0) or [rows] (1), or NULL      */
+  int gate_dtype;
+  int gate_per_row;         /* one value a row; gate_rows is then 1                                         */
+  int64_t gate_rows;        /* consecutive rows that share a gate                                           */
+  float residual_scale, epsilon;
+  int64_t rows, width;
+  const void* smooth;       /* quantised form: [width] or NULL                                              */
+  int smooth_dtype;
+  void* y;                  /* [rows, width], x's dtype or int8                                             */
+  void* h;                  /* [rows, width], x's dtype                                                     */
+  float* scale;             /* [rows]: not NULL asks for the quantised form                                 */
+  float* rstd;              /* [rows] 1 / rms of h, or NULL; read by the gradient                           */
+  float* post_rstd;         /* [rows] 1 / rms of x, or NULL; read by the gradient                           */
+} b200q_gated_norm_args;
+
+typedef struct {
+  const void* dy;           /* [rows, width], x's dtype (as all of [rows, width])                           */
+  const void* dh;           /* the gradient that reaches h directly, or NULL                                */
+  void* dx;
+  void* dresidual;
+  void* dgamma;             /* [width], gamma's dtype                                                       */
+  void* dpost_gamma;        /* [width], post_gamma's dtype; unused without post_gamma                       */
+  void* dgate;              /* gate's shape and dtype; unused without gate                                  */
+  void* workspace;          /* >= b200q_gated_norm_grad_workspace_bytes(), 256-byte aligned                 */
+  size_t workspace_bytes;
+} b200q_gated_norm_grads;
+
+int b200q_gated_norm(const b200q_gated_norm_args* args, void* stream);
+/* Gradient; of args it reads x, residual, the parameters, residual_scale, rstd and post_rstd.  Sums over rows are added
+ * in fp32 in a fixed order. */
+size_t b200q_gated_norm_grad_workspace_bytes(const b200q_gated_norm_args* args);
+int b200q_gated_norm_grad(const b200q_gated_norm_args* args, const b200q_gated_norm_grads* grads, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -70,3 +70,44 @@ def combine_grad(dy: torch.Tensor, rows: torch.Tensor, row_idx: torch.Tensor, we
     terms = rows.to(F64)[idx[t, k]] * dy.to(F64)[t]
     dw[t, k], size[t, k] = terms.sum(1), terms.abs().sum(1)
     return drows, dw, size
+
+
+def gated_add_rms_norm(x, residual, gamma, post_gamma, gate, residual_scale, epsilon):
+    """``(y, h, rstd, post_rstd)`` of the norm after a block, its gate and residual scale, and the norm before the next."""
+    z = x.to(F64)
+    post_rstd = None
+    if post_gamma is not None:
+        post_rstd = 1 / torch.sqrt((z * z).mean(-1) + epsilon)
+        z = z * post_rstd[..., None] * post_gamma.to(F64)
+    h = residual_scale * residual.to(F64) + (z if gate is None else gate.to(F64) * z)
+    rstd = 1 / torch.sqrt((h * h).mean(-1) + epsilon)
+    return h * rstd[..., None] * gamma.to(F64), h, rstd, post_rstd
+
+
+def gated_add_rms_norm_grad(x, residual, gamma, post_gamma, gate, residual_scale, epsilon, dy, dh):
+    """``(gradients, bounds)`` by name.  The gradients are autograd's of the definition; a bound is the sum of the magnitudes
+    of the terms that the gradient's formula adds for one element (over rows too, where the gradient sums over rows)."""
+    named = [(n, t) for n, t in (("x", x), ("residual", residual), ("gamma", gamma), ("post_gamma", post_gamma), ("gate", gate)) if t is not None]
+    at = {n: t.detach().to(F64).requires_grad_() for n, t in named}
+    y, h, rstd, post_rstd = gated_add_rms_norm(at["x"], at["residual"], at["gamma"], at.get("post_gamma"), at.get("gate"), residual_scale, epsilon)
+    loss = (y * dy.to(F64)).sum() + (h * dh.to(F64)).sum()
+    grads = dict(zip(at, torch.autograd.grad(loss, list(at.values()))))
+    with torch.no_grad():
+        w2, hn = gamma.to(F64), h * rstd[..., None]
+        u = dy.to(F64) * w2
+        m2 = (u * hn).abs().mean(-1, keepdim=True)
+        dhs = dh.to(F64).abs() + rstd[..., None] * (u.abs() + hn.abs() * m2)
+        xn = x.to(F64) if post_gamma is None else x.to(F64) * post_rstd[..., None]
+        z = xn if post_gamma is None else xn * post_gamma.to(F64)
+        dz = dhs if gate is None else dhs * gate.to(F64).abs()
+        flat = lambda t: t.reshape(-1, x.shape[-1]).sum(0)  # noqa: E731
+        bounds = {"gamma": flat((dy.to(F64) * hn).abs()), "residual": abs(residual_scale) * dhs}
+        if gate is not None:
+            bounds["gate"] = (dhs * z.abs()).sum_to_size(gate.shape)
+        if post_gamma is None:
+            bounds["x"] = dz
+        else:
+            bounds["post_gamma"] = flat(dz * xn.abs())
+            v = dz * post_gamma.to(F64).abs()
+            bounds["x"] = post_rstd[..., None] * (v + xn.abs() * (v * xn.abs()).mean(-1, keepdim=True))
+    return grads, bounds

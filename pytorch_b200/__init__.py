@@ -34,6 +34,9 @@ OPS = (
     "npu_moe_token_permute_grad",
     "npu_moe_token_unpermute",
     "npu_moe_token_unpermute_grad",
+    "npu_gated_add_rms_norm",
+    "npu_gated_add_rms_norm_grad",
+    "npu_gated_add_rms_norm_dynamic_quant",
 )
 
 
@@ -60,6 +63,9 @@ npu_moe_token_permute = _torch.ops.npu.npu_moe_token_permute
 npu_moe_token_permute_grad = _torch.ops.npu.npu_moe_token_permute_grad
 npu_moe_token_unpermute = _torch.ops.npu.npu_moe_token_unpermute
 npu_moe_token_unpermute_grad = _torch.ops.npu.npu_moe_token_unpermute_grad
+npu_gated_add_rms_norm = _torch.ops.npu.npu_gated_add_rms_norm
+npu_gated_add_rms_norm_grad = _torch.ops.npu.npu_gated_add_rms_norm_grad
+npu_gated_add_rms_norm_dynamic_quant = _torch.ops.npu.npu_gated_add_rms_norm_dynamic_quant
 
 from . import collective_ops  # noqa: E402,F401  (defines the three collective-fused operators in torch.ops.npu)
 

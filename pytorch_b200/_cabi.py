@@ -30,6 +30,7 @@ EXPORTS = (
     "b200q_peer_barrier", "b200q_reduce_slots", "b200q_copy_columns",
     "b200q_moe_route_workspace_bytes", "b200q_moe_route", "b200q_moe_combine",
     "b200q_moe_combine_grad_workspace_bytes", "b200q_moe_combine_grad",
+    "b200q_gated_norm", "b200q_gated_norm_grad_workspace_bytes", "b200q_gated_norm_grad",
 )
 
 
@@ -90,6 +91,26 @@ class MoeCombineGradArgs(C.Structure):
     ]
 
 
+class GatedNormArgs(C.Structure):
+    _fields_ = [
+        ("x", C.c_void_p), ("residual", C.c_void_p), ("dtype", C.c_int),
+        ("gamma", C.c_void_p), ("gamma_dtype", C.c_int),
+        ("post_gamma", C.c_void_p), ("post_gamma_dtype", C.c_int),
+        ("gate", C.c_void_p), ("gate_dtype", C.c_int), ("gate_per_row", C.c_int), ("gate_rows", C.c_int64),
+        ("residual_scale", C.c_float), ("epsilon", C.c_float),
+        ("rows", C.c_int64), ("width", C.c_int64),
+        ("smooth", C.c_void_p), ("smooth_dtype", C.c_int),
+        ("y", C.c_void_p), ("h", C.c_void_p), ("scale", C.c_void_p), ("rstd", C.c_void_p), ("post_rstd", C.c_void_p),
+    ]
+
+
+class GatedNormGrads(C.Structure):
+    _fields_ = [
+        ("dy", C.c_void_p), ("dh", C.c_void_p), ("dx", C.c_void_p), ("dresidual", C.c_void_p), ("dgamma", C.c_void_p),
+        ("dpost_gamma", C.c_void_p), ("dgate", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
+    ]
+
+
 class B200QError(RuntimeError):
     def __init__(self, status: int, message: str):
         super().__init__(f"b200q status {status}: {message}")
@@ -147,6 +168,10 @@ def lib() -> C.CDLL:
         l.b200q_moe_combine_grad_workspace_bytes.restype = C.c_size_t
         l.b200q_moe_combine_grad_workspace_bytes.argtypes = [C.c_int64]
         l.b200q_moe_combine_grad.argtypes = [C.POINTER(MoeCombineGradArgs), C.c_void_p]
+        l.b200q_gated_norm.argtypes = [C.POINTER(GatedNormArgs), C.c_void_p]
+        l.b200q_gated_norm_grad_workspace_bytes.restype = C.c_size_t
+        l.b200q_gated_norm_grad_workspace_bytes.argtypes = [C.POINTER(GatedNormArgs)]
+        l.b200q_gated_norm_grad.argtypes = [C.POINTER(GatedNormArgs), C.POINTER(GatedNormGrads), C.c_void_p]
         _lib = l
     return _lib
 

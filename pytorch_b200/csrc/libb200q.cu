@@ -11,3 +11,4 @@
 #include "w4a16_gemm.cu"
 #include "peer_scatter.cu"
 #include "moe_routing.cu"
+#include "gated_norm.cu"

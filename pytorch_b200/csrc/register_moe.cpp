@@ -292,6 +292,191 @@ std::tuple<Tensor, Tensor> unpermute_grad_meta(const Tensor& rows, const Tensor&
 }
 
 // ---------------------------------------------------------------------------------------------
+// npu_gated_add_rms_norm(x, residual, gamma, *, post_gamma, gate, residual_scale, epsilon) -> (y, rstd, h, post_rstd)
+struct GateSpec {
+  bool per_row = false;
+  int64_t rows = 1;            // rows that share a gate
+};
+
+GateSpec gate_spec(const char* op, const Tensor& x, const Tensor& gate) {
+  const int64_t width = x.size(-1), rows = width ? x.numel() / width : 0, d = x.dim();
+  GateSpec s;
+  TORCH_CHECK(is_float_type(gate.scalar_type()), op, ": gate must be float16, bfloat16 or float32, got ", gate.scalar_type());
+  if (gate.dim() == 1 && gate.size(0) == width) {
+    s.rows = std::max<int64_t>(1, rows);
+    return s;
+  }
+  TORCH_CHECK(gate.dim() == d && (gate.size(-1) == width || gate.size(-1) == 1), op, ": gate ", gate.sizes(), " does not fit x ", x.sizes(),
+              " (one value a channel, a row or an element, or a row of channels for each leading index)");
+  // The leading sizes are x's up to some dimension and 1 from there on.
+  int64_t i = 0;
+  while (i + 1 < d && gate.size(i) == x.size(i)) ++i;
+  int64_t shared = 1;
+  for (int64_t j = i; j + 1 < d; ++j) {
+    TORCH_CHECK(gate.size(j) == 1, op, ": gate ", gate.sizes(), " does not fit x ", x.sizes());
+    shared *= x.size(j);
+  }
+  s.rows = std::max<int64_t>(1, shared);
+  s.per_row = gate.size(-1) == 1 && width != 1;
+  TORCH_CHECK(!s.per_row || s.rows == 1, op, ": a gate of one value a row needs x's leading sizes, got ", gate.sizes(), " for x ", x.sizes());
+  return s;
+}
+
+// Fills the arguments that both directions share; the tensors must be contiguous.
+b200q_gated_norm_args norm_args(const char* op, const Tensor& x, const Tensor& residual, const Tensor& gamma, const Tensor& post, const Tensor& gate,
+                                double residual_scale, double epsilon) {
+  b200q_gated_norm_args a{};
+  a.x = x.data_ptr(); a.residual = residual.data_ptr(); a.dtype = dtype_enum(x.scalar_type());
+  a.gamma = gamma.data_ptr(); a.gamma_dtype = dtype_enum(gamma.scalar_type());
+  if (post.defined()) { a.post_gamma = post.data_ptr(); a.post_gamma_dtype = dtype_enum(post.scalar_type()); }
+  a.gate_rows = 1;
+  if (gate.defined()) {
+    const GateSpec g = gate_spec(op, x, gate);
+    a.gate = gate.data_ptr(); a.gate_dtype = dtype_enum(gate.scalar_type());
+    a.gate_per_row = g.per_row ? 1 : 0;
+    a.gate_rows = g.rows;
+  }
+  a.residual_scale = static_cast<float>(residual_scale);
+  a.epsilon = static_cast<float>(epsilon);
+  a.width = x.size(-1);
+  a.rows = a.width ? x.numel() / a.width : 0;
+  return a;
+}
+
+void norm_check(const char* op, const Tensor& x, const Tensor& residual, const Tensor& gamma, const optional<Tensor>& post, const optional<Tensor>& gate) {
+  TORCH_CHECK(x.dim() >= 1 && is_float_type(x.scalar_type()), op, ": x must be float16, bfloat16 or float32, got ", x.scalar_type());
+  TORCH_CHECK(residual.sizes() == x.sizes() && residual.scalar_type() == x.scalar_type(), op, ": residual must have x's shape and dtype, got ",
+              residual.scalar_type(), " ", residual.sizes(), " for ", x.scalar_type(), " ", x.sizes());
+  auto vector = [&](const Tensor& v, const char* name) {
+    TORCH_CHECK(v.dim() == 1 && v.size(0) == x.size(-1) && is_float_type(v.scalar_type()), op, ": ", name, " must be a float16, bfloat16 or float32 [",
+                x.size(-1), "], got ", v.scalar_type(), " ", v.sizes());
+  };
+  vector(gamma, "gamma");
+  if (post.has_value()) vector(*post, "post_gamma");
+  if (gate.has_value()) gate_spec(op, x, *gate);
+}
+
+Tensor contiguous_or_none(const optional<Tensor>& t) { return t.has_value() ? t->contiguous() : Tensor(); }
+
+std::vector<int64_t> row_sizes(const Tensor& x) {
+  auto s = x.sizes().vec();
+  s.pop_back();
+  return s;
+}
+
+using NormOutputs = std::tuple<Tensor, Tensor, Tensor, Tensor>;
+
+NormOutputs norm_meta(const Tensor& x, const Tensor& residual, const Tensor& gamma, const optional<Tensor>& post, const optional<Tensor>& gate,
+                      double, double) {
+  norm_check("npu_gated_add_rms_norm", x, residual, gamma, post, gate);
+  const auto rows = row_sizes(x);
+  const auto f32 = x.options().dtype(at::kFloat);
+  return {at::empty(x.sizes(), x.options()), at::empty(rows, f32), at::empty(x.sizes(), x.options()),
+          post.has_value() ? at::empty(rows, f32) : at::empty({0}, f32)};
+}
+
+NormOutputs norm_cuda(const Tensor& x, const Tensor& residual, const Tensor& gamma, const optional<Tensor>& post, const optional<Tensor>& gate,
+                      double residual_scale, double epsilon) {
+  constexpr const char* op = "npu_gated_add_rms_norm";
+  const optional<Tensor> ro(residual), go(gamma);
+  check_same_device(op, x, {&ro, &go, &post, &gate});
+  c10::cuda::CUDAGuard guard(x.device());
+  surface_device_error(op, x);
+  auto [y, rstd, h, post_rstd] = norm_meta(x, residual, gamma, post, gate, residual_scale, epsilon);
+  Tensor xc = x.contiguous(), rc = residual.contiguous(), wc = gamma.contiguous(), pc = contiguous_or_none(post), gc = contiguous_or_none(gate);
+  b200q_gated_norm_args a = norm_args(op, xc, rc, wc, pc, gc, residual_scale, epsilon);
+  a.y = y.data_ptr(); a.h = h.data_ptr();
+  a.rstd = static_cast<float*>(rstd.data_ptr());
+  if (post.has_value()) a.post_rstd = static_cast<float*>(post_rstd.data_ptr());
+  check_status(b200q_gated_norm(&a, stream_of(x)), op);
+  return {y, rstd, h, post_rstd};
+}
+
+// npu_gated_add_rms_norm_dynamic_quant(x, residual, gamma, *, post_gamma, gate, smooth_scales, residual_scale, epsilon) -> (y int8, scale, h)
+std::tuple<Tensor, Tensor, Tensor> norm_quant_meta(const Tensor& x, const Tensor& residual, const Tensor& gamma, const optional<Tensor>& post,
+                                                   const optional<Tensor>& gate, const optional<Tensor>& smooth, double, double) {
+  constexpr const char* op = "npu_gated_add_rms_norm_dynamic_quant";
+  norm_check(op, x, residual, gamma, post, gate);
+  if (smooth.has_value())
+    TORCH_CHECK(smooth->dim() == 1 && smooth->size(0) == x.size(-1) && is_float_type(smooth->scalar_type()), op,
+                ": smooth_scales must be a float16, bfloat16 or float32 [", x.size(-1), "], got ", smooth->scalar_type(), " ", smooth->sizes());
+  return {at::empty(x.sizes(), x.options().dtype(at::kChar)), at::empty(row_sizes(x), x.options().dtype(at::kFloat)),
+          at::empty(x.sizes(), x.options())};
+}
+
+std::tuple<Tensor, Tensor, Tensor> norm_quant_cuda(const Tensor& x, const Tensor& residual, const Tensor& gamma, const optional<Tensor>& post,
+                                                   const optional<Tensor>& gate, const optional<Tensor>& smooth, double residual_scale,
+                                                   double epsilon) {
+  constexpr const char* op = "npu_gated_add_rms_norm_dynamic_quant";
+  const optional<Tensor> ro(residual), go(gamma);
+  check_same_device(op, x, {&ro, &go, &post, &gate, &smooth});
+  c10::cuda::CUDAGuard guard(x.device());
+  surface_device_error(op, x);
+  auto [y, scale, h] = norm_quant_meta(x, residual, gamma, post, gate, smooth, residual_scale, epsilon);
+  if (x.size(-1) == 0) return {y, scale.zero_(), h};
+  Tensor xc = x.contiguous(), rc = residual.contiguous(), wc = gamma.contiguous(), pc = contiguous_or_none(post), gc = contiguous_or_none(gate);
+  Tensor sc = contiguous_or_none(smooth);
+  b200q_gated_norm_args a = norm_args(op, xc, rc, wc, pc, gc, residual_scale, epsilon);
+  a.y = y.data_ptr(); a.h = h.data_ptr();
+  a.scale = static_cast<float*>(scale.data_ptr());
+  if (sc.defined()) { a.smooth = sc.data_ptr(); a.smooth_dtype = dtype_enum(sc.scalar_type()); }
+  if (a.rows > 0) check_status(b200q_gated_norm(&a, stream_of(x)), op);
+  return {y, scale, h};
+}
+
+// npu_gated_add_rms_norm_grad(grad_y, grad_h, x, residual, gamma, rstd, *, post_gamma, gate, post_rstd, residual_scale)
+//   -> (grad_x, grad_residual, grad_gamma, grad_post_gamma, grad_gate); what there is no parameter for is empty.
+using NormGrads = std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor>;
+
+NormGrads norm_grad_meta(const Tensor& dy, const optional<Tensor>& dh, const Tensor& x, const Tensor& residual, const Tensor& gamma, const Tensor& rstd,
+                         const optional<Tensor>& post, const optional<Tensor>& gate, const optional<Tensor>& post_rstd, double) {
+  constexpr const char* op = "npu_gated_add_rms_norm_grad";
+  norm_check(op, x, residual, gamma, post, gate);
+  const int64_t rows = x.size(-1) ? x.numel() / x.size(-1) : rstd.numel();
+  auto like_x = [&](const Tensor& t, const char* name) {
+    TORCH_CHECK(t.sizes() == x.sizes() && t.scalar_type() == x.scalar_type(), op, ": ", name, " must have x's shape and dtype, got ", t.scalar_type(), " ",
+                t.sizes());
+  };
+  auto stat = [&](const Tensor& t, const char* name) {
+    TORCH_CHECK(t.scalar_type() == at::kFloat && t.numel() == rows, op, ": ", name, " must be float32 with one value a row (", rows, "), got ",
+                t.scalar_type(), " ", t.sizes());
+  };
+  like_x(dy, "grad_y");
+  if (dh.has_value()) like_x(*dh, "grad_h");
+  stat(rstd, "rstd");
+  TORCH_CHECK(!post.has_value() || post_rstd.has_value(), op, ": post_gamma needs post_rstd");
+  if (post.has_value()) stat(*post_rstd, "post_rstd");
+  auto like = [&](const optional<Tensor>& t) { return t.has_value() ? at::empty(t->sizes(), t->options()) : at::empty({0}, x.options()); };
+  return {at::empty(x.sizes(), x.options()), at::empty(x.sizes(), x.options()), at::empty(gamma.sizes(), gamma.options()), like(post), like(gate)};
+}
+
+NormGrads norm_grad_cuda(const Tensor& dy, const optional<Tensor>& dh, const Tensor& x, const Tensor& residual, const Tensor& gamma, const Tensor& rstd,
+                         const optional<Tensor>& post, const optional<Tensor>& gate, const optional<Tensor>& post_rstd, double residual_scale) {
+  constexpr const char* op = "npu_gated_add_rms_norm_grad";
+  const optional<Tensor> xo(x), ro(residual), go(gamma), so(rstd);
+  check_same_device(op, dy, {&dh, &xo, &ro, &go, &so, &post, &gate, &post_rstd});
+  c10::cuda::CUDAGuard guard(x.device());
+  surface_device_error(op, x);
+  auto [dx, dres, dgamma, dpost, dgate] = norm_grad_meta(dy, dh, x, residual, gamma, rstd, post, gate, post_rstd, residual_scale);
+  Tensor xc = x.contiguous(), rc = residual.contiguous(), wc = gamma.contiguous(), pc = contiguous_or_none(post), gc = contiguous_or_none(gate);
+  Tensor yc = dy.contiguous(), hc = contiguous_or_none(dh), sc = rstd.contiguous(), qc = contiguous_or_none(post_rstd);
+  if (x.numel() == 0 && gate.has_value()) dgate.zero_();
+  b200q_gated_norm_args a = norm_args(op, xc, rc, wc, pc, gc, residual_scale, 0.0);
+  a.rstd = static_cast<float*>(sc.data_ptr());
+  if (post.has_value()) a.post_rstd = static_cast<float*>(qc.data_ptr());
+  Tensor ws = scratch(b200q_gated_norm_grad_workspace_bytes(&a), x);
+  b200q_gated_norm_grads g{};
+  g.dy = yc.data_ptr();
+  if (hc.defined()) g.dh = hc.data_ptr();
+  g.dx = dx.data_ptr(); g.dresidual = dres.data_ptr(); g.dgamma = dgamma.data_ptr();
+  if (post.has_value()) g.dpost_gamma = dpost.data_ptr();
+  if (gate.has_value()) g.dgate = dgate.data_ptr();
+  if (ws.defined()) { g.workspace = ws.data_ptr(); g.workspace_bytes = ws.numel(); }
+  check_status(b200q_gated_norm_grad(&a, &g, stream_of(x)), op);
+  return {dx, dres, dgamma, dpost, dgate};
+}
+
+// ---------------------------------------------------------------------------------------------
 // Autograd
 class PermuteFunction : public torch::autograd::Function<PermuteFunction> {
  public:
@@ -356,6 +541,49 @@ Tensor unpermute_autograd(const Tensor& rows, const Tensor& sorted, const option
   return UnpermuteFunction::apply(rows, sorted, probs, padded_mode, restore_shape)[0];
 }
 
+class NormFunction : public torch::autograd::Function<NormFunction> {
+ public:
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& residual, const Tensor& gamma, const optional<Tensor>& post,
+                               const optional<Tensor>& gate, double residual_scale, double epsilon) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    auto [y, rstd, h, post_rstd] = norm_cuda(x, residual, gamma, post, gate, residual_scale, epsilon);
+    ctx->set_materialize_grads(false);
+    ctx->mark_non_differentiable({rstd, post_rstd});
+    ctx->save_for_backward({x, residual, gamma, post.value_or(Tensor()), gate.value_or(Tensor()), rstd, post_rstd});
+    ctx->saved_data["residual_scale"] = residual_scale;
+    return {y, rstd, h, post_rstd};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    variable_list out(7);
+    if (!grads[0].defined() && !grads[2].defined()) return out;
+    no_second_derivative("npu_gated_add_rms_norm_grad");
+    auto s = ctx->get_saved_variables();
+    auto opt = [](const Tensor& t) { return t.defined() ? optional<Tensor>(t) : optional<Tensor>(); };
+    c10::cuda::CUDAGuard guard(s[0].device());
+    const Tensor dy = grads[0].defined() ? grads[0] : at::zeros(s[0].sizes(), s[0].options());
+    auto [dx, dres, dgamma, dpost, dgate] = norm_grad_cuda(dy, opt(grads[2]), s[0], s[1], s[2], s[5], opt(s[3]), opt(s[4]), opt(s[6]),
+                                                           ctx->saved_data["residual_scale"].toDouble());
+    out[0] = dx;
+    out[1] = dres;
+    out[2] = dgamma;
+    if (s[3].defined()) out[3] = dpost;
+    if (s[4].defined()) out[4] = dgate;
+    return out;
+  }
+};
+
+NormOutputs norm_autograd(const Tensor& x, const Tensor& residual, const Tensor& gamma, const optional<Tensor>& post, const optional<Tensor>& gate,
+                          double residual_scale, double epsilon) {
+  const bool wanted = x.requires_grad() || residual.requires_grad() || gamma.requires_grad() || (post.has_value() && post->requires_grad()) ||
+                      (gate.has_value() && gate->requires_grad());
+  if (!(at::GradMode::is_enabled() && wanted)) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    return norm_cuda(x, residual, gamma, post, gate, residual_scale, epsilon);
+  }
+  auto o = NormFunction::apply(x, residual, gamma, post, gate, residual_scale, epsilon);
+  return {o[0], o[1], o[2], o[3]};
+}
+
 }  // namespace
 
 TORCH_LIBRARY_FRAGMENT(npu, m) {
@@ -369,6 +597,13 @@ TORCH_LIBRARY_FRAGMENT(npu, m) {
         "int[]? restore_shape=None) -> Tensor");
   m.def("npu_moe_token_unpermute_grad(Tensor permuted_tokens, Tensor grad_unpermuted_tokens, Tensor sorted_indices, Tensor? probs=None, "
         "bool padded_mode=False, int[]? restore_shape=None) -> (Tensor, Tensor)");
+  m.def("npu_gated_add_rms_norm(Tensor x, Tensor residual, Tensor gamma, *, Tensor? post_gamma=None, Tensor? gate=None, "
+        "float residual_scale=1.0, float epsilon=1e-06) -> (Tensor, Tensor, Tensor, Tensor)");
+  m.def("npu_gated_add_rms_norm_dynamic_quant(Tensor x, Tensor residual, Tensor gamma, *, Tensor? post_gamma=None, Tensor? gate=None, "
+        "Tensor? smooth_scales=None, float residual_scale=1.0, float epsilon=1e-06) -> (Tensor, Tensor, Tensor)");
+  m.def("npu_gated_add_rms_norm_grad(Tensor grad_y, Tensor? grad_h, Tensor x, Tensor residual, Tensor gamma, Tensor rstd, *, "
+        "Tensor? post_gamma=None, Tensor? gate=None, Tensor? post_rstd=None, float residual_scale=1.0) "
+        "-> (Tensor, Tensor, Tensor, Tensor, Tensor)");
 }
 
 TORCH_LIBRARY_IMPL(npu, CUDA, m) {
@@ -377,11 +612,15 @@ TORCH_LIBRARY_IMPL(npu, CUDA, m) {
   m.impl("npu_moe_token_permute_grad", TORCH_FN(permute_grad_cuda));
   m.impl("npu_moe_token_unpermute", TORCH_FN(unpermute_cuda));
   m.impl("npu_moe_token_unpermute_grad", TORCH_FN(unpermute_grad_cuda));
+  m.impl("npu_gated_add_rms_norm", TORCH_FN(norm_cuda));
+  m.impl("npu_gated_add_rms_norm_dynamic_quant", TORCH_FN(norm_quant_cuda));
+  m.impl("npu_gated_add_rms_norm_grad", TORCH_FN(norm_grad_cuda));
 }
 
 TORCH_LIBRARY_IMPL(npu, AutogradCUDA, m) {
   m.impl("npu_moe_token_permute", TORCH_FN(permute_autograd));
   m.impl("npu_moe_token_unpermute", TORCH_FN(unpermute_autograd));
+  m.impl("npu_gated_add_rms_norm", TORCH_FN(norm_autograd));
 }
 
 TORCH_LIBRARY_IMPL(npu, Meta, m) {
@@ -390,4 +629,7 @@ TORCH_LIBRARY_IMPL(npu, Meta, m) {
   m.impl("npu_moe_token_permute_grad", TORCH_FN(permute_grad_meta));
   m.impl("npu_moe_token_unpermute", TORCH_FN(unpermute_meta));
   m.impl("npu_moe_token_unpermute_grad", TORCH_FN(unpermute_grad_meta));
+  m.impl("npu_gated_add_rms_norm", TORCH_FN(norm_meta));
+  m.impl("npu_gated_add_rms_norm_dynamic_quant", TORCH_FN(norm_quant_meta));
+  m.impl("npu_gated_add_rms_norm_grad", TORCH_FN(norm_grad_meta));
 }

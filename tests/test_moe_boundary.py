@@ -131,3 +131,73 @@ def test_combine_argument_checks(lib):
     assert bwd(workspace_bytes=0) == cabi.ERR_WORKSPACE and bwd(workspace=p + 16) == cabi.ERR_WORKSPACE
     assert bwd(drows=None) == cabi.ERR_BAD_ARG and bwd(num_rows=0) == cabi.OK
     assert lib.b200q_moe_combine_grad_workspace_bytes(33) == 256 and lib.b200q_moe_combine_grad_workspace_bytes(0) == 0
+
+
+def test_gated_norm_meta_contract(pkg):
+    x, w = meta(4, 6, 64), meta(64)
+    y, rstd, h, prstd = pkg.npu_gated_add_rms_norm(x, x, w, post_gamma=w, gate=meta(4, 1, 64))
+    assert y.shape == h.shape == x.shape and rstd.shape == prstd.shape == (4, 6) and rstd.dtype == F32
+    assert pkg.npu_gated_add_rms_norm(x, x, w)[3].shape == (0,)
+    q, s, h = pkg.npu_gated_add_rms_norm_dynamic_quant(x, x, w, gate=meta(4, 6, 1), smooth_scales=meta(64, dtype=F32))
+    assert q.dtype == torch.int8 and q.shape == x.shape and s.shape == (4, 6) and h.dtype == torch.bfloat16
+    g = pkg.npu_gated_add_rms_norm_grad(y, None, x, x, w, rstd, post_gamma=w, gate=meta(64, dtype=F32), post_rstd=prstd)
+    assert [t.shape for t in g] == [x.shape, x.shape, w.shape, w.shape, (64,)] and g[4].dtype == F32
+    for gate in (meta(6, 64), meta(1, 6, 64), meta(4, 1, 1), meta(1, 1, 1), meta(4, 6, 32), meta(1), meta(6, 1)):
+        with pytest.raises(RuntimeError, match="gate"):
+            pkg.npu_gated_add_rms_norm(x, x, w, gate=gate)
+    for kw, what in [(dict(residual=meta(4, 64)), "residual"), (dict(residual=meta(4, 6, 64, dtype=F32)), "residual"), (dict(gamma=meta(32)), "gamma"),
+                     (dict(post_gamma=meta(4, 64)), "post_gamma"), (dict(x=meta(4, 6, 64, dtype=I32)), "x must be"),
+                     (dict(gate=meta(64, dtype=I32)), "gate must be")]:
+        a = dict(x=x, residual=x, gamma=w) | kw
+        with pytest.raises(RuntimeError, match=what):
+            pkg.npu_gated_add_rms_norm(a.pop("x"), a.pop("residual"), a.pop("gamma"), **a)
+    with pytest.raises(RuntimeError, match="smooth_scales"):
+        pkg.npu_gated_add_rms_norm_dynamic_quant(x, x, w, smooth_scales=meta(32))
+    with pytest.raises(RuntimeError, match="post_rstd"):
+        pkg.npu_gated_add_rms_norm_grad(y, None, x, x, w, rstd, post_gamma=w)
+    with pytest.raises(RuntimeError, match="rstd must be"):
+        pkg.npu_gated_add_rms_norm_grad(y, None, x, x, w, meta(4, 5, dtype=F32))
+    with pytest.raises(RuntimeError, match="grad_y"):
+        pkg.npu_gated_add_rms_norm_grad(meta(4, 6, 32), None, x, x, w, rstd)
+
+
+def test_gated_norm_argument_checks(lib):
+    last = lambda: lib.b200q_last_error().decode()  # noqa: E731
+    buf = (C.c_uint8 * 4096)()
+    p = C.addressof(buf) + (-C.addressof(buf)) % 256
+
+    def args(**kw):
+        a = cabi.GatedNormArgs()
+        a.x = a.residual = a.gamma = a.y = a.h = p
+        a.dtype, a.gamma_dtype, a.rows, a.width, a.gate_rows = cabi.BF16, cabi.BF16, 2, 16, 1
+        for k, v in kw.items():
+            setattr(a, k, v)
+        return a
+
+    fwd = lambda **kw: lib.b200q_gated_norm(C.byref(args(**kw)), None)  # noqa: E731
+    assert lib.b200q_gated_norm(None, None) == cabi.ERR_BAD_ARG
+    for kw, status, what in [
+            (dict(rows=-1), cabi.ERR_BAD_ARG, "negative"), (dict(dtype=cabi.I8), cabi.ERR_UNSUPPORTED, "bf16, f16 or f32"),
+            (dict(width=16385), cabi.ERR_UNSUPPORTED, "at most 16384"), (dict(gamma_dtype=cabi.I8), cabi.ERR_UNSUPPORTED, "gamma"),
+            (dict(gate=p, gate_rows=0), cabi.ERR_BAD_ARG, "gate_rows"), (dict(gate=p, gate_rows=2, gate_per_row=1), cabi.ERR_UNSUPPORTED, "one row"),
+            (dict(smooth=p), cabi.ERR_BAD_ARG, "quantised"), (dict(scale=p, smooth=p, smooth_dtype=cabi.I8), cabi.ERR_UNSUPPORTED, "smooth"),
+            (dict(x=None), cabi.ERR_BAD_ARG, "NULL"), (dict(h=p + 1), cabi.ERR_BAD_ARG, "misaligned"), (dict(rstd=p + 2), cabi.ERR_BAD_ARG, "misaligned")]:
+        assert fwd(**kw) == status and what in last(), (kw, last())
+    assert fwd(rows=0) == cabi.OK and fwd(width=0) == cabi.OK
+
+    def bwd(a=None, **kw):
+        g = cabi.GatedNormGrads()
+        g.dy = g.dx = g.dresidual = g.dgamma = g.workspace = p
+        g.workspace_bytes = 4096
+        for k, v in kw.items():
+            setattr(g, k, v)
+        return lib.b200q_gated_norm_grad(C.byref(a or args(rstd=p)), C.byref(g), None)
+
+    assert bwd(a=args()) == cabi.ERR_BAD_ARG and "NULL" in last()
+    assert bwd(dy=None) == cabi.ERR_BAD_ARG and bwd(dgamma=p + 1) == cabi.ERR_BAD_ARG
+    assert bwd(workspace_bytes=64) == cabi.ERR_WORKSPACE and bwd(workspace=p + 16) == cabi.ERR_WORKSPACE
+    assert bwd(a=args(rstd=p, gate=p)) == cabi.ERR_BAD_ARG                       # no place for the gate's gradient
+    assert bwd(a=args(rstd=p, post_gamma=p, post_rstd=p)) == cabi.ERR_BAD_ARG
+    assert lib.b200q_gated_norm_grad_workspace_bytes(C.byref(args())) == 2 * 2 * 16 * 4
+    assert lib.b200q_gated_norm_grad_workspace_bytes(C.byref(args(gate=p, gate_rows=2))) == (2 * 2 + 2 + 1) * 16 * 4
+    assert bwd(a=args(rstd=p, rows=70000 * 2, gate=p, gate_rows=2), dgate=p) == cabi.ERR_UNSUPPORTED and "65533" in last()
