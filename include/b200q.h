@@ -355,6 +355,28 @@ int b200q_gated_norm(const b200q_gated_norm_args* args, void* stream);
 size_t b200q_gated_norm_grad_workspace_bytes(const b200q_gated_norm_args* args);
 int b200q_gated_norm_grad(const b200q_gated_norm_args* args, const b200q_gated_norm_grads* grads, void* stream);
 
+/* npu_grouped_matmul, int8 form: rows of x sorted by group, each times its group's weight.
+ * out[m,n] = cast( float(sum_k x[m,k] * weight[g](k,n) + bias_i32[g,n]) * scale[g,n] * row_scale[m] + bias_float[g,n] ),
+ * g the group of row m; int32 output returns the accumulator (with an int32 bias).  Rows past the last group are zero.
+ * Ends that go down or past m are clamped, so no list makes the kernel leave its buffers. */
+typedef struct {
+  const int8_t* x;          /* [m, k], row stride k                                                         */
+  const int8_t* weight;     /* element (g, k_, n_) at weight[g*w_stride_g + k_*w_stride_k + n_*w_stride_n]  */
+  int64_t m, k, n, groups;  /* at most 1024 groups                                                          */
+  int64_t w_stride_g, w_stride_k, w_stride_n;   /* tensor cores: w_stride_k 1, the others multiples of 16   */
+  const int64_t* group_list;    /* [groups] end row of each group, or (counts != 0) its number of rows      */
+  int counts;
+  const void* scale;        /* [groups, n] f32, bf16 or i64; unused for int32 output                        */
+  int scale_dtype;
+  const float* row_scale;   /* [m] or NULL                                                                  */
+  const void* bias;         /* [groups, n] or NULL: i32 joins the accumulator, bf16/f16/f32 are added last  */
+  int bias_dtype;
+  void* out;                /* [m, n] f16, bf16 or i32                                                      */
+  int out_dtype;
+} b200q_grouped_matmul_args;
+
+int b200q_grouped_matmul(const b200q_grouped_matmul_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -111,3 +111,18 @@ def gated_add_rms_norm_grad(x, residual, gamma, post_gamma, gate, residual_scale
             v = dz * post_gamma.to(F64).abs()
             bounds["x"] = post_rstd[..., None] * (v + xn.abs() * (v * xn.abs()).mean(-1, keepdim=True))
     return grads, bounds
+
+
+def grouped_matmul(x, weight, group_ends, scale, row_scale, bias, out_dtype):
+    """Rows of ``x`` times their group's ``weight [groups, k, n]`` with ``quant_oracle.quant_matmul``'s epilogue (the same fp32
+    steps as the kernel's, so the result is bit-exact); rows past the last group are zero."""
+    out = torch.zeros((x.shape[0], weight.shape[2]), dtype=out_dtype)
+    start = 0
+    for g in range(weight.shape[0]):
+        end = min(max(int(group_ends[g]), start), x.shape[0])
+        if end > start:
+            out[start:end] = quant_oracle.quant_matmul(
+                x[start:end], weight[g], torch.ones(1) if scale is None else scale[g],
+                pertoken_scale=None if row_scale is None else row_scale[start:end], bias=None if bias is None else bias[g], output_dtype=out_dtype)
+        start = end
+    return out

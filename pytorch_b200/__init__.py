@@ -37,6 +37,7 @@ OPS = (
     "npu_gated_add_rms_norm",
     "npu_gated_add_rms_norm_grad",
     "npu_gated_add_rms_norm_dynamic_quant",
+    "npu_grouped_matmul",
 )
 
 
@@ -66,6 +67,7 @@ npu_moe_token_unpermute_grad = _torch.ops.npu.npu_moe_token_unpermute_grad
 npu_gated_add_rms_norm = _torch.ops.npu.npu_gated_add_rms_norm
 npu_gated_add_rms_norm_grad = _torch.ops.npu.npu_gated_add_rms_norm_grad
 npu_gated_add_rms_norm_dynamic_quant = _torch.ops.npu.npu_gated_add_rms_norm_dynamic_quant
+npu_grouped_matmul = _torch.ops.npu.npu_grouped_matmul
 
 from . import collective_ops  # noqa: E402,F401  (defines the three collective-fused operators in torch.ops.npu)
 

@@ -31,6 +31,7 @@ EXPORTS = (
     "b200q_moe_route_workspace_bytes", "b200q_moe_route", "b200q_moe_combine",
     "b200q_moe_combine_grad_workspace_bytes", "b200q_moe_combine_grad",
     "b200q_gated_norm", "b200q_gated_norm_grad_workspace_bytes", "b200q_gated_norm_grad",
+    "b200q_grouped_matmul",
 )
 
 
@@ -111,6 +112,19 @@ class GatedNormGrads(C.Structure):
     ]
 
 
+class GroupedMatmulArgs(C.Structure):
+    _fields_ = [
+        ("x", C.c_void_p), ("weight", C.c_void_p),
+        ("m", C.c_int64), ("k", C.c_int64), ("n", C.c_int64), ("groups", C.c_int64),
+        ("w_stride_g", C.c_int64), ("w_stride_k", C.c_int64), ("w_stride_n", C.c_int64),
+        ("group_list", C.c_void_p), ("counts", C.c_int),
+        ("scale", C.c_void_p), ("scale_dtype", C.c_int),
+        ("row_scale", C.c_void_p),
+        ("bias", C.c_void_p), ("bias_dtype", C.c_int),
+        ("out", C.c_void_p), ("out_dtype", C.c_int),
+    ]
+
+
 class B200QError(RuntimeError):
     def __init__(self, status: int, message: str):
         super().__init__(f"b200q status {status}: {message}")
@@ -171,6 +185,7 @@ def lib() -> C.CDLL:
         l.b200q_gated_norm.argtypes = [C.POINTER(GatedNormArgs), C.c_void_p]
         l.b200q_gated_norm_grad_workspace_bytes.restype = C.c_size_t
         l.b200q_gated_norm_grad_workspace_bytes.argtypes = [C.POINTER(GatedNormArgs)]
+        l.b200q_grouped_matmul.argtypes = [C.POINTER(GroupedMatmulArgs), C.c_void_p]
         l.b200q_gated_norm_grad.argtypes = [C.POINTER(GatedNormArgs), C.POINTER(GatedNormGrads), C.c_void_p]
         _lib = l
     return _lib

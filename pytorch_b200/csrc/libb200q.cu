@@ -12,3 +12,4 @@
 #include "peer_scatter.cu"
 #include "moe_routing.cu"
 #include "gated_norm.cu"
+#include "grouped_matmul.cu"

@@ -477,6 +477,113 @@ NormGrads norm_grad_cuda(const Tensor& dy, const optional<Tensor>& dh, const Ten
 }
 
 // ---------------------------------------------------------------------------------------------
+// npu_grouped_matmul(x, weight, *, bias, scale, per_token_scale, group_list, split_item, group_type, group_list_type, output_dtype)
+// One x, one weight [groups, k, n] and one output (split_item 2 or 3, group_type 0), int8 operands.
+struct GroupedSpec {
+  int64_t m, k, n, groups;
+  at::ScalarType out;
+};
+
+GroupedSpec grouped_check(at::TensorList x, at::TensorList weight, const c10::optional<std::vector<Tensor>>& bias,
+                          const c10::optional<std::vector<Tensor>>& scale, bool others, const c10::optional<std::vector<Tensor>>& row_scale,
+                          const optional<Tensor>& group_list, int64_t split_item, int64_t group_type, int64_t list_type, int64_t act_type,
+                          optional<at::ScalarType> output_dtype) {
+  constexpr const char* op = "npu_grouped_matmul";
+  TORCH_CHECK(x.size() == 1 && weight.size() == 1, op, ": one x and one weight [groups, k, n] are implemented, got ", x.size(), " and ", weight.size(),
+              " tensors");
+  TORCH_CHECK(!others, op, ": offset, antiquant_scale, antiquant_offset and activation inputs are not implemented (the int8 form takes scale, ",
+              "per_token_scale and bias)");
+  TORCH_CHECK(split_item == 2 || split_item == 3, op, ": split_item must be 2 or 3 (one output), got ", split_item);
+  TORCH_CHECK(group_type == 0, op, ": group_type must be 0 (rows of x are grouped), got ", group_type);
+  TORCH_CHECK(list_type == 0 || list_type == 1, op, ": group_list_type must be 0 (cumulative) or 1 (counts), got ", list_type);
+  TORCH_CHECK(act_type == 0, op, ": act_type must be 0, got ", act_type);
+  const Tensor &a = x[0], &w = weight[0];
+  TORCH_CHECK(a.dim() == 2 && a.scalar_type() == at::kChar && w.dim() == 3 && w.scalar_type() == at::kChar, op,
+              ": x must be int8 [m, k] and weight int8 [groups, k, n], got ", a.scalar_type(), " ", a.sizes(), " and ", w.scalar_type(), " ", w.sizes());
+  TORCH_CHECK(w.size(1) == a.size(1), op, ": inner dimensions differ: x ", a.sizes(), " and weight ", w.sizes());
+  GroupedSpec s{a.size(0), a.size(1), w.size(2), w.size(0), output_dtype.value_or(at::kBFloat16)};
+  TORCH_CHECK(s.groups >= 1 && s.groups <= 1024, op, ": 1 to 1024 groups, got ", s.groups);
+  TORCH_CHECK(s.out == at::kBFloat16 || s.out == at::kHalf || s.out == at::kInt, op, ": output_dtype must be bfloat16, float16 or int32, got ", s.out);
+  TORCH_CHECK(group_list.has_value() && group_list->dim() == 1 && group_list->size(0) == s.groups &&
+                  (group_list->scalar_type() == at::kLong || group_list->scalar_type() == at::kInt),
+              op, ": group_list must be an int64 tensor with one entry for each of the ", s.groups, " groups");
+  auto one = [&](const c10::optional<std::vector<Tensor>>& list, const char* name) -> const Tensor* {
+    if (!list.has_value() || list->empty()) return nullptr;
+    TORCH_CHECK(list->size() == 1, op, ": ", name, " must hold one tensor, got ", list->size());
+    return &(*list)[0];
+  };
+  if (const Tensor* t = one(scale, "scale")) {
+    TORCH_CHECK(t->numel() == s.groups * s.n && t->size(-1) == s.n &&
+                    (t->scalar_type() == at::kFloat || t->scalar_type() == at::kBFloat16 || t->scalar_type() == at::kLong),
+                op, ": scale must be float32, bfloat16 or int64 [", s.groups, ", ", s.n, "], got ", t->scalar_type(), " ", t->sizes());
+  } else {
+    TORCH_CHECK(s.out == at::kInt, op, ": scale is needed unless output_dtype is int32");
+  }
+  if (const Tensor* t = one(row_scale, "per_token_scale"))
+    TORCH_CHECK(t->numel() == s.m && t->scalar_type() == at::kFloat, op, ": per_token_scale must be float32 [", s.m, "], got ", t->scalar_type(), " ",
+                t->sizes());
+  if (const Tensor* t = one(bias, "bias"))
+    TORCH_CHECK(t->numel() == s.groups * s.n && t->size(-1) == s.n && (t->scalar_type() == at::kInt || (s.out != at::kInt && is_float_type(t->scalar_type()))),
+                op, ": bias must be int32 or (not for int32 output) a float type, [", s.groups, ", ", s.n, "], got ", t->scalar_type(), " ", t->sizes());
+  return s;
+}
+
+bool given(const c10::optional<std::vector<Tensor>>& list) { return list.has_value() && !list->empty(); }
+
+std::vector<Tensor> grouped_matmul_cuda(at::TensorList x, at::TensorList weight, const c10::optional<std::vector<Tensor>>& bias,
+                                        const c10::optional<std::vector<Tensor>>& scale, const c10::optional<std::vector<Tensor>>& offset,
+                                        const c10::optional<std::vector<Tensor>>& antiquant_scale,
+                                        const c10::optional<std::vector<Tensor>>& antiquant_offset,
+                                        const c10::optional<std::vector<Tensor>>& row_scale, const optional<Tensor>& group_list,
+                                        const c10::optional<std::vector<Tensor>>& act_input, const c10::optional<std::vector<Tensor>>& act_quant_scale,
+                                        const c10::optional<std::vector<Tensor>>& act_quant_offset, int64_t split_item, int64_t group_type,
+                                        int64_t list_type, int64_t act_type, at::OptionalIntArrayRef /*tuning_config*/,
+                                        optional<at::ScalarType> output_dtype) {
+  constexpr const char* op = "npu_grouped_matmul";
+  const GroupedSpec s = grouped_check(x, weight, bias, scale,
+                                      given(offset) || given(antiquant_scale) || given(antiquant_offset) || given(act_input) || given(act_quant_scale) ||
+                                          given(act_quant_offset),
+                                      row_scale, group_list, split_item, group_type, list_type, act_type, output_dtype);
+  auto first = [](const c10::optional<std::vector<Tensor>>& list) { return given(list) ? optional<Tensor>((*list)[0]) : optional<Tensor>(); };
+  const Tensor& a = x[0];
+  const optional<Tensor> wo(weight[0]), bo = first(bias), so = first(scale), ro = first(row_scale);
+  check_same_device(op, a, {&wo, &bo, &so, &ro, &group_list});
+  c10::cuda::CUDAGuard guard(a.device());
+  surface_device_error(op, a);
+  Tensor out = at::empty({s.m, s.n}, a.options().dtype(s.out));
+  Tensor xc = a.contiguous(), list = group_list->to(at::kLong).contiguous();
+  Tensor bc = contiguous_or_none(bo), sc = contiguous_or_none(so), rc = contiguous_or_none(ro);
+  const Tensor& w = weight[0];
+  b200q_grouped_matmul_args g{};
+  g.x = static_cast<const int8_t*>(xc.data_ptr()); g.weight = static_cast<const int8_t*>(w.data_ptr());
+  g.m = s.m; g.k = s.k; g.n = s.n; g.groups = s.groups;
+  g.w_stride_g = w.stride(0); g.w_stride_k = w.stride(1); g.w_stride_n = w.stride(2);
+  g.group_list = static_cast<const int64_t*>(list.data_ptr()); g.counts = list_type == 1 ? 1 : 0;
+  if (sc.defined()) { g.scale = sc.data_ptr(); g.scale_dtype = dtype_enum(sc.scalar_type()); }
+  if (rc.defined()) g.row_scale = static_cast<const float*>(rc.data_ptr());
+  g.bias_dtype = B200Q_NONE;
+  if (bc.defined()) { g.bias = bc.data_ptr(); g.bias_dtype = dtype_enum(bc.scalar_type()); }
+  g.out = out.data_ptr(); g.out_dtype = dtype_enum(s.out);
+  check_status(b200q_grouped_matmul(&g, stream_of(a)), op);
+  return {out};
+}
+
+std::vector<Tensor> grouped_matmul_meta(at::TensorList x, at::TensorList weight, const c10::optional<std::vector<Tensor>>& bias,
+                                        const c10::optional<std::vector<Tensor>>& scale, const c10::optional<std::vector<Tensor>>& offset,
+                                        const c10::optional<std::vector<Tensor>>& antiquant_scale,
+                                        const c10::optional<std::vector<Tensor>>& antiquant_offset,
+                                        const c10::optional<std::vector<Tensor>>& row_scale, const optional<Tensor>& group_list,
+                                        const c10::optional<std::vector<Tensor>>& act_input, const c10::optional<std::vector<Tensor>>& act_quant_scale,
+                                        const c10::optional<std::vector<Tensor>>& act_quant_offset, int64_t split_item, int64_t group_type,
+                                        int64_t list_type, int64_t act_type, at::OptionalIntArrayRef, optional<at::ScalarType> output_dtype) {
+  const GroupedSpec s = grouped_check(x, weight, bias, scale,
+                                      given(offset) || given(antiquant_scale) || given(antiquant_offset) || given(act_input) || given(act_quant_scale) ||
+                                          given(act_quant_offset),
+                                      row_scale, group_list, split_item, group_type, list_type, act_type, output_dtype);
+  return {at::empty({s.m, s.n}, x[0].options().dtype(s.out))};
+}
+
+// ---------------------------------------------------------------------------------------------
 // Autograd
 class PermuteFunction : public torch::autograd::Function<PermuteFunction> {
  public:
@@ -604,6 +711,10 @@ TORCH_LIBRARY_FRAGMENT(npu, m) {
   m.def("npu_gated_add_rms_norm_grad(Tensor grad_y, Tensor? grad_h, Tensor x, Tensor residual, Tensor gamma, Tensor rstd, *, "
         "Tensor? post_gamma=None, Tensor? gate=None, Tensor? post_rstd=None, float residual_scale=1.0) "
         "-> (Tensor, Tensor, Tensor, Tensor, Tensor)");
+  m.def("npu_grouped_matmul(Tensor[] x, Tensor[] weight, *, Tensor[]? bias=None, Tensor[]? scale=None, Tensor[]? offset=None, "
+        "Tensor[]? antiquant_scale=None, Tensor[]? antiquant_offset=None, Tensor[]? per_token_scale=None, Tensor? group_list=None, "
+        "Tensor[]? activation_input=None, Tensor[]? activation_quant_scale=None, Tensor[]? activation_quant_offset=None, int split_item=0, "
+        "int group_type=0, int group_list_type=0, int act_type=0, int[]? tuning_config=None, ScalarType? output_dtype=None) -> Tensor[]");
 }
 
 TORCH_LIBRARY_IMPL(npu, CUDA, m) {
@@ -615,6 +726,7 @@ TORCH_LIBRARY_IMPL(npu, CUDA, m) {
   m.impl("npu_gated_add_rms_norm", TORCH_FN(norm_cuda));
   m.impl("npu_gated_add_rms_norm_dynamic_quant", TORCH_FN(norm_quant_cuda));
   m.impl("npu_gated_add_rms_norm_grad", TORCH_FN(norm_grad_cuda));
+  m.impl("npu_grouped_matmul", TORCH_FN(grouped_matmul_cuda));
 }
 
 TORCH_LIBRARY_IMPL(npu, AutogradCUDA, m) {
@@ -632,4 +744,5 @@ TORCH_LIBRARY_IMPL(npu, Meta, m) {
   m.impl("npu_gated_add_rms_norm", TORCH_FN(norm_meta));
   m.impl("npu_gated_add_rms_norm_dynamic_quant", TORCH_FN(norm_quant_meta));
   m.impl("npu_gated_add_rms_norm_grad", TORCH_FN(norm_grad_meta));
+  m.impl("npu_grouped_matmul", TORCH_FN(grouped_matmul_meta));
 }

@@ -201,3 +201,54 @@ def test_gated_norm_argument_checks(lib):
     assert lib.b200q_gated_norm_grad_workspace_bytes(C.byref(args())) == 2 * 2 * 16 * 4
     assert lib.b200q_gated_norm_grad_workspace_bytes(C.byref(args(gate=p, gate_rows=2))) == (2 * 2 + 2 + 1) * 16 * 4
     assert bwd(a=args(rstd=p, rows=70000 * 2, gate=p, gate_rows=2), dgate=p) == cabi.ERR_UNSUPPORTED and "65533" in last()
+
+
+def test_grouped_matmul_meta_contract(pkg):
+    x, w = meta(40, 64, dtype=torch.int8), meta(4, 64, 24, dtype=torch.int8)
+    sc, rs, gl = meta(4, 24, dtype=F32), meta(40, dtype=F32), meta(4, dtype=I64)
+    ok = dict(scale=[sc], per_token_scale=[rs], group_list=gl, split_item=3, output_dtype=torch.float16)
+    out = pkg.npu_grouped_matmul([x], [w], **ok)
+    assert len(out) == 1 and out[0].shape == (40, 24) and out[0].dtype == torch.float16
+    assert pkg.npu_grouped_matmul([x], [w], group_list=gl, split_item=2, output_dtype=I32)[0].dtype == I32
+    for kw, what in [(dict(split_item=0), "split_item"), (dict(group_type=2), "group_type"), (dict(group_list_type=2), "group_list_type"),
+                     (dict(act_type=1), "act_type"), (dict(group_list=None), "group_list"), (dict(group_list=meta(3, dtype=I64)), "group_list"),
+                     (dict(group_list=meta(4, dtype=F32)), "group_list"), (dict(scale=None), "scale is needed"), (dict(scale=[meta(4, 23, dtype=F32)]), "scale"),
+                     (dict(scale=[sc, sc]), "one tensor"), (dict(per_token_scale=[meta(39, dtype=F32)]), "per_token_scale"),
+                     (dict(bias=[meta(24, dtype=F32)]), "bias"), (dict(output_dtype=F32), "output_dtype"), (dict(offset=[sc]), "not implemented"),
+                     (dict(antiquant_scale=[sc]), "not implemented")]:
+        with pytest.raises(RuntimeError, match=what):
+            pkg.npu_grouped_matmul([x], [w], **(ok | kw))
+    with pytest.raises(RuntimeError, match="one x"):
+        pkg.npu_grouped_matmul([x, x], [w], **ok)
+    with pytest.raises(RuntimeError, match="int8"):
+        pkg.npu_grouped_matmul([meta(40, 64)], [w], **ok)
+    with pytest.raises(RuntimeError, match="inner dimensions"):
+        pkg.npu_grouped_matmul([meta(40, 32, dtype=torch.int8)], [w], **ok)
+    with pytest.raises(RuntimeError, match="bias"):
+        pkg.npu_grouped_matmul([x], [w], group_list=gl, split_item=2, output_dtype=I32, bias=[meta(4, 24, dtype=F32)])
+
+
+def test_grouped_matmul_argument_checks(lib):
+    last = lambda: lib.b200q_last_error().decode()  # noqa: E731
+    buf = (C.c_uint8 * 4096)()
+    p = C.addressof(buf) + (-C.addressof(buf)) % 256
+
+    def run(**kw):
+        a = cabi.GroupedMatmulArgs()
+        a.x = a.weight = a.group_list = a.scale = a.out = p
+        a.m, a.k, a.n, a.groups, a.w_stride_g, a.w_stride_k, a.w_stride_n = 4, 16, 8, 2, 128, 1, 16
+        a.scale_dtype, a.bias_dtype, a.out_dtype = cabi.F32, cabi.NONE, cabi.BF16
+        for k, v in kw.items():
+            setattr(a, k, v)
+        return lib.b200q_grouped_matmul(C.byref(a), None)
+
+    assert lib.b200q_grouped_matmul(None, None) == cabi.ERR_BAD_ARG
+    for kw, status, what in [
+            (dict(m=-1), cabi.ERR_BAD_ARG, "negative"), (dict(groups=0), cabi.ERR_UNSUPPORTED, "groups"), (dict(groups=1025), cabi.ERR_UNSUPPORTED, "groups"),
+            (dict(m=2 ** 31), cabi.ERR_UNSUPPORTED, "out of range"), (dict(out_dtype=cabi.I8), cabi.ERR_UNSUPPORTED, "output dtype"),
+            (dict(scale_dtype=cabi.F16), cabi.ERR_UNSUPPORTED, "scale"), (dict(bias=p, bias_dtype=cabi.I8), cabi.ERR_UNSUPPORTED, "bias"),
+            (dict(out_dtype=cabi.I32, bias=p, bias_dtype=cabi.F32), cabi.ERR_UNSUPPORTED, "bias"), (dict(group_list=None), cabi.ERR_BAD_ARG, "NULL"),
+            (dict(scale=None), cabi.ERR_BAD_ARG, "NULL"), (dict(group_list=p + 4), cabi.ERR_BAD_ARG, "misaligned"),
+            (dict(out=p + 1), cabi.ERR_BAD_ARG, "misaligned")]:
+        assert run(**kw) == status and what in last(), (kw, last())
+    assert run(m=0) == cabi.OK and run(n=0) == cabi.OK
