@@ -319,16 +319,14 @@ typedef struct {
   const void* residual;     /* the same                                                                     */
   int dtype;
   const void* gamma;        /* [width]                                                                      */
-  int gamma_dtype;
   const void* post_gamma;   /* [width] or NULL                                                              */
-  int post_gamma_dtype;
   const void* gate;         /* [ceil(rows / gate_rows), width] (gate_per_row 0) or [rows] (1), or NULL      */
-  int gate_dtype;
+  int param_dtype;          /* of gamma, post_gamma and gate: x's, or f32                                   */
   int gate_per_row;         /* one value a row; gate_rows is then 1                                         */
   int64_t gate_rows;        /* consecutive rows that share a gate                                           */
   float residual_scale, epsilon;
   int64_t rows, width;
-  const void* smooth;       /* quantised form: [width] or NULL                                              */
+  const void* smooth;       /* quantised form: [width] or NULL, in x's dtype or f32                         */
   int smooth_dtype;
   void* y;                  /* [rows, width], x's dtype or int8                                             */
   void* h;                  /* [rows, width], x's dtype                                                     */
@@ -342,9 +340,9 @@ typedef struct {
   const void* dh;           /* the gradient that reaches h directly, or NULL                                */
   void* dx;
   void* dresidual;
-  void* dgamma;             /* [width], gamma's dtype                                                       */
-  void* dpost_gamma;        /* [width], post_gamma's dtype; unused without post_gamma                       */
-  void* dgate;              /* gate's shape and dtype; unused without gate                                  */
+  void* dgamma;             /* [width], param_dtype                                                         */
+  void* dpost_gamma;        /* [width], param_dtype; unused without post_gamma                              */
+  void* dgate;              /* gate's shape, param_dtype; unused without gate                               */
   void* workspace;          /* >= b200q_gated_norm_grad_workspace_bytes(), 256-byte aligned                 */
   size_t workspace_bytes;
 } b200q_gated_norm_grads;

@@ -95,9 +95,8 @@ class MoeCombineGradArgs(C.Structure):
 class GatedNormArgs(C.Structure):
     _fields_ = [
         ("x", C.c_void_p), ("residual", C.c_void_p), ("dtype", C.c_int),
-        ("gamma", C.c_void_p), ("gamma_dtype", C.c_int),
-        ("post_gamma", C.c_void_p), ("post_gamma_dtype", C.c_int),
-        ("gate", C.c_void_p), ("gate_dtype", C.c_int), ("gate_per_row", C.c_int), ("gate_rows", C.c_int64),
+        ("gamma", C.c_void_p), ("post_gamma", C.c_void_p), ("gate", C.c_void_p), ("param_dtype", C.c_int),
+        ("gate_per_row", C.c_int), ("gate_rows", C.c_int64),
         ("residual_scale", C.c_float), ("epsilon", C.c_float),
         ("rows", C.c_int64), ("width", C.c_int64),
         ("smooth", C.c_void_p), ("smooth_dtype", C.c_int),

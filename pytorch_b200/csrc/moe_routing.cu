@@ -40,15 +40,16 @@ __device__ __forceinline__ int expert_of(const IdT* __restrict__ ids, int64_t i,
 // ------------------------------------------------------------------------------------------------ sorting
 // Stable counting sort of up to 2^31 indices by one cluster of CTAs.  Warp w of CTA c owns a contiguous piece of
 // the indices, so (c, w, position) is the order of the assignments.  Pass 1 counts every warp's experts in shared
-// memory, 32 indices a step (the lanes that hold the same expert find one another with match.any, one of them
-// adds); a prefix over warps, over the CTAs of the cluster (through distributed shared memory) and over the
-// experts turns the counts into first rows; pass 2 walks the indices again and hands the rows out.  No global
-// scratch, no atomics, no waiting but the cluster's barrier.
+// memory; a prefix over warps, over the CTAs of the cluster (through distributed shared memory) and over the experts
+// turns the counts into first rows; pass 2 walks the indices again, 32 a step, and hands the rows out: the lanes with the
+// same expert find one another by a ballot for each bit of the expert's number, and one of them moves the expert's next
+// row on.  No global scratch, no atomics outside shared memory, no waiting but the cluster's barrier.
 constexpr int kSortThreads = 1024;
 constexpr int kSortWarps = kSortThreads / 32;
+constexpr int kSortBatch = 8;             // index loads in flight per lane
 
-template <typename IdT>
-__global__ void __launch_bounds__(kSortThreads)
+template <typename IdT, int BITS>           // BITS hold the numbers 0 .. experts
+__global__ void __launch_bounds__(kSortThreads, 1)
 moe_sort_kernel(const IdT* __restrict__ ids, int64_t n, int64_t begin, int experts, int strict_limit,
                 int32_t* __restrict__ row_idx, int32_t* __restrict__ row_src, int64_t* __restrict__ expert_tokens,
                 int cumulative, int32_t* __restrict__ valid_rows) {
@@ -56,46 +57,61 @@ moe_sort_kernel(const IdT* __restrict__ ids, int64_t n, int64_t begin, int exper
   int* hist = sort_smem;                                   // [kSortWarps][experts]
   int* total = hist + kSortWarps * experts;                // [experts] this CTA's counts
   __shared__ int warp_sums[32];
+  launch_dependents();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = (int)cluster_ctarank(), ctas = (int)cluster_nctarank();
-  for (int i = threadIdx.x; i < kSortWarps * experts; i += kSortThreads) hist[i] = 0;
-  __syncthreads();
-
   const int64_t steps = (n + 31) >> 5;                     // groups of 32 indices, dealt out in contiguous pieces
   const int64_t piece = rank * (int64_t)kSortWarps + warp, pieces = (int64_t)ctas * kSortWarps;
   const int64_t s0 = steps * piece / pieces, s1 = steps * (piece + 1) / pieces;
   int* mine = hist + warp * experts;
-  for (int64_t s = s0; s < s1; ++s) {
-    const int64_t i = s * 32 + lane;
-    int e = kNoExpert;
-    if (i < n) {
-      e = expert_of(ids, i, begin, experts);
-      if (strict_limit && static_cast<int64_t>(ids[i]) >= strict_limit) record_device_error(kDevExpertRange);
+  // The experts of one batch of steps (kNoExpert past the end or outside the range).
+  auto load = [&](int64_t s, int (&e)[kSortBatch]) {
+#pragma unroll
+    for (int b = 0; b < kSortBatch; ++b) {
+      const int64_t i = (s + b) * 32 + lane;
+      e[b] = kNoExpert;
+      if (s + b < s1 && i < n) {
+        const int64_t id = static_cast<int64_t>(ids[i]);
+        if (id - begin >= 0 && id - begin < experts) e[b] = static_cast<int>(id - begin);
+        else if (strict_limit && id >= strict_limit) record_device_error(kDevExpertRange);
+      }
     }
-    const unsigned same = __match_any_sync(0xffffffffu, e);
-    if (e >= 0 && lane == __ffs(same) - 1) mine[e] += __popc(same);
-    __syncwarp();
+  };
+  int e[kSortBatch];
+  load(s0, e);
+  for (int i = lane; i < experts; i += 32) mine[i] = 0;
+  __syncwarp();
+  for (int64_t s = s0;;) {
+#pragma unroll
+    for (int b = 0; b < kSortBatch; ++b)
+      if (e[b] >= 0) atomicAdd(mine + e[b], 1);
+    s += kSortBatch;
+    if (s >= s1) break;
+    load(s, e);
   }
   __syncthreads();
-  for (int e = threadIdx.x; e < experts; e += kSortThreads) {
-    int run = 0;
-    for (int w = 0; w < kSortWarps; ++w) {
-      const int c = hist[w * experts + e];
-      hist[w * experts + e] = run;
-      run += c;
-    }
-    total[e] = run;
-  }
-  if (ctas > 1) cluster_sync_all(); else __syncthreads();
 
-  // One expert a thread: rows of that expert in the lower CTAs and in all, then an exclusive scan over the experts.
-  const int e = threadIdx.x;
-  int lower = 0, all = 0;
-  if (e < experts) {
-    for (int c = 0; c < ctas; ++c) {
-      const int v = ctas > 1 ? (int)ld_shared_cluster_u32(map_to_cta(smem_u32(total + e), c)) : total[e];
-      if (c < rank) lower += v;
-      all += v;
+  // One expert a thread: its rows in this CTA's warps, in the lower CTAs and in all, then a scan over the experts.
+  const int x = threadIdx.x;
+  int count[kSortWarps];
+  int here = 0;
+  if (x < experts) {
+#pragma unroll
+    for (int w = 0; w < kSortWarps; ++w) count[w] = hist[w * experts + x];
+#pragma unroll
+    for (int w = 0; w < kSortWarps; ++w) here += count[w];
+    total[x] = here;
+  }
+  int lower = 0, all = here;
+  if (ctas > 1) {
+    cluster_sync_all();
+    all = 0;
+    if (x < experts) {
+      for (int c = 0; c < ctas; ++c) {
+        const int v = (int)ld_shared_cluster_u32(map_to_cta(smem_u32(total + x), c));
+        if (c < rank) lower += v;
+        all += v;
+      }
     }
   }
   int incl = all;
@@ -118,26 +134,48 @@ moe_sort_kernel(const IdT* __restrict__ ids, int64_t n, int64_t begin, int exper
   __syncthreads();
   if (warp > 0) incl += warp_sums[warp - 1];
   const int valid = warp_sums[31];
-  if (e < experts) {
-    const int first = incl - all + lower;
-    for (int w = 0; w < kSortWarps; ++w) hist[w * experts + e] += first;
-    if (rank == 0 && expert_tokens != nullptr) expert_tokens[e] = cumulative ? incl : all;
+  if (x < experts) {
+    int next = incl - all + lower;
+#pragma unroll
+    for (int w = 0; w < kSortWarps; ++w) {
+      hist[w * experts + x] = next;
+      next += count[w];
+    }
+    if (rank == 0 && expert_tokens != nullptr) expert_tokens[x] = cumulative ? incl : all;
   }
   if (rank == 0 && threadIdx.x == 0 && valid_rows != nullptr) *valid_rows = valid;
   if (row_src != nullptr)                                  // rows that no assignment owns
     for (int64_t r = valid + (int64_t)rank * kSortThreads + threadIdx.x; r < n; r += (int64_t)ctas * kSortThreads) row_src[r] = -1;
   __syncthreads();
 
-  for (int64_t s = s0; s < s1; ++s) {
-    const int64_t i = s * 32 + lane;
-    const int x = i < n ? expert_of(ids, i, begin, experts) : kNoExpert;
-    const unsigned same = __match_any_sync(0xffffffffu, x);
-    const int row = x >= 0 ? mine[x] + __popc(same & ((1u << lane) - 1)) : -1;
-    __syncwarp();
-    if (x >= 0 && lane == __ffs(same) - 1) mine[x] += __popc(same);
-    __syncwarp();
-    if (i < n) row_idx[i] = row;
-    if (x >= 0 && row_src != nullptr) row_src[row] = (int32_t)i;
+  if (s1 - s0 > kSortBatch) load(s0, e);                   // else they are still there
+  for (int64_t s = s0; s < s1;) {
+#pragma unroll
+    for (int b = 0; b < kSortBatch; ++b) {
+      if (s + b >= s1) break;
+      const int key = e[b] < 0 ? experts : e[b];
+      unsigned same = 0xffffffffu;
+#pragma unroll
+      for (int q = 0; q < BITS; ++q) {
+        const bool one = (key >> q) & 1;
+        const unsigned ballot = __ballot_sync(0xffffffffu, one);
+        same &= one ? ballot : ~ballot;
+      }
+      const int leader = __ffs(same) - 1;
+      int base = 0;
+      if (e[b] >= 0 && lane == leader) {
+        base = mine[key];
+        mine[key] = base + __popc(same);
+      }
+      base = __shfl_sync(0xffffffffu, base, leader);
+      const int64_t i = (s + b) * 32 + lane;
+      const int row = e[b] >= 0 ? base + __popc(same & ((1u << lane) - 1)) : -1;
+      if (i < n) row_idx[i] = row;
+      if (row >= 0 && row_src != nullptr) row_src[row] = (int32_t)i;
+      __syncwarp();
+    }
+    s += kSortBatch;
+    if (s < s1) load(s, e);
   }
   if (ctas > 1) cluster_sync_all();                        // nobody leaves while its counts may still be read
 }
@@ -271,6 +309,7 @@ moe_copy_kernel(const VT* __restrict__ x, VT* __restrict__ out, int64_t tokens, 
                 const int32_t* __restrict__ valid_rows, int64_t move_blocks) {
   const int lane = threadIdx.x & 31;
   if ((int64_t)blockIdx.x >= move_blocks) {
+    wait_for_primary();
     const int64_t zb = blockIdx.x - move_blocks, zn = gridDim.x - move_blocks;
     for (int64_t row = *valid_rows + zb; row < out_rows; row += zn) {
       for (int64_t v = threadIdx.x; v < nvec; v += blockDim.x) out[row * nvec + v] = VT{};
@@ -287,6 +326,7 @@ moe_copy_kernel(const VT* __restrict__ x, VT* __restrict__ out, int64_t tokens, 
 #pragma unroll
   for (int u = 0; u < U; ++u)
     if (v0 + 32 * u < nvec) val[u] = x[t * nvec + v0 + 32 * u];
+  wait_for_primary();                                      // the sort's rows; x does not depend on it
   for (int k0 = 0; k0 < topk; k0 += 32) {
     const int mine = k0 + lane < topk ? row_idx[t * topk + k0 + lane] : -1;
     const int kc = min(32, topk - k0);
@@ -304,18 +344,24 @@ moe_copy_kernel(const VT* __restrict__ x, VT* __restrict__ out, int64_t tokens, 
 // ------------------------------------------------------------------------------------------------ routing + int8
 // One row: smooth multiply, row maximum, scale, quantised values, all with the helpers (and bits) of
 // npu_dynamic_quant.  The CTA owns the row; each thread holds ITERS vectors of eight values.
-template <typename T, typename ST, int ITERS>
-__device__ __forceinline__ void quant_row_store(const uint4 (&raw)[ITERS], const ST* __restrict__ smooth, int nvec,
+template <typename ST, int ITERS>
+__device__ __forceinline__ void load_smooth_row(const ST* __restrict__ smooth, int nvec, float2 (&sm)[ITERS][4]) {
+#pragma unroll
+  for (int i = 0; i < ITERS; ++i) {
+    const int v = threadIdx.x + i * blockDim.x;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) sm[i][j] = make_float2(1.0f, 1.0f);
+    if (smooth != nullptr && v < nvec) load_smooth8(smooth + (int64_t)v * 8, sm[i]);
+  }
+}
+
+template <typename T, int ITERS>
+__device__ __forceinline__ void quant_row_store(const uint4 (&raw)[ITERS], const float2 (&sm)[ITERS][4], int nvec,
                                                 int8_t* __restrict__ y, float* __restrict__ scale_out, float* red) {
   float2 f[ITERS][4];
   float amax = 0.0f;
 #pragma unroll
-  for (int i = 0; i < ITERS; ++i) {
-    const int v = threadIdx.x + i * blockDim.x;
-    float2 sm[4] = {{1.0f, 1.0f}, {1.0f, 1.0f}, {1.0f, 1.0f}, {1.0f, 1.0f}};
-    if (smooth != nullptr && v < nvec) load_smooth8(smooth + (int64_t)v * 8, sm);
-    products8<T, true>(raw[i], sm, f[i], amax);
-  }
+  for (int i = 0; i < ITERS; ++i) products8<T, true>(raw[i], sm[i], f[i], amax);
   amax = block_max(amax, red);
   const float scale = scale_of_amax(amax);
   if (threadIdx.x == 0) *scale_out = scale;
@@ -372,7 +418,11 @@ moe_quant_direct_kernel(const RouteIds r, const T* __restrict__ x, int64_t width
   const T* xr = x + (int64_t)(i / r.topk) * width;
   const int nvec = (int)(width >> 3);
   uint4 raw[ITERS ? ITERS : 1];
+  float2 sm_row[ITERS ? ITERS : 1][4];
+  const int e = expert_of(ids, i, r.begin, r.experts);
+  const ST* sm = smooth == nullptr ? nullptr : smooth + (smooth_rows > 1 ? (int64_t)max(e, 0) * width : 0);
   if constexpr (ITERS > 0) {                               // in flight while the row is being found
+    load_smooth_row<ST, ITERS>(sm, nvec, sm_row);
 #pragma unroll
     for (int q = 0; q < ITERS; ++q) {
       const int v = threadIdx.x + q * blockDim.x;
@@ -382,7 +432,6 @@ moe_quant_direct_kernel(const RouteIds r, const T* __restrict__ x, int64_t width
   int rows[1];
   direct_rows(ids, n, r.begin, r.experts, i, red_i, rows);
   const int64_t row = rows[0];
-  const int e = expert_of(ids, i, r.begin, r.experts);
   if (threadIdx.x == 0) {
     row_idx[i] = e >= 0 ? (int)row : -1;
     if (row_src != nullptr) row_src[row] = e >= 0 ? i : -1;
@@ -391,22 +440,24 @@ moe_quant_direct_kernel(const RouteIds r, const T* __restrict__ x, int64_t width
     zero_quant_row(out + row * width, out_scale + row, width);
     return;
   }
-  const ST* sm = smooth == nullptr ? nullptr : smooth + (smooth_rows > 1 ? (int64_t)e * width : 0);
-  if constexpr (ITERS > 0) quant_row_store<T, ST, ITERS>(raw, sm, nvec, out + row * width, out_scale + row, red);
+  if constexpr (ITERS > 0) quant_row_store<T, ITERS>(raw, sm_row, nvec, out + row * width, out_scale + row, red);
   else quant_row_generic<T, ST>(xr, sm, width, out + row * width, out_scale + row, red);
 }
 
-// Many assignments: persistent CTAs take contiguous pieces of the sorted rows (so a piece stays with one expert's
-// smooth scales, which the SM's L1 then holds); the next row is in flight during the arithmetic of this one.
+// Many assignments: persistent CTAs take contiguous pieces of the sorted rows, so a piece mostly stays with one expert,
+// whose smooth scales stay in registers; the next row is in flight during the arithmetic of this one.
 template <typename IdT, typename T, typename ST, int ITERS>
 __global__ void __launch_bounds__(512)
 moe_quant_kernel(const RouteIds r, const T* __restrict__ x, int64_t width, const ST* __restrict__ smooth, int smooth_rows,
                  int8_t* __restrict__ out, float* __restrict__ out_scale, const int32_t* __restrict__ row_src) {
   const IdT* ids = static_cast<const IdT*>(r.ids);
   __shared__ float red[2][32];
+  wait_for_primary();
   const int nvec = (int)(width >> 3);
   const int64_t r0 = r.n * blockIdx.x / gridDim.x, r1 = r.n * (blockIdx.x + 1) / gridDim.x;
   uint4 raw[ITERS ? ITERS : 1], nxt[ITERS ? ITERS : 1];
+  float2 sm_row[ITERS ? ITERS : 1][4];
+  int sm_expert = -1;
   auto load = [&](int src, uint4(&to)[ITERS ? ITERS : 1]) {
     if constexpr (ITERS > 0) {
       const uint4* xr = reinterpret_cast<const uint4*>(x + (int64_t)(src / r.topk) * width);
@@ -417,7 +468,9 @@ moe_quant_kernel(const RouteIds r, const T* __restrict__ x, int64_t width, const
       }
     }
   };
+  // Row r's assignment is read two rows ahead, its expert and x one row ahead.
   int src = r0 < r1 ? row_src[r0] : -1;
+  int expert = src >= 0 ? expert_of(ids, src, r.begin, r.experts) : 0;
   if (src >= 0) load(src, nxt);
   int after = r0 + 1 < r1 ? row_src[r0 + 1] : -1;
   int par = 0;
@@ -427,18 +480,22 @@ moe_quant_kernel(const RouteIds r, const T* __restrict__ x, int64_t width, const
       for (int q = 0; q < ITERS; ++q) raw[q] = nxt[q];
       if (after >= 0) load(after, nxt);
     }
-    const int here = src;
+    const int here = src, e = expert;
     src = after;
+    if (src >= 0) expert = expert_of(ids, src, r.begin, r.experts);
     after = row + 2 < r1 ? row_src[row + 2] : -1;
     if (here < 0) {
       zero_quant_row(out + row * width, out_scale + row, width);
       continue;
     }
     par ^= 1;                                              // a buffer is written again only behind the other one's barrier
-    const int e = expert_of(ids, here, r.begin, r.experts);
     const ST* sm = smooth == nullptr ? nullptr : smooth + (smooth_rows > 1 ? (int64_t)e * width : 0);
     if constexpr (ITERS > 0) {
-      quant_row_store<T, ST, ITERS>(raw, sm, nvec, out + row * width, out_scale + row, red[par]);
+      if (sm_expert < 0 || (smooth_rows > 1 && e != sm_expert)) {
+        load_smooth_row<ST, ITERS>(sm, nvec, sm_row);
+        sm_expert = e;
+      }
+      quant_row_store<T, ITERS>(raw, sm_row, nvec, out + row * width, out_scale + row, red[par]);
     } else {
       quant_row_generic<T, ST>(x + (int64_t)(here / r.topk) * width, sm, width, out + row * width, out_scale + row, red[par]);
     }
@@ -590,6 +647,168 @@ moe_combine_grad_kernel(const T* __restrict__ dy, const T* __restrict__ rows, in
   }
 }
 
+// Both directions for many tokens, as a pipeline: a producer warp brings the rows of a token (lane k the row of slot k) and,
+// for the gradient, dy into shared memory with bulk copies, kGatherBytes of every row a stage; eight warps work on them,
+// a 16-byte vector of every row a thread.  The rows lie all over HBM and their indices have to be read first; the ring of
+// copies keeps about 200 KB an SM in flight whatever the registers allow, and the indices of the next token are read a
+// token ahead.  Waits are bounded; a thread that gives one up goes on without loading or storing, so that the barriers
+// still meet.
+constexpr int kGatherBytes = 4096;        // of a row, per stage
+constexpr int kGatherWarps = 8;
+constexpr int kGatherThreads = 32 * (kGatherWarps + 1);
+constexpr int kGatherSmem = 112 * 1024;   // two CTAs an SM
+
+template <int KC, bool GRAD>
+struct GatherLayout {
+  static constexpr int kRows = KC + (GRAD ? 1 : 0);
+  static constexpr int kStageBytes = kRows * kGatherBytes;
+  static constexpr int kFit = (kGatherSmem - 1024) / kStageBytes;
+  static constexpr int kStages = kFit < 16 ? kFit : 16;
+  static constexpr int kBarOff = kStages * kStageBytes;        // full[S], empty[S]
+  static constexpr int kMetaOff = kBarOff + 2 * kStages * 8;   // per stage and slot: row, weight
+  static constexpr int kDynamic = kMetaOff + kStages * KC * 8 + 128;
+};
+
+template <typename T, int KC, bool GRAD>
+__global__ void __launch_bounds__(kGatherThreads, 2)
+moe_gather_kernel(const T* __restrict__ dy, const T* __restrict__ rows, int64_t num_rows, const int32_t* __restrict__ row_idx,
+                  const void* __restrict__ weights, int weight_dtype, T* __restrict__ out, void* __restrict__ dweights,
+                  uint32_t* __restrict__ marks, int64_t tokens, int topk, int64_t row_bytes) {
+  using L = GatherLayout<KC, GRAD>;
+  using E = Lanes<T, true>;
+  extern __shared__ uint8_t gather_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(gather_raw) + 127) & ~uintptr_t(127));
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::kBarOff);
+  uint64_t* empty = full + L::kStages;
+  int2* meta = reinterpret_cast<int2*>(smem + L::kMetaOff);
+  __shared__ int abort_word;
+  __shared__ float red[2][KC][kGatherWarps];
+  volatile int* abort_flag = &abort_word;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < L::kStages; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], kGatherWarps);
+    }
+    abort_word = 0;
+    fence_mbar_init();
+  }
+  __syncthreads();
+  const int segs = (int)((row_bytes + kGatherBytes - 1) / kGatherBytes);
+  int stage = 0;
+  uint32_t phase = 0;
+
+  if (warp == kGatherWarps) {
+    // ------------------------------------------------------------ producer: lane k copies slot k, lane KC copies dy
+    int next = -1;
+    float next_w = 1.0f;
+    auto look = [&](int64_t t) {
+      next = lane < topk && t < tokens ? row_idx[t * topk + lane] : -1;
+      if (weights != nullptr && lane < topk && t < tokens) next_w = load_as_f32(weights, weight_dtype, t * topk + lane);
+    };
+    look(blockIdx.x);
+    bool ok = true;
+    for (int64_t t = blockIdx.x; t < tokens && ok; t += gridDim.x) {
+      const int64_t row = next < num_rows ? next : -1;
+      const float w = next_w;
+      look(t + gridDim.x);
+      const uint8_t* src = nullptr;
+      if (row >= 0) {
+        src = reinterpret_cast<const uint8_t*>(rows) + row * row_bytes;
+        if (GRAD && marks != nullptr) {
+          const uint32_t bit = 1u << (row & 31);
+          if (atomicOr(marks + (row >> 5), bit) & bit) record_device_error(kDevRowTwice);
+        }
+      }
+      if (GRAD && lane == KC) src = reinterpret_cast<const uint8_t*>(dy) + t * row_bytes;
+      const int copies = __popc(__ballot_sync(0xffffffffu, src != nullptr));
+      for (int sg = 0; sg < segs; ++sg) {
+        const uint32_t bytes = (uint32_t)min((int64_t)kGatherBytes, row_bytes - (int64_t)sg * kGatherBytes);
+        ok = __all_sync(0xffffffffu, mbar_wait(&empty[stage], phase ^ 1, abort_flag, kDevTimeoutProducer));
+        if (!ok) break;
+        if (lane < KC) meta[stage * KC + lane] = make_int2((int)row, __float_as_int(w));
+        __syncwarp();
+        if (lane == 0) mbar_arrive_expect_tx(&full[stage], bytes * copies);
+        __syncwarp();
+        if (src != nullptr)
+          bulk_load(smem + stage * L::kStageBytes + lane * kGatherBytes, src + (int64_t)sg * kGatherBytes, bytes, &full[stage]);
+        if (++stage == L::kStages) { stage = 0; phase ^= 1; }
+      }
+    }
+    // Give copies that are still in flight time to land before shared memory is released.
+    if (!ok)
+      for (int i = 0; i < 200; ++i) __nanosleep(1000);
+  } else {
+    // ------------------------------------------------------------ eight warps: one vector of every row a thread
+    bool ok = true;
+    int par = 0;
+    for (int64_t t = blockIdx.x; t < tokens; t += gridDim.x, par ^= 1) {
+      float dot[KC];
+#pragma unroll
+      for (int k = 0; k < KC; ++k) dot[k] = 0.0f;
+      for (int sg = 0; sg < segs; ++sg) {
+        ok = mbar_wait(&full[stage], phase, abort_flag, kDevTimeoutEpilogue) && ok;
+        const int64_t at = (int64_t)sg * kGatherBytes + threadIdx.x * 16;
+        if (ok && at < row_bytes) {
+          const uint8_t* in = smem + stage * L::kStageBytes + threadIdx.x * 16;
+          if constexpr (GRAD) {
+            float g[E::N];
+            E::unpack(*reinterpret_cast<const uint4*>(in + KC * kGatherBytes), g);
+#pragma unroll
+            for (int k = 0; k < KC; ++k) {
+              const int2 m = meta[stage * KC + k];
+              if (m.x < 0) continue;
+              const float w = __int_as_float(m.y);
+              float f[E::N];
+              E::unpack(*reinterpret_cast<const uint4*>(in + k * kGatherBytes), f);
+#pragma unroll
+              for (int j = 0; j < E::N; ++j) {
+                dot[k] = fmaf(f[j], g[j], dot[k]);
+                f[j] = w * g[j];
+              }
+              __stcs(reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(out) + m.x * row_bytes + at), E::pack(f));
+            }
+          } else {
+            float acc[E::N];
+#pragma unroll
+            for (int j = 0; j < E::N; ++j) acc[j] = 0.0f;
+#pragma unroll
+            for (int k = 0; k < KC; ++k) {
+              const int2 m = meta[stage * KC + k];
+              if (m.x < 0) continue;
+              const float w = __int_as_float(m.y);
+              float f[E::N];
+              E::unpack(*reinterpret_cast<const uint4*>(in + k * kGatherBytes), f);
+#pragma unroll
+              for (int j = 0; j < E::N; ++j) acc[j] = fmaf(w, f[j], acc[j]);
+            }
+            __stcs(reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(out) + t * row_bytes + at), E::pack(acc));
+          }
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&empty[stage]);
+        if (++stage == L::kStages) { stage = 0; phase ^= 1; }
+      }
+      if constexpr (GRAD) {
+#pragma unroll
+        for (int k = 0; k < KC; ++k) {
+#pragma unroll
+          for (int o = 16; o > 0; o >>= 1) dot[k] += __shfl_xor_sync(0xffffffffu, dot[k], o);
+          if (lane == 0) red[par][k][warp] = dot[k];
+        }
+        named_barrier_sync(1, 32 * kGatherWarps);
+        if (ok && (int)threadIdx.x < topk) {
+          float s = 0.0f;
+#pragma unroll
+          for (int i = 0; i < kGatherWarps; ++i) s += red[par][threadIdx.x][i];
+          store_from_f32(dweights, weight_dtype, t * topk + threadIdx.x, s);   // no row: nothing was added
+        }
+      }
+    }
+  }
+  __syncthreads();
+}
+
 template <typename VT>
 __global__ void __launch_bounds__(256)
 moe_clear_rows_kernel(const uint32_t* __restrict__ marks, VT* __restrict__ drows, int64_t num_rows, int64_t nvec) {
@@ -620,15 +839,19 @@ inline int element_bytes(int dtype) {
   }
 }
 
-// Launches the sort: one cluster whose size grows with the number of indices (a CTA sorts 16384 in a few
-// microseconds; more CTAs than that only add the cluster's barriers).
-template <typename IdT>
-int launch_sort(const RouteIds& r, int32_t* row_idx, int32_t* row_src, int64_t* expert_tokens, int cumulative, int32_t* valid_rows,
-                cudaStream_t st) {
+// Launches the sort: one cluster of a CTA for every 2048 indices, up to sixteen (the ballots of pass 2 keep an SM's
+// schedulers busy for about 4 us per 4096 indices, the cluster's barriers cost less).
+constexpr int kSortClusterMax = 16;
+
+template <typename IdT, int BITS>
+int launch_sort_bits(const RouteIds& r, int32_t* row_idx, int32_t* row_src, int64_t* expert_tokens, int cumulative, int32_t* valid_rows,
+                     cudaStream_t st) {
+  constexpr auto kern = moe_sort_kernel<IdT, BITS>;
   const int smem = (kSortWarps + 1) * r.experts * (int)sizeof(int);
-  if (int rc = ensure_dynamic_smem<moe_sort_kernel<IdT>>((kSortWarps + 1) * kMaxExperts * (int)sizeof(int), "moe_route (sort)")) return rc;
+  if (int rc = ensure_dynamic_smem<kern>((kSortWarps + 1) * kMaxExperts * (int)sizeof(int), "moe_route (sort)")) return rc;
+  if (int rc = ensure_wide_clusters<kern>("moe_route (sort)")) return rc;
   int ctas = 1;
-  while (ctas < 8 && (int64_t)ctas * 8192 < r.n) ctas *= 2;
+  while (ctas < kSortClusterMax && (int64_t)ctas * 2048 < r.n) ctas *= 2;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(ctas);
   cfg.blockDim = dim3(kSortThreads);
@@ -641,10 +864,18 @@ int launch_sort(const RouteIds& r, int32_t* row_idx, int32_t* row_src, int64_t* 
   attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  cudaError_t err = cudaLaunchKernelEx(&cfg, moe_sort_kernel<IdT>, static_cast<const IdT*>(r.ids), r.n, r.begin, r.experts, r.strict_limit,
+  cudaError_t err = cudaLaunchKernelEx(&cfg, kern, static_cast<const IdT*>(r.ids), r.n, r.begin, r.experts, r.strict_limit,
                                        row_idx, row_src, expert_tokens, cumulative, valid_rows);
   if (err != cudaSuccess) return fail(B200Q_ERR_LAUNCH, "moe_route (sort): %s", cudaGetErrorString(err));
   return check_launch("moe_route (sort)");
+}
+
+template <typename IdT>
+int launch_sort(const RouteIds& r, int32_t* row_idx, int32_t* row_src, int64_t* expert_tokens, int cumulative, int32_t* valid_rows,
+                cudaStream_t st) {
+  if (r.experts < 64) return launch_sort_bits<IdT, 6>(r, row_idx, row_src, expert_tokens, cumulative, valid_rows, st);
+  if (r.experts < 256) return launch_sort_bits<IdT, 8>(r, row_idx, row_src, expert_tokens, cumulative, valid_rows, st);
+  return launch_sort_bits<IdT, 11>(r, row_idx, row_src, expert_tokens, cumulative, valid_rows, st);
 }
 
 template <typename IdT, int BYTES>
@@ -664,9 +895,8 @@ int launch_copy(const b200q_moe_route_args& a, const RouteIds& r, int64_t row_by
   const int64_t segs = nvec == 0 ? 1 : ceil_div(nvec, 32 * U);
   const int64_t move_blocks = ceil_div(a.tokens * segs, 8), blocks = move_blocks + 2 * sm_count();
   B200Q_REQUIRE(blocks <= 0x7fffffffLL, B200Q_ERR_UNSUPPORTED, "moe_route: too many rows");
-  moe_copy_kernel<VT, U><<<(unsigned)blocks, 256, 0, st>>>(x, out, a.tokens, r.topk, nvec, (int)segs, a.out_rows, scale, a.out_scale, a.row_idx,
-                                                           valid_rows, move_blocks);
-  return check_launch("moe_route (copy)");
+  return launch_dependent(moe_copy_kernel<VT, U>, (unsigned)blocks, 256, st, "moe_route (copy)", x, out, a.tokens, r.topk, nvec, (int)segs, a.out_rows,
+                          scale, a.out_scale, static_cast<const int32_t*>(a.row_idx), static_cast<const int32_t*>(valid_rows), move_blocks);
 }
 
 template <typename IdT, typename T, typename ST, int ITERS>
@@ -680,12 +910,9 @@ int launch_route_quant_iters(const b200q_moe_route_args& a, const RouteIds& r, i
     return check_launch("moe_route (quantised, few tokens)");
   }
   if (int rc = launch_sort<IdT>(r, a.row_idx, row_src, a.expert_tokens, a.cumulative, valid_rows, st)) return rc;
-  int per_sm = 1;
-  cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, moe_quant_kernel<IdT, T, ST, ITERS>, threads, 0);
-  const int64_t cap = (int64_t)sm_count() * (per_sm > 0 ? per_sm : 1);
-  moe_quant_kernel<IdT, T, ST, ITERS><<<(unsigned)(r.n < cap ? r.n : cap), threads, 0, st>>>(r, x, a.hidden, sm, (int)a.scale_rows, out, a.out_scale,
-                                                                                             row_src);
-  return check_launch("moe_route (quantised)");
+  const int64_t cap = (int64_t)sm_count() * resident_ctas<moe_quant_kernel<IdT, T, ST, ITERS>>(threads);
+  return launch_dependent(moe_quant_kernel<IdT, T, ST, ITERS>, (unsigned)(r.n < cap ? r.n : cap), threads, st, "moe_route (quantised)", r, x, a.hidden, sm,
+                          (int)a.scale_rows, out, a.out_scale, static_cast<const int32_t*>(row_src));
 }
 
 template <typename IdT, typename T, typename ST>
@@ -746,9 +973,39 @@ int launch_combine(const void* rows, int64_t num_rows, const int32_t* row_idx, c
   return check_launch("moe_combine");
 }
 
+// The pipeline pays from a few tokens a CTA on and for rows of at least a stage's length; up to eight slots.
+inline bool use_gather(int64_t tokens, int64_t topk, int64_t row_bytes) {
+  return topk <= 8 && tokens >= 4 * sm_count() && row_bytes >= 1024;
+}
+
+template <typename T, int KC, bool GRAD>
+int launch_gather(const void* dy, const void* rows, int64_t num_rows, const int32_t* row_idx, const void* w, int w_dtype, void* out, void* dw,
+                  uint32_t* marks, int64_t tokens, int topk, int64_t row_bytes, cudaStream_t st) {
+  using L = GatherLayout<KC, GRAD>;
+  constexpr auto kern = moe_gather_kernel<T, KC, GRAD>;
+  if (int rc = ensure_dynamic_smem<kern>(L::kDynamic, "moe_combine")) return rc;
+  const int64_t cap = 2 * (int64_t)sm_count();
+  kern<<<(unsigned)(tokens < cap ? tokens : cap), kGatherThreads, L::kDynamic, st>>>(
+      static_cast<const T*>(dy), static_cast<const T*>(rows), num_rows, row_idx, w, w_dtype, static_cast<T*>(out), dw, marks, tokens, topk, row_bytes);
+  return check_launch(GRAD ? "moe_combine_grad" : "moe_combine");
+}
+
+template <typename T, bool GRAD>
+int gather(const void* dy, const void* rows, int64_t num_rows, const int32_t* row_idx, const void* w, int w_dtype, void* out, void* dw,
+           uint32_t* marks, int64_t tokens, int topk, int64_t row_bytes, cudaStream_t st) {
+#define B200Q_GATHER(KC) return launch_gather<T, KC, GRAD>(dy, rows, num_rows, row_idx, w, w_dtype, out, dw, marks, tokens, topk, row_bytes, st)
+  if (topk == 1) B200Q_GATHER(1);
+  if (topk == 2) B200Q_GATHER(2);
+  if (topk <= 4) B200Q_GATHER(4);
+  B200Q_GATHER(8);
+#undef B200Q_GATHER
+}
+
 template <typename T>
 int combine(const void* rows, int64_t num_rows, const int32_t* row_idx, const void* w, int w_dtype, void* out, int64_t tokens, int topk,
             int64_t hidden, cudaStream_t st) {
+  if (chunk_bytes(hidden * (int)sizeof(T), {rows, out}) == 16 && use_gather(tokens, topk, hidden * (int)sizeof(T)))
+    return gather<T, false>(nullptr, rows, num_rows, row_idx, w, w_dtype, out, nullptr, nullptr, tokens, topk, hidden * (int)sizeof(T), st);
   if (chunk_bytes(hidden * (int)sizeof(T), {rows, out}) == 16)
     return launch_combine<T, true>(rows, num_rows, row_idx, w, w_dtype, out, tokens, topk, hidden, st);
   return launch_combine<T, false>(rows, num_rows, row_idx, w, w_dtype, out, tokens, topk, hidden, st);
@@ -764,7 +1021,11 @@ int launch_combine_grad(const b200q_moe_combine_grad_args& a, cudaStream_t st) {
   uint32_t* marks = static_cast<uint32_t*>(a.workspace);
   cudaError_t err = cudaMemsetAsync(marks, 0, (size_t)ceil_div(a.num_rows, 32) * 4, st);
   if (err != cudaSuccess) return fail(B200Q_ERR_LAUNCH, "moe_combine_grad: memset: %s", cudaGetErrorString(err));
-  if (a.tokens > 0) {
+  if (VEC && a.dweights != nullptr && use_gather(a.tokens, a.topk, a.hidden * (int)sizeof(T))) {
+    if (int rc = gather<T, true>(dy, rows, a.num_rows, a.row_idx, a.weights, a.weight_dtype, drows, a.dweights, marks, a.tokens, (int)a.topk,
+                                 a.hidden * (int)sizeof(T), st))
+      return rc;
+  } else if (a.tokens > 0) {
     const int threads = nvec >= 256 ? 256 : (int)(nvec <= 32 ? 32 : ceil_div(nvec, 32) * 32);
 #define B200Q_COMBINE_GRAD(KC)                                                                                                       \
   moe_combine_grad_kernel<T, VEC, KC><<<(unsigned)a.tokens, threads, 0, st>>>(dy, rows, a.num_rows, a.row_idx, a.weights, a.weight_dtype, \

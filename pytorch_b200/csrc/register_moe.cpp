@@ -327,12 +327,12 @@ b200q_gated_norm_args norm_args(const char* op, const Tensor& x, const Tensor& r
                                 double residual_scale, double epsilon) {
   b200q_gated_norm_args a{};
   a.x = x.data_ptr(); a.residual = residual.data_ptr(); a.dtype = dtype_enum(x.scalar_type());
-  a.gamma = gamma.data_ptr(); a.gamma_dtype = dtype_enum(gamma.scalar_type());
-  if (post.defined()) { a.post_gamma = post.data_ptr(); a.post_gamma_dtype = dtype_enum(post.scalar_type()); }
+  a.gamma = gamma.data_ptr(); a.param_dtype = dtype_enum(gamma.scalar_type());
+  if (post.defined()) a.post_gamma = post.data_ptr();
   a.gate_rows = 1;
   if (gate.defined()) {
     const GateSpec g = gate_spec(op, x, gate);
-    a.gate = gate.data_ptr(); a.gate_dtype = dtype_enum(gate.scalar_type());
+    a.gate = gate.data_ptr();
     a.gate_per_row = g.per_row ? 1 : 0;
     a.gate_rows = g.rows;
   }
@@ -355,6 +355,14 @@ void norm_check(const char* op, const Tensor& x, const Tensor& residual, const T
   if (post.has_value()) vector(*post, "post_gamma");
   if (gate.has_value()) gate_spec(op, x, *gate);
 }
+
+// The kernels take the parameters all in x's dtype or all in float32: any mix is brought to float32 first.
+at::ScalarType param_type(const Tensor& x, const Tensor& gamma, const optional<Tensor>& post, const optional<Tensor>& gate) {
+  auto differs = [&](const optional<Tensor>& t) { return t.has_value() && t->scalar_type() != gamma.scalar_type(); };
+  const bool one_type = !differs(post) && !differs(gate);
+  return one_type && gamma.scalar_type() == x.scalar_type() ? x.scalar_type() : at::kFloat;
+}
+Tensor as_param(const optional<Tensor>& t, at::ScalarType type) { return t.has_value() ? t->to(type).contiguous() : Tensor(); }
 
 Tensor contiguous_or_none(const optional<Tensor>& t) { return t.has_value() ? t->contiguous() : Tensor(); }
 
@@ -383,7 +391,8 @@ NormOutputs norm_cuda(const Tensor& x, const Tensor& residual, const Tensor& gam
   c10::cuda::CUDAGuard guard(x.device());
   surface_device_error(op, x);
   auto [y, rstd, h, post_rstd] = norm_meta(x, residual, gamma, post, gate, residual_scale, epsilon);
-  Tensor xc = x.contiguous(), rc = residual.contiguous(), wc = gamma.contiguous(), pc = contiguous_or_none(post), gc = contiguous_or_none(gate);
+  const at::ScalarType pt = param_type(x, gamma, post, gate);
+  Tensor xc = x.contiguous(), rc = residual.contiguous(), wc = as_param(gamma, pt), pc = as_param(post, pt), gc = as_param(gate, pt);
   b200q_gated_norm_args a = norm_args(op, xc, rc, wc, pc, gc, residual_scale, epsilon);
   a.y = y.data_ptr(); a.h = h.data_ptr();
   a.rstd = static_cast<float*>(rstd.data_ptr());
@@ -414,8 +423,9 @@ std::tuple<Tensor, Tensor, Tensor> norm_quant_cuda(const Tensor& x, const Tensor
   surface_device_error(op, x);
   auto [y, scale, h] = norm_quant_meta(x, residual, gamma, post, gate, smooth, residual_scale, epsilon);
   if (x.size(-1) == 0) return {y, scale.zero_(), h};
-  Tensor xc = x.contiguous(), rc = residual.contiguous(), wc = gamma.contiguous(), pc = contiguous_or_none(post), gc = contiguous_or_none(gate);
-  Tensor sc = contiguous_or_none(smooth);
+  const at::ScalarType pt = param_type(x, gamma, post, gate);
+  Tensor xc = x.contiguous(), rc = residual.contiguous(), wc = as_param(gamma, pt), pc = as_param(post, pt), gc = as_param(gate, pt);
+  Tensor sc = as_param(smooth, smooth.has_value() && smooth->scalar_type() == x.scalar_type() ? x.scalar_type() : at::kFloat);
   b200q_gated_norm_args a = norm_args(op, xc, rc, wc, pc, gc, residual_scale, epsilon);
   a.y = y.data_ptr(); a.h = h.data_ptr();
   a.scale = static_cast<float*>(scale.data_ptr());
@@ -458,9 +468,13 @@ NormGrads norm_grad_cuda(const Tensor& dy, const optional<Tensor>& dh, const Ten
   c10::cuda::CUDAGuard guard(x.device());
   surface_device_error(op, x);
   auto [dx, dres, dgamma, dpost, dgate] = norm_grad_meta(dy, dh, x, residual, gamma, rstd, post, gate, post_rstd, residual_scale);
-  Tensor xc = x.contiguous(), rc = residual.contiguous(), wc = gamma.contiguous(), pc = contiguous_or_none(post), gc = contiguous_or_none(gate);
+  const at::ScalarType pt = param_type(x, gamma, post, gate);
+  Tensor xc = x.contiguous(), rc = residual.contiguous(), wc = as_param(gamma, pt), pc = as_param(post, pt), gc = as_param(gate, pt);
   Tensor yc = dy.contiguous(), hc = contiguous_or_none(dh), sc = rstd.contiguous(), qc = contiguous_or_none(post_rstd);
   if (x.numel() == 0 && gate.has_value()) dgate.zero_();
+  // Gradients of parameters that had to change their type are computed in float32 and rounded afterwards.
+  auto as_grad = [&](const Tensor& t) { return t.scalar_type() == pt ? t : at::empty(t.sizes(), t.options().dtype(pt)); };
+  Tensor gw = as_grad(dgamma), gp = post.has_value() ? as_grad(dpost) : dpost, gg = gate.has_value() ? as_grad(dgate) : dgate;
   b200q_gated_norm_args a = norm_args(op, xc, rc, wc, pc, gc, residual_scale, 0.0);
   a.rstd = static_cast<float*>(sc.data_ptr());
   if (post.has_value()) a.post_rstd = static_cast<float*>(qc.data_ptr());
@@ -468,11 +482,14 @@ NormGrads norm_grad_cuda(const Tensor& dy, const optional<Tensor>& dh, const Ten
   b200q_gated_norm_grads g{};
   g.dy = yc.data_ptr();
   if (hc.defined()) g.dh = hc.data_ptr();
-  g.dx = dx.data_ptr(); g.dresidual = dres.data_ptr(); g.dgamma = dgamma.data_ptr();
-  if (post.has_value()) g.dpost_gamma = dpost.data_ptr();
-  if (gate.has_value()) g.dgate = dgate.data_ptr();
+  g.dx = dx.data_ptr(); g.dresidual = dres.data_ptr(); g.dgamma = gw.data_ptr();
+  if (post.has_value()) g.dpost_gamma = gp.data_ptr();
+  if (gate.has_value()) g.dgate = gg.data_ptr();
   if (ws.defined()) { g.workspace = ws.data_ptr(); g.workspace_bytes = ws.numel(); }
   check_status(b200q_gated_norm_grad(&a, &g, stream_of(x)), op);
+  if (!gw.is_same(dgamma)) dgamma.copy_(gw);
+  if (!gp.is_same(dpost)) dpost.copy_(gp);
+  if (!gg.is_same(dgate) && x.numel() > 0) dgate.copy_(gg);
   return {dx, dres, dgamma, dpost, dgate};
 }
 

@@ -169,7 +169,7 @@ def test_gated_norm_argument_checks(lib):
     def args(**kw):
         a = cabi.GatedNormArgs()
         a.x = a.residual = a.gamma = a.y = a.h = p
-        a.dtype, a.gamma_dtype, a.rows, a.width, a.gate_rows = cabi.BF16, cabi.BF16, 2, 16, 1
+        a.dtype, a.param_dtype, a.rows, a.width, a.gate_rows = cabi.BF16, cabi.BF16, 2, 16, 1
         for k, v in kw.items():
             setattr(a, k, v)
         return a
@@ -178,7 +178,7 @@ def test_gated_norm_argument_checks(lib):
     assert lib.b200q_gated_norm(None, None) == cabi.ERR_BAD_ARG
     for kw, status, what in [
             (dict(rows=-1), cabi.ERR_BAD_ARG, "negative"), (dict(dtype=cabi.I8), cabi.ERR_UNSUPPORTED, "bf16, f16 or f32"),
-            (dict(width=16385), cabi.ERR_UNSUPPORTED, "at most 16384"), (dict(gamma_dtype=cabi.I8), cabi.ERR_UNSUPPORTED, "gamma"),
+            (dict(width=16385), cabi.ERR_UNSUPPORTED, "at most 16384"), (dict(param_dtype=cabi.F16), cabi.ERR_UNSUPPORTED, "gamma"),
             (dict(gate=p, gate_rows=0), cabi.ERR_BAD_ARG, "gate_rows"), (dict(gate=p, gate_rows=2, gate_per_row=1), cabi.ERR_UNSUPPORTED, "one row"),
             (dict(smooth=p), cabi.ERR_BAD_ARG, "quantised"), (dict(scale=p, smooth=p, smooth_dtype=cabi.I8), cabi.ERR_UNSUPPORTED, "smooth"),
             (dict(x=None), cabi.ERR_BAD_ARG, "NULL"), (dict(h=p + 1), cabi.ERR_BAD_ARG, "misaligned"), (dict(rstd=p + 2), cabi.ERR_BAD_ARG, "misaligned")]:
