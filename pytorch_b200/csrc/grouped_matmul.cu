@@ -12,11 +12,12 @@
 // multiple of 128 or 256 rows.  Every CTA builds the same list of non-empty groups and their tiles from the group list in
 // shared memory and walks it with a stride of the grid; token tiles of one weight tile are neighbours, so a weight tile
 // is fetched from HBM once and its other readers find it in L2.
-//   warp 0      TMA producer: a 128 x 128-byte weight tile and the tokens' rows (boxes of 256 / 64 / 16 rows) a stage
+//   warp 0      TMA producer: a 128 x 128-byte weight tile and the tokens' rows a stage, one copy each (a tensor map for
+//               every number of rows a tile can have)
 //   warp 1      MMA issuer; accumulators in TMEM, two buffers, so that one tile's epilogue overlaps the next one's products
-//   warps 2-5   epilogue: a lane owns a channel; neighbouring lanes exchange tokens so that a lane stores two channels
-// Two instantiations: CTA pairs with up to 256 tokens a tile (bound by the tensor cores), and single CTAs with up to 64
-// and a deeper ring (few rows an expert: bound by reading the weights).
+//   warps 2-9   epilogue: a lane owns a channel; neighbouring lanes exchange tokens so that a lane stores two channels
+// Three instantiations: CTA pairs and single CTAs with up to 256 tokens a tile (bound by the tensor cores), and single CTAs
+// with up to 64 and a deeper ring (few rows an expert: bound by reading the weights).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -30,6 +31,22 @@ namespace b200q {
 namespace {
 
 constexpr int kMaxGroups = 1024;
+constexpr int kGroupedEpiThreads = 256;
+constexpr int kGroupedThreads = 64 + kGroupedEpiThreads;
+
+// AND of a predicate over the epilogue warps (named barrier 1): a barrier, and the common decision whether to go on.
+__device__ __forceinline__ bool grouped_epilogue_all(bool pred) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.u32 p, %1, 0;\n\t"
+      "bar.red.and.pred q, 1, %2, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(r)
+      : "r"((uint32_t)pred), "r"(kGroupedEpiThreads)
+      : "memory");
+  return r != 0;
+}
 
 struct GroupedArgs {
   const int64_t* group_list;   // [groups] ends (cumulative) or counts
@@ -44,6 +61,8 @@ struct GroupedArgs {
   void* out;                   // [m, n]
   int scale_dtype, bias_dtype, out_dtype;
 };
+
+__device__ __forceinline__ bool aligned_word(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3) == 0; }
 
 // The non-empty groups, in order.
 struct GroupTable {
@@ -109,23 +128,57 @@ __device__ void build_group_table(const GroupedArgs& a, GroupTable& t, int lane)
   }
 }
 
-// A unit's place: group, channel tile, rows [row0, row0 + live) computed as `width` columns.
+// A unit's place: group, channel tile, rows [row0, row0 + live) computed as `width` columns.  A group's rows, in steps of
+// STEP, are dealt out evenly: the first tiles get one step more, and only the last step of the group can have idle columns.
 struct Unit {
   int group, tile_n, row0, live, width;
 };
 template <int MAX_TOKENS, int STEP>
 __device__ __forceinline__ Unit find_unit(const GroupTable& t, int u, int& at) {
   while (at + 1 < t.count && u >= t.unit[at + 1]) ++at;
-  const int rows = t.rows[at], tiles = (rows + MAX_TOKENS - 1) / MAX_TOKENS;
-  const int per = (rows + tiles - 1) / tiles;                 // rows a tile; the last one may have fewer
-  const int local = u - t.unit[at], tt = local % tiles;
+  const int rows = t.rows[at], tiles = (rows + MAX_TOKENS - 1) / MAX_TOKENS, steps = (rows + STEP - 1) / STEP;
+  const int local = u - t.unit[at], tile_n = local / tiles, tt = local - tile_n * tiles;
+  const int per = steps / tiles, more = steps - per * tiles;
+  const int first = (tt * per + min(tt, more)) * STEP;
   Unit r;
   r.group = t.group[at];
-  r.tile_n = local / tiles;
-  r.row0 = t.start[at] + tt * per;
-  r.live = min(per, rows - tt * per);
-  r.width = (r.live + STEP - 1) / STEP * STEP;
+  r.tile_n = tile_n;
+  r.row0 = t.start[at] + first;
+  r.width = (per + (tt < more ? 1 : 0)) * STEP;
+  r.live = min(r.width, rows - first);
   return r;
+}
+
+// Finishes CH accumulator columns (tokens) of a lane's channel for a 16-bit output without bias, all columns live: scale and
+// row scale as packed two-wide products (each rounded like the scalar one), one conversion for two tokens, one exchange with
+// the neighbouring lane.  Even lanes then hold token j of channels n, n + 1, odd lanes token j + 1 of channels n - 1, n: a
+// 32-bit store each.  The tensor cores keep shared memory and its crossbar busy, so every LDS and shuffle here costs them
+// time: four row scales a load, half a shuffle an element.
+template <bool BF16, int CH>
+__device__ __forceinline__ void store_columns(const uint32_t (&r)[CH], const float* row_scale, float sc, bool scaled, uint8_t* out, int64_t pitch,
+                                              bool live) {
+  const float2 sc2 = make_float2(sc, sc);
+  const uint32_t pick = (threadIdx.x & 1) ? 0x3276u : 0x5410u;
+#pragma unroll
+  for (int j = 0; j < CH; j += 4) {
+    float4 rs = make_float4(1.0f, 1.0f, 1.0f, 1.0f);
+    if (scaled) rs = *reinterpret_cast<const float4*>(row_scale + j);
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      float2 v = __fmul2_rn(make_float2(__int2float_rn((int)r[j + 2 * q]), __int2float_rn((int)r[j + 2 * q + 1])), sc2);
+      if (scaled) v = __fmul2_rn(v, q == 0 ? make_float2(rs.x, rs.y) : make_float2(rs.z, rs.w));
+      uint32_t w;
+      if constexpr (BF16) {
+        const __nv_bfloat162 h = __float22bfloat162_rn(v);
+        w = *reinterpret_cast<const uint32_t*>(&h);
+      } else {
+        const __half2 h = __float22half2_rn(v);
+        w = *reinterpret_cast<const uint32_t*>(&h);
+      }
+      w = __byte_perm(w, __shfl_xor_sync(0xffffffffu, w, 1), pick);
+      if (live) *reinterpret_cast<uint32_t*>(out + (j + 2 * q) * pitch) = w;
+    }
+  }
 }
 
 template <int CTAS, int MAX_TOKENS, int STAGES>
@@ -135,20 +188,23 @@ struct GroupedLayout {
   static constexpr int kTiles = STAGES * (kATileBytes + kBTileBytes);
   static constexpr int kBarOff = kTiles;                       // full[S], empty[S], tfull[2], tempty[2]
   static constexpr int kMiscOff = kBarOff + (2 * STAGES + 4) * 8;
-  static constexpr int kRowScaleOff = kMiscOff + 16;           // MAX_TOKENS floats
-  static constexpr int kTableOff = kRowScaleOff + MAX_TOKENS * 4;
+  static constexpr int kRowScaleOff = kMiscOff + 16;           // 2 x MAX_TOKENS floats
+  static constexpr int kTableOff = kRowScaleOff + 2 * MAX_TOKENS * 4;
   static constexpr int kTotal = kTableOff + (int)sizeof(GroupTable);
   static constexpr int kDynamic = kTotal + 1024;
 };
 
+template <int B_ROWS>
 struct GroupedMaps {
   CUtensorMap w;               // weight [groups, n, k]: box 1 x 128 x 128
-  CUtensorMap x[3];            // x [m, k]: boxes of kBRows, 64 and 16 rows
+  CUtensorMap x[B_ROWS / 16];  // x [m, k]: a box for every number of rows a tile can have, 16 (i + 1)
 };
 
-template <int CTAS, int MAX_TOKENS, int STAGES>
+// STREAM: weights are read once (evicted first from L2, so that they do not push out the tokens; measured 144 us for 56
+// weights of 4096 x 4096 where builds without the hint took between 144 and 160).
+template <int CTAS, int MAX_TOKENS, int STAGES, bool STREAM>
 __device__ __forceinline__ void
-grouped_matmul_body(const GroupedMaps& maps, const GroupedArgs& a) {
+grouped_matmul_body(const GroupedMaps<MAX_TOKENS / CTAS>& maps, const GroupedArgs& a) {
   using L = GroupedLayout<CTAS, MAX_TOKENS, STAGES>;
   constexpr int kStep = 16 * CTAS;
   constexpr uint32_t kTmemCols = 2 * MAX_TOKENS;
@@ -179,12 +235,11 @@ grouped_matmul_body(const GroupedMaps& maps, const GroupedArgs& a) {
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&tfull[i], 1);
-      mbar_init(&tempty[i], CTAS * (kEpiThreads / 32));            // epilogue warps of all CTAs
+      mbar_init(&tempty[i], CTAS * (kGroupedEpiThreads / 32));     // epilogue warps of all CTAs
     }
     *abort_flag = 0;
     fence_mbar_init();
     prefetch_tensormap(&maps.w);
-    for (int i = 0; i < 3; ++i) prefetch_tensormap(&maps.x[i]);
   }
   if (warp == 1) {
     if constexpr (CTAS == 2) {
@@ -206,6 +261,7 @@ grouped_matmul_body(const GroupedMaps& maps, const GroupedArgs& a) {
   if (warp == 0) {
     // ------------------------------------------------------------ TMA producer (every CTA loads its own rows)
     if (lane == 0) {
+      const uint64_t once = policy_evict_first();
       int stage = 0, at = 0;
       uint32_t phase = 0;
       bool ok = true;
@@ -220,14 +276,9 @@ grouped_matmul_body(const GroupedMaps& maps, const GroupedArgs& a) {
           if (rank == 0) mbar_arrive_expect_tx(&full[stage], bytes);
           uint32_t bar = smem_u32(&full[stage]);
           if constexpr (CTAS == 2) bar = map_to_cta(bar, 0);
-          tma_load_3d<CTAS>(dst_a, &maps.w, bar, kb * kBK, n0, t.group);
-          int r = 0;
-          if (b_rows == L::kBRows) {
-            tma_load_2d_to<CTAS>(dst_b, &maps.x[0], bar, kb * kBK, m0);
-            r = L::kBRows;
-          }
-          for (; r + 64 <= b_rows; r += 64) tma_load_2d_to<CTAS>(dst_b + r * kBK, &maps.x[1], bar, kb * kBK, m0 + r);
-          for (; r < b_rows; r += 16) tma_load_2d_to<CTAS>(dst_b + r * kBK, &maps.x[2], bar, kb * kBK, m0 + r);
+          if constexpr (STREAM) tma_load_3d_hint(dst_a, &maps.w, bar, kb * kBK, n0, t.group, once);
+          else tma_load_3d<CTAS>(dst_a, &maps.w, bar, kb * kBK, n0, t.group);
+          tma_load_2d_to<CTAS>(dst_b, &maps.x[b_rows / 16 - 1], bar, kb * kBK, m0);
           if (++stage == STAGES) { stage = 0; phase ^= 1; }
         }
       }
@@ -277,55 +328,78 @@ grouped_matmul_body(const GroupedMaps& maps, const GroupedArgs& a) {
       }
     }
   } else {
-    // ---------------------------------------------------------------- epilogue: this CTA's 128 channels, all columns
-    constexpr int CH = kStep >= 32 ? 32 : 16;                      // accumulator columns per tcgen05.ld
+    // ---------------------------------------------------------------- epilogue: this CTA's 128 channels, all columns.
+    // Two warps a quadrant of TMEM lanes, chunks of CH columns in turn.  The next tile's scales are loaded during this tile's
+    // work; one barrier a tile stands between the row scales' writers and readers (two buffers) and makes the warps agree on
+    // whether the accumulator came.
+    constexpr int CH = 32;                                         // accumulator columns per tcgen05.ld
     const int et = threadIdx.x - 64;
-    const int quad = warp & 3;                                     // TMEM lane quadrant this warp may read
+    const int quad = warp & 3, half = (warp - 2) >> 2;
     const bool two_byte = a.out_dtype == B200Q_BF16 || a.out_dtype == B200Q_F16;
-    const bool words = two_byte && a.n % 2 == 0;                   // two channels of a row make an aligned word
+    const bool words = two_byte && a.n % 2 == 0 && aligned_word(a.out);   // two channels of a row make an aligned word
+    const bool plain = words && a.bias == nullptr;
+    const bool scaled = a.row_scale != nullptr;
     Epi e{};
     e.scale = a.scale; e.scale_dtype = a.scale_dtype;
     e.bias = a.bias; e.bias_dtype = a.bias_dtype;
     e.out = a.out; e.out_dtype = a.out_dtype;
-    e.flags = (a.row_scale != nullptr ? (uint32_t)kHasPt : 0u) |
+    e.flags = (scaled ? (uint32_t)kHasPt : 0u) |
               (a.bias != nullptr ? (a.bias_dtype == B200Q_I32 ? (uint32_t)kHasIntBias : (uint32_t)kHasFloatBias) : 0u);
+    const int lane_n = rank * kTileA + quad * 32 + lane;           // this lane's channel within a tile
     int buf = 0, at = 0;
     uint32_t tphase = 0;
+    Unit t{};
+    float sc = 0.0f, rs = 1.0f;
+    auto look = [&](int u) {                                       // unit u's place, this lane's scale and row scale
+      if (u >= units) return;
+      t = find_unit<MAX_TOKENS, kStep>(table, u, at);
+      const int n = t.tile_n * CTAS * kTileA + lane_n;
+      sc = n < a.n && a.scale != nullptr ? load_scale(e, (int64_t)t.group * a.n + n) : 0.0f;
+      rs = scaled && et < t.live ? __ldg(a.row_scale + t.row0 + et) : 1.0f;
+    };
+    look(first);
     for (int u = first; u < units; u += stride) {
-      const Unit t = find_unit<MAX_TOKENS, kStep>(table, u, at);
-      const int n = (t.tile_n * CTAS + rank) * kTileA + quad * 32 + lane;
+      float* scales = row_scale + buf * MAX_TOKENS;
+      if (et < MAX_TOKENS) scales[et] = rs;
+      const Unit now = t;
+      const float sc_now = sc;
+      const int n = now.tile_n * CTAS * kTileA + lane_n;
       const bool nv = n < a.n;
-      const int64_t gn = (int64_t)t.group * a.n + n;
-      const float sc = nv && a.scale != nullptr ? load_scale(e, gn) : 0.0f, fb = nv ? load_float_bias(e, gn) : 0.0f;
+      const int64_t gn = (int64_t)now.group * a.n + n;
+      const float fb = nv ? load_float_bias(e, gn) : 0.0f;
       const int ib = nv ? load_int_bias(e, gn) : 0;
-      named_barrier_sync(1, kEpiThreads);                          // the last tile's row scales have been read
-      for (int i = et; i < t.live; i += kEpiThreads) row_scale[i] = a.row_scale != nullptr ? __ldg(a.row_scale + t.row0 + i) : 1.0f;
-      named_barrier_sync(1, kEpiThreads);
-      if (!epilogue_all(mbar_wait(&tfull[buf], tphase, abort_flag, kDevTimeoutEpilogue))) break;
+      if (!grouped_epilogue_all(mbar_wait(&tfull[buf], tphase, abort_flag, kDevTimeoutEpilogue))) break;
       tc_fence_after();
+      look(u + stride);
       const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + buf * MAX_TOKENS;
 #pragma unroll 1
-      for (int c = 0; c < t.live; c += CH) {
+      for (int c = half * CH; c < now.live; c += 2 * CH) {
         uint32_t r[CH];
         __syncwarp();
         tmem_ld_chunk<CH>(taddr + c, r);
         tmem_ld_wait();
+        if (plain && c + CH <= now.live) {
+          // this lane's first word: token c (even lanes) or c + 1, channels n & ~1 and the next
+          uint8_t* at_out = static_cast<uint8_t*>(a.out) + ((now.row0 + c + (lane & 1)) * (int64_t)a.n + (n & ~1)) * 2;
+          if (a.out_dtype == B200Q_BF16) store_columns<true, CH>(r, scales + c, sc_now, scaled, at_out, (int64_t)a.n * 2, nv);
+          else store_columns<false, CH>(r, scales + c, sc_now, scaled, at_out, (int64_t)a.n * 2, nv);
+          continue;
+        }
 #pragma unroll
         for (int j = 0; j < CH; j += 2) {
-          const float v0 = dequant((int)r[j], ib, sc, row_scale[min(c + j, MAX_TOKENS - 1)], fb, 0.0f, e.flags);
-          const float v1 = dequant((int)r[j + 1], ib, sc, row_scale[min(c + j + 1, MAX_TOKENS - 1)], fb, 0.0f, e.flags);
-          const int64_t row = t.row0 + c + j;
+          if (c + j >= now.live) break;                            // the same in every lane
+          const float v0 = dequant((int)r[j], ib, sc_now, scales[c + j], fb, 0.0f, e.flags);
+          const float v1 = dequant((int)r[j + 1], ib, sc_now, scales[c + j + 1], fb, 0.0f, e.flags);
+          const int64_t row = now.row0 + c + j;
           if (words) {
-            // even lanes finish token j for channels n, n+1; odd lanes token j+1 for n-1, n
             const uint32_t b0 = to_bits16(v0, a.out_dtype), b1 = to_bits16(v1, a.out_dtype);
             const uint32_t other = __shfl_xor_sync(0xffffffffu, (lane & 1) ? b0 : b1, 1);
             const uint32_t w = (lane & 1) ? (other | (b1 << 16)) : (b0 | (other << 16));
-            const int jj = c + j + (lane & 1);
-            if (jj < t.live && nv)                                 // n is even: n < N for both or for neither
+            if (c + j + (lane & 1) < now.live && nv)               // n is even: n < N for both or for neither
               *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.out) + (row + (lane & 1)) * a.n + (n & ~1)) = w;
           } else if (nv) {
-            if (c + j < t.live) store_one(e, row * a.n + n, (int)r[j], ib, v0);
-            if (c + j + 1 < t.live) store_one(e, (row + 1) * a.n + n, (int)r[j + 1], ib, v1);
+            store_one(e, row * a.n + n, (int)r[j], ib, v0);
+            if (c + j + 1 < now.live) store_one(e, (row + 1) * a.n + n, (int)r[j + 1], ib, v1);
           }
         }
       }
@@ -340,7 +414,7 @@ grouped_matmul_body(const GroupedMaps& maps, const GroupedArgs& a) {
     // Rows behind the last group.
     const int ob = two_byte ? 2 : 4;
     for (int64_t row = (int64_t)table.total + blockIdx.x; row < a.m; row += gridDim.x)
-      for (int c = et; c < a.n; c += kEpiThreads) {
+      for (int c = et; c < a.n; c += kGroupedEpiThreads) {
         if (ob == 2) static_cast<uint16_t*>(a.out)[row * a.n + c] = 0;
         else static_cast<uint32_t*>(a.out)[row * a.n + c] = 0;
       }
@@ -359,14 +433,14 @@ grouped_matmul_body(const GroupedMaps& maps, const GroupedArgs& a) {
 }
 
 template <int MAX_TOKENS, int STAGES>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
-grouped_matmul_pair_kernel(const __grid_constant__ GroupedMaps maps, const GroupedArgs a) {
-  grouped_matmul_body<2, MAX_TOKENS, STAGES>(maps, a);
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGroupedThreads, 1)
+grouped_matmul_pair_kernel(const __grid_constant__ GroupedMaps<MAX_TOKENS / 2> maps, const GroupedArgs a) {
+  grouped_matmul_body<2, MAX_TOKENS, STAGES, false>(maps, a);
 }
 template <int MAX_TOKENS, int STAGES>
-__global__ void __launch_bounds__(kThreads, 1)
-grouped_matmul_kernel(const __grid_constant__ GroupedMaps maps, const GroupedArgs a) {
-  grouped_matmul_body<1, MAX_TOKENS, STAGES>(maps, a);
+__global__ void __launch_bounds__(kGroupedThreads, 1)
+grouped_matmul_kernel(const __grid_constant__ GroupedMaps<MAX_TOKENS> maps, const GroupedArgs a) {
+  grouped_matmul_body<1, MAX_TOKENS, STAGES, MAX_TOKENS <= 64>(maps, a);
 }
 
 // Any k, strides and alignment: one thread an output element.
@@ -407,14 +481,13 @@ grouped_matmul_simt_kernel(const int8_t* __restrict__ x, const int8_t* __restric
 template <int CTAS, int MAX_TOKENS, int STAGES>
 int launch_grouped(const b200q_grouped_matmul_args& in, const GroupedArgs& a, cudaStream_t st) {
   using L = GroupedLayout<CTAS, MAX_TOKENS, STAGES>;
-  GroupedMaps maps;
+  GroupedMaps<L::kBRows> maps;
   if (int rc = make_tmap_3d_cached(&maps.w, in.weight, (uint64_t)in.k, (uint64_t)in.n, (uint64_t)in.groups, (uint64_t)in.w_stride_n,
                                    (uint64_t)in.w_stride_g, kBK, kTileA, "grouped_matmul (weight)"))
     return rc;
-  const uint32_t boxes[3] = {(uint32_t)L::kBRows, 64, 16};
-  for (int i = 0; i < 3; ++i)
-    if (int rc = make_tmap_2d_cached(&maps.x[i], CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, in.x, (uint64_t)in.k, (uint64_t)in.m, (uint64_t)in.k, kBK, boxes[i],
-                                     CU_TENSOR_MAP_SWIZZLE_128B, "grouped_matmul (x)"))
+  for (int i = 0; i < L::kBRows / 16; ++i)
+    if (int rc = make_tmap_2d_cached(&maps.x[i], CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, in.x, (uint64_t)in.k, (uint64_t)in.m, (uint64_t)in.k, kBK,
+                                     16 * (i + 1), CU_TENSOR_MAP_SWIZZLE_128B, "grouped_matmul (x)"))
       return rc;
   // No more CTAs than there can be units.
   const int64_t tiles = in.m / MAX_TOKENS + (in.groups < in.m ? in.groups : in.m);
@@ -423,12 +496,12 @@ int launch_grouped(const b200q_grouped_matmul_args& in, const GroupedArgs& a, cu
   if constexpr (CTAS == 2) {
     constexpr auto kern = grouped_matmul_pair_kernel<MAX_TOKENS, STAGES>;
     if (int rc = ensure_dynamic_smem<kern>(L::kDynamic, "grouped_matmul")) return rc;
-    const int64_t fit = resident_clusters<kern>(2, L::kDynamic);
-    kern<<<(unsigned)(2 * (most < fit ? most : fit)), kThreads, L::kDynamic, st>>>(maps, a);
+    const int64_t fit = resident_clusters<kern>(2, L::kDynamic, kGroupedThreads);
+    kern<<<(unsigned)(2 * (most < fit ? most : fit)), kGroupedThreads, L::kDynamic, st>>>(maps, a);
   } else {
     constexpr auto kern = grouped_matmul_kernel<MAX_TOKENS, STAGES>;
     if (int rc = ensure_dynamic_smem<kern>(L::kDynamic, "grouped_matmul")) return rc;
-    kern<<<(unsigned)(most < sm_count() ? most : sm_count()), kThreads, L::kDynamic, st>>>(maps, a);
+    kern<<<(unsigned)(most < sm_count() ? most : sm_count()), kGroupedThreads, L::kDynamic, st>>>(maps, a);
   }
   return check_launch("grouped_matmul (tcgen05)");
 }
@@ -478,10 +551,18 @@ extern "C" int b200q_grouped_matmul(const b200q_grouped_matmul_args* a, void* st
     grouped_matmul_simt_kernel<<<grid, dim3(32, 8), sizeof(GroupTable), st>>>(a->x, a->weight, a->w_stride_g, a->w_stride_k, a->w_stride_n, g);
     return check_launch("grouped_matmul (simt)");
   }
-  // Few rows an expert: the time goes into reading the weights, which many CTAs with deep rings do best.
-  if (a->m <= 64 * a->groups) {
+  // Few rows a group: the time goes into reading the weights, which small tiles with a deep ring do best.  Between: single CTAs,
+  // whose tiles are half a pair's, waste less at the end of a group and of the launch.  Many rows: pairs, which read each
+  // weight and token tile from L2 half as often and draw less power for it.  Measured for weights of 4096 x 4096 (us; small
+  // tiles / single CTAs / pairs): 64 groups of 2 rows 146 / 166 / 178, of 32 rows 193 / 209 / 220, of 64 rows 244 / 232 / 243, of
+  // 256 rows 655 / 368 / 390; 8 groups of 1024 rows 280 / 145 / 153; 8 groups of 2048 rows and 4096 x 22016 - / 1220 / 1180.
+  if (a->m <= 48 * a->groups) {
     g.tiles_n = (int)ceil_div(a->n, kTileA);
     return launch_grouped<1, 64, 8>(*a, g, st);
+  }
+  if (a->m < 1536 * a->groups) {
+    g.tiles_n = (int)ceil_div(a->n, kTileA);
+    return launch_grouped<1, 256, 4>(*a, g, st);
   }
   g.tiles_n = (int)ceil_div(a->n, 2 * kTileA);
   return launch_grouped<2, 256, 6>(*a, g, st);

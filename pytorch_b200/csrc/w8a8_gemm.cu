@@ -1221,7 +1221,7 @@ int launch_umma(const CUtensorMap& tmA, const CUtensorMap& tmB, const Epi& e, co
 
 // Number of clusters of `csize` CTAs of `kern` that can be resident at once (cached per device and size).
 template <auto Kern>
-int resident_clusters(int csize, int dynamic_smem) {
+int resident_clusters(int csize, int dynamic_smem, int threads = kThreads) {
   static std::mutex mu;
   static int cached[64][9] = {};
   int dev = 0;
@@ -1230,7 +1230,7 @@ int resident_clusters(int csize, int dynamic_smem) {
   if (cached[dev][csize] == 0) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(csize * (sm_count() / csize));
-    cfg.blockDim = dim3(kThreads);
+    cfg.blockDim = dim3(threads);
     cfg.dynamicSmemBytes = dynamic_smem;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
