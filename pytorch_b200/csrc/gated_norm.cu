@@ -28,8 +28,9 @@ namespace b200q {
 namespace {
 
 // A thread's place among the threads that share a row, and its columns: eight values i, VEC: eight neighbours
-// (columns (i * threads + tid) * 8 ..), one or two 16-byte accesses; else columns (i * 8 + j) * threads + tid, one by one,
-// for any width and alignment.
+// (columns (i * threads + tid) * 8 ..), one or two 16-byte accesses, every one of them inside the row (the launch sees to that:
+// predicates cost these kernels more than memory does); else columns (i * 8 + j) * threads + tid, one by one, for any width
+// and alignment.
 struct Place {
   int tid, threads;
   template <bool VEC>
@@ -43,13 +44,14 @@ template <typename T>
 struct Pack8 {
   uint4 v[sizeof(T) / 2];
 };
-template <typename T, bool VEC>
+// ONCE: the row is read once and need not stay in L1 (where the parameters are).
+template <typename T, bool VEC, bool ONCE = true>
 __device__ __forceinline__ void load8(const T* __restrict__ row, int i, int width, const Place& at, Pack8<T>& raw) {
   const int c = at.col<VEC>(i, 0);
   if constexpr (VEC) {
 #pragma unroll
     for (int q = 0; q < (int)sizeof(T) / 2; ++q)
-      raw.v[q] = c < width ? ld_stream(reinterpret_cast<const uint4*>(row + c) + q) : make_uint4(0, 0, 0, 0);
+      raw.v[q] = ONCE ? ld_stream(reinterpret_cast<const uint4*>(row + c) + q) : __ldg(reinterpret_cast<const uint4*>(row + c) + q);
   } else if constexpr (sizeof(T) == 4) {
     uint32_t w[8];
 #pragma unroll
@@ -89,7 +91,6 @@ template <typename T, bool VEC>
 __device__ __forceinline__ void store8(T* __restrict__ row, int i, int width, const Place& at, const float2 (&f)[4]) {
   const int c = at.col<VEC>(i, 0);
   if constexpr (VEC) {
-    if (c >= width) return;
     if constexpr (sizeof(T) == 4) {
       __stcs(reinterpret_cast<float4*>(row + c), make_float4(f[0].x, f[0].y, f[1].x, f[1].y));
       __stcs(reinterpret_cast<float4*>(row + c) + 1, make_float4(f[2].x, f[2].y, f[3].x, f[3].y));
@@ -108,7 +109,7 @@ template <typename P, bool VEC>
 __device__ __forceinline__ void param8(const P* __restrict__ p, int i, int width, const Place& at, float2 (&f)[4]) {
   const int c = at.col<VEC>(i, 0);
   if constexpr (VEC) {
-    load_smooth8(p + min(c, width - 8), f);
+    load_smooth8(p + c, f);
   } else {
 #pragma unroll
     for (int j = 0; j < 4; ++j)
@@ -157,8 +158,141 @@ __device__ __forceinline__ void row_sum(float (&v)[N], float (*red)[32], const P
   }
 }
 
+// Maxima of N non-negative values over the threads of a row.
+template <int N>
+__device__ __forceinline__ void row_max(float (&v)[N], float (*red)[32], const Place& at, int barrier) {
+  unsigned m[N];
+#pragma unroll
+  for (int k = 0; k < N; ++k) m[k] = __reduce_max_sync(0xffffffffu, __float_as_uint(v[k]));
+  if (at.threads > 32) {
+    const int warp = at.tid >> 5, lane = at.tid & 31, nwarps = at.threads >> 5;
+#pragma unroll
+    for (int k = 0; k < N; ++k)
+      if (lane == 0) red[k][warp] = __uint_as_float(m[k]);
+    named_barrier_sync(barrier, at.threads);
+#pragma unroll
+    for (int k = 0; k < N; ++k) m[k] = __reduce_max_sync(0xffffffffu, __float_as_uint(lane < nwarps ? red[k][lane] : 0.0f));
+  }
+#pragma unroll
+  for (int k = 0; k < N; ++k) v[k] = __uint_as_float(m[k]);
+}
+
+template <bool VEC>
+__device__ __forceinline__ void store8_int8(int8_t* __restrict__ row, int i, int width, const Place& at, uint2 v) {
+  const int c = at.col<VEC>(i, 0);
+  if constexpr (VEC) {
+    st_stream(reinterpret_cast<uint2*>(row + c), v);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (c + j * at.threads < width) row[c + j * at.threads] = (int8_t)(((j < 4 ? v.x : v.y) >> (8 * (j & 3))) & 0xff);
+  }
+}
+
 __device__ __forceinline__ float rstd_of(float sum, float inv_width, float eps) {
   return __frsqrt_rn(__fadd_rn(__fmul_rn(sum, inv_width), eps));
+}
+
+// ------------------------------------------------------------------------------------------------ rows through shared memory
+// For more than a handful of rows, the CTA's first warp brings its rows into a ring in shared memory with bulk copies, a chunk
+// of `groups` consecutive rows of every operand a stage, so that the loads of several rows are always under way and no
+// registers hold rows.  It refills a chunk's stage while it works on the next chunk (a warp of its own would cost the others a
+// quarter of their registers: 17 warps get 96 each, 16 get 128).  A chunk is one contiguous piece of each operand; a piece that
+// does not start or end on a 16-byte boundary (rows of odd width) is copied from the boundary before to the one behind, except
+// at the operand's end, whose last bytes the warp copies by itself.  Operands start on a 16-byte boundary.
+// The ring leaves part of the SM's 228 KB to L1, which holds the parameters.
+constexpr int kRowPipeSmem = 150 * 1024;
+constexpr int kRowPipeMaxStages = 4;
+
+// Where the filling of the ring stands: next row, stage, and whether every wait was met.
+struct RowPipeFeed {
+  int64_t row;
+  int stage;
+  uint32_t phase;
+  bool ok;
+  __device__ __forceinline__ void next(int64_t to, int stages) {
+    row = to;
+    if (++stage == stages) { stage = 0; phase ^= 1; }
+  }
+};
+
+struct RowPipe {
+  uint8_t* data;             // [stages][arrays][array_bytes]
+  uint64_t* full;
+  uint64_t* empty;
+  volatile int* abort_flag;
+  int stages, arrays, array_bytes;
+  int64_t row_bytes, total_bytes;
+  __device__ __forceinline__ uint8_t* slot(int stage, int array) const { return data + (int64_t)(stage * arrays + array) * array_bytes; }
+};
+
+// Host and device: bytes of one operand's place in a stage.
+inline __host__ __device__ int row_pipe_array_bytes(int groups, int64_t row_bytes) { return (int)((groups * row_bytes + 16 + 15) & ~int64_t(15)); }
+
+__device__ __forceinline__ RowPipe row_pipe_init(uint8_t* smem, int stages, int arrays, int groups, int64_t row_bytes, int64_t rows, int readers) {
+  __shared__ uint64_t bars[2 * kRowPipeMaxStages];
+  __shared__ int abort_word;
+  RowPipe p{smem, bars, bars + kRowPipeMaxStages, &abort_word, stages, arrays, row_pipe_array_bytes(groups, row_bytes), row_bytes, rows * row_bytes};
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < stages; ++i) {
+      mbar_init(&p.full[i], 1);
+      mbar_init(&p.empty[i], readers);
+    }
+    abort_word = 0;
+    fence_mbar_init();
+  }
+  __syncthreads();
+  return p;
+}
+
+// One chunk, rows [row, row + count), by a whole warp: waits for the stage and starts its copies.
+template <int ARRAYS>
+__device__ __forceinline__ bool row_pipe_fill(const RowPipe& p, const void* const (&src)[ARRAYS], int stage, uint32_t phase, int64_t row, int count,
+                                              int lane) {
+  if (!__all_sync(0xffffffffu, mbar_wait(&p.empty[stage], phase ^ 1, p.abort_flag, kDevTimeoutProducer))) return false;
+  const int64_t lo = row * p.row_bytes, hi = lo + count * p.row_bytes, first = lo & ~int64_t(15);
+  int64_t last = (hi + 15) & ~int64_t(15);
+  if (last > p.total_bytes) {                              // the operand's end: its last bytes one by one
+    last = p.total_bytes & ~int64_t(15);
+    for (int q = 0; q < ARRAYS; ++q)
+      if (src[q] != nullptr && last + lane < hi) p.slot(stage, q)[last - first + lane] = static_cast<const uint8_t*>(src[q])[last + lane];
+    __syncwarp();
+  }
+  const uint32_t bytes = (uint32_t)(last - first);
+  int copies = 0;
+#pragma unroll
+  for (int q = 0; q < ARRAYS; ++q) copies += src[q] != nullptr;
+  if (lane == 0) mbar_arrive_expect_tx(&p.full[stage], bytes * copies);
+  __syncwarp();
+#pragma unroll
+  for (int q = 0; q < ARRAYS; ++q)
+    if (lane == q && src[q] != nullptr && bytes != 0) bulk_load(p.slot(stage, q), static_cast<const uint8_t*>(src[q]) + first, bytes, &p.full[stage]);
+  return true;
+}
+
+// Eight values of a row in shared memory.
+template <typename T, bool VEC>
+__device__ __forceinline__ Pack8<T> smem8(const uint8_t* row, int i, int width, const Place& at) {
+  Pack8<T> raw;
+  const int c = at.col<VEC>(i, 0);
+  if constexpr (VEC) {
+#pragma unroll
+    for (int q = 0; q < (int)sizeof(T) / 2; ++q)
+      raw.v[q] = reinterpret_cast<const uint4*>(row + c * (int)sizeof(T))[q];
+  } else {
+    using Word = typename Chunk<sizeof(T)>::type;
+    const Word* p = reinterpret_cast<const Word*>(row);
+    uint32_t w[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) w[j] = c + j * at.threads < width ? (uint32_t)p[c + j * at.threads] : 0u;
+    if constexpr (sizeof(T) == 4) {
+      raw.v[0] = make_uint4(w[0], w[1], w[2], w[3]);
+      raw.v[1] = make_uint4(w[4], w[5], w[6], w[7]);
+    } else {
+      raw.v[0] = make_uint4(w[0] | (w[1] << 16), w[2] | (w[3] << 16), w[4] | (w[5] << 16), w[6] | (w[7] << 16));
+    }
+  }
+  return raw;
 }
 
 struct NormArgs {
@@ -182,8 +316,8 @@ struct NormArgs {
 // One CTA a row at a time.  The next row's x and residual are in flight from the moment this row's have become h.  With
 // ITERS 1 (rows spread over many threads: few rows, where latency counts) the parameters are loaded with the row, not behind
 // the reductions.
-template <typename T, typename P, bool VEC, int ITERS, bool QUANT, int MAX_THREADS>
-__global__ void __launch_bounds__(MAX_THREADS)
+template <typename T, typename P, bool VEC, int ITERS, bool QUANT, int MAX_THREADS, int MIN_CTAS>
+__global__ void __launch_bounds__(MAX_THREADS, MIN_CTAS)
 gated_norm_kernel(const NormArgs a) {
   constexpr bool EARLY = ITERS == 1;
   __shared__ float red[3][1][32];
@@ -281,21 +415,169 @@ gated_norm_kernel(const NormArgs a) {
       int8_t* q = static_cast<int8_t*>(a.y) + row * a.width;
 #pragma unroll
       for (int i = 0; i < ITERS; ++i) {
-        const uint2 o = inv == inv ? quantize8<false>(h[i], scale, inv) : quantize8<true>(h[i], scale, inv);
-        const int c = at.col<VEC>(i, 0);
-        if constexpr (VEC) {
-          if (c < a.width) st_stream(reinterpret_cast<uint2*>(q + c), o);
-        } else {
-#pragma unroll
-          for (int j = 0; j < 8; ++j)
-            if (c + j * at.threads < a.width) q[c + j * at.threads] = (int8_t)(((j < 4 ? o.x : o.y) >> (8 * (j & 3))) & 0xff);
-        }
+        store8_int8<VEC>(q, i, a.width, at, inv == inv ? quantize8<false>(h[i], scale, inv) : quantize8<true>(h[i], scale, inv));
       }
     }
     // The buffers of one row are written again for the next one only behind another buffer's barrier, except when a row
     // has a single reduction.
     if (post == nullptr && !QUANT) __syncthreads();
   }
+}
+
+// The same for rows that do not come as full vectors, through shared memory: `threads_per_row` threads work on two rows at once
+// (the reductions' latencies and the parameters are then shared by two rows), as many such groups as fit into the CTA.
+constexpr int kRowPipeThreads = 512;      // at most
+
+template <typename T, typename P, bool QUANT>
+__global__ void __launch_bounds__(kRowPipeThreads, 1)
+gated_norm_pipe_kernel(const NormArgs a, int threads_per_row, int stages) {
+  constexpr bool VEC = false;
+  constexpr int ITERS = 1, ROWS = 2;
+  extern __shared__ __align__(16) uint8_t pipe_smem[];
+  __shared__ float red[3][kRowPipeThreads / 32][ROWS][32];
+  const int groups = blockDim.x / threads_per_row, chunk_rows = groups * ROWS;
+  const RowPipe pipe = row_pipe_init(pipe_smem, stages, 2, chunk_rows, (int64_t)a.width * sizeof(T), a.rows, blockDim.x / 32);
+  const int64_t r0 = a.rows * blockIdx.x / gridDim.x, r1 = a.rows * (blockIdx.x + 1) / gridDim.x;
+  const void* const src[2] = {a.x, a.residual};
+  RowPipeFeed feed{r0, 0, 0, true};
+  auto fill = [&]() {                                      // by the first warp
+    if (feed.row >= r1 || !feed.ok) return;
+    feed.ok = row_pipe_fill(pipe, src, feed.stage, feed.phase, feed.row, (int)min((int64_t)chunk_rows, r1 - feed.row), threadIdx.x & 31);
+    feed.next(feed.row + chunk_rows, stages);
+  };
+  if (threadIdx.x < 32)
+    for (int i = 0; i < stages; ++i) fill();
+  int stage = 0;
+  uint32_t phase = 0;
+  const int group = threadIdx.x / threads_per_row;
+  const Place at{(int)threadIdx.x - group * threads_per_row, threads_per_row};
+  const P* gamma = static_cast<const P*>(a.gamma);
+  const P* post = static_cast<const P*>(a.post);
+  const float2 alpha = splat(a.alpha);
+  bool ok = true;
+  for (int64_t chunk = r0; chunk < r1; chunk += chunk_rows) {
+    ok = mbar_wait(&pipe.full[stage], phase, pipe.abort_flag, kDevTimeoutEpilogue) && ok;
+    if (threadIdx.x < 32 && chunk > r0) fill();
+    const int64_t row = chunk + group * ROWS;
+    if (row < r1) {                                        // the same for all threads of the row
+      // Past the CTA's last row the row before is worked on again and not stored.
+      const int live = (int)min((int64_t)ROWS, r1 - row);
+      const uint8_t *xs[ROWS], *rs[ROWS];
+      int64_t gate_row[ROWS];
+      const int64_t off = chunk * pipe.row_bytes - ((chunk * pipe.row_bytes) & ~int64_t(15)) + (int64_t)group * ROWS * pipe.row_bytes;
+#pragma unroll
+      for (int k = 0; k < ROWS; ++k) {
+        const int kk = min(k, live - 1);
+        xs[k] = pipe.slot(stage, 0) + off + kk * pipe.row_bytes;
+        rs[k] = pipe.slot(stage, 1) + off + kk * pipe.row_bytes;
+        gate_row[k] = a.gate.rows_per == 1 ? row + kk : (row + kk) / a.gate.rows_per;
+      }
+      float r1s[ROWS];
+#pragma unroll
+      for (int k = 0; k < ROWS; ++k) r1s[k] = 1.0f;
+      if (post != nullptr) {
+        float2 s2[ROWS];
+        float s[ROWS];
+#pragma unroll
+        for (int k = 0; k < ROWS; ++k) {
+          s2[k] = splat(0.0f);
+#pragma unroll
+          for (int i = 0; i < ITERS; ++i) {
+            const Pack8<T> xr = smem8<T, VEC>(xs[k], i, a.width, at);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const float2 v = pair_of<T>(xr, j);
+              s2[k] = __ffma2_rn(v, v, s2[k]);
+            }
+          }
+          s[k] = s2[k].x + s2[k].y;
+        }
+        row_sum<ROWS>(s, red[0][group], at, 1 + group);
+#pragma unroll
+        for (int k = 0; k < ROWS; ++k) {
+          r1s[k] = rstd_of(s[k], a.inv_width, a.eps);
+          if (at.tid == 0 && a.post_rstd != nullptr && ok && k < live) a.post_rstd[row + k] = r1s[k];
+        }
+      }
+      float2 h[ROWS][ITERS][4], s2[ROWS];
+#pragma unroll
+      for (int k = 0; k < ROWS; ++k) s2[k] = splat(0.0f);
+#pragma unroll
+      for (int i = 0; i < ITERS; ++i) {
+        float2 g[4], w[4];
+        if (post != nullptr) param8<P, VEC>(post, i, a.width, at, w);
+#pragma unroll
+        for (int k = 0; k < ROWS; ++k) {
+          if (k == 0 || gate_row[k] != gate_row[0]) gate8<P, VEC>(a.gate, gate_row[k], i, a.width, at, g);
+          const Pack8<T> xr = smem8<T, VEC>(xs[k], i, a.width, at), rr = smem8<T, VEC>(rs[k], i, a.width, at);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            float2 z = pair_of<T>(xr, j);
+            if (post != nullptr) z = __fmul2_rn(__fmul2_rn(z, splat(r1s[k])), w[j]);
+            h[k][i][j] = __ffma2_rn(g[j], z, __fmul2_rn(alpha, pair_of<T>(rr, j)));
+            s2[k] = __ffma2_rn(h[k][i][j], h[k][i][j], s2[k]);
+          }
+          if (ok && k < live) store8<T, VEC>(static_cast<T*>(a.h) + (row + k) * a.width, i, a.width, at, h[k][i]);
+        }
+      }
+      float s[ROWS], r2[ROWS], amax[ROWS];
+#pragma unroll
+      for (int k = 0; k < ROWS; ++k) s[k] = s2[k].x + s2[k].y;
+      row_sum<ROWS>(s, red[1][group], at, 1 + group);
+#pragma unroll
+      for (int k = 0; k < ROWS; ++k) {
+        r2[k] = rstd_of(s[k], a.inv_width, a.eps);
+        amax[k] = 0.0f;
+        if (at.tid == 0 && a.rstd != nullptr && ok && k < live) a.rstd[row + k] = r2[k];
+      }
+#pragma unroll
+      for (int i = 0; i < ITERS; ++i) {
+        float2 w[4], sm[4];
+        param8<P, VEC>(gamma, i, a.width, at, w);
+        if (QUANT && a.smooth != nullptr) {
+          if (a.smooth_f32) param8<float, VEC>(static_cast<const float*>(a.smooth), i, a.width, at, sm);
+          else param8<T, VEC>(static_cast<const T*>(a.smooth), i, a.width, at, sm);
+        }
+#pragma unroll
+        for (int k = 0; k < ROWS; ++k) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            float2 y = __fmul2_rn(__fmul2_rn(h[k][i][j], splat(r2[k])), w[j]);
+            if (QUANT) {
+              if (a.smooth != nullptr) y = __fmul2_rn(y, sm[j]);
+              amax[k] = fmaxf(amax[k], fmaxf(fabsf(y.x), fabsf(y.y)));
+            }
+            h[k][i][j] = y;
+          }
+          if (!QUANT && ok && k < live) store8<T, VEC>(static_cast<T*>(a.y) + (row + k) * a.width, i, a.width, at, h[k][i]);
+        }
+      }
+      if constexpr (QUANT) {
+        row_max<ROWS>(amax, red[2][group], at, 1 + group);
+#pragma unroll
+        for (int k = 0; k < ROWS; ++k) {
+          if (!ok || k >= live) continue;
+          const float scale = scale_of_amax(amax[k]);
+          if (at.tid == 0) a.scale[row + k] = scale;
+          const float inv = quant_inverse(scale);
+#pragma unroll
+          for (int i = 0; i < ITERS; ++i)
+            store8_int8<VEC>(static_cast<int8_t*>(a.y) + (row + k) * a.width, i, a.width, at,
+                             inv == inv ? quantize8<false>(h[k][i], scale, inv) : quantize8<true>(h[k][i], scale, inv));
+        }
+      } else if (post == nullptr) {
+        // a single reduction a row: its buffer is written again only behind this barrier
+        if (at.threads > 32) named_barrier_sync(1 + group, at.threads);
+      }
+    }
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) mbar_arrive(&pipe.empty[stage]);
+    if (++stage == stages) { stage = 0; phase ^= 1; }
+  }
+  // Give copies that are still in flight time to land before shared memory is released.
+  if (!feed.ok || *pipe.abort_flag)
+    for (int i = 0; i < 200; ++i) __nanosleep(1000);
+  __syncthreads();
 }
 
 struct NormGradArgs {
@@ -319,199 +601,315 @@ struct NormGradArgs {
   int width;
 };
 
-constexpr int kNormGradThreads = 512;     // at most: the sums over rows need up to 128 registers a thread
+constexpr int kNormGradThreads = 512;
 
-// A CTA takes the rows [rows * c / CTAs, rows * (c + 1) / CTAs), `threads_per_row` threads a row and as many rows at a time as
-// fit into the CTA.  Its threads keep the same columns throughout, so the sums over its rows stay with them: in registers
-// while a row is one vector a thread (ITERS 1), else in shared memory, in two planes of four columns a vector, so that a
-// warp's 16-byte accesses touch every bank once.  At the end (for a gate: at the end of the gate's rows) the CTA's row groups
-// add theirs in shared memory in a fixed order and one partial row goes out.  SUM_GATE: the gate's gradient is a sum over the
-// rows that share a gate; without it there is no gate, or one value a row, or one gate a row.
-template <typename T, typename P, bool VEC, int ITERS, bool SUM_GATE>
-__global__ void __launch_bounds__(kNormGradThreads, 1)
-gated_norm_grad_kernel(const NormGradArgs a, int threads_per_row) {
-  constexpr bool SHARED = ITERS > 1;
-  extern __shared__ float4 column_sums[];                  // SHARED: gamma's, post gamma's and the gate's sums; else [width] floats
-  __shared__ float red[2][kNormGradThreads / 32][2][32];
-  const int group = threadIdx.x / threads_per_row, groups = blockDim.x / threads_per_row;
-  const Place at{(int)threadIdx.x - group * threads_per_row, threads_per_row};
-  const T* x = static_cast<const T*>(a.x);
-  const T* res = static_cast<const T*>(a.residual);
-  const T* dy = static_cast<const T*>(a.dy);
-  const T* dhp = static_cast<const T*>(a.dh);
+// The arithmetic of one row of the gradient for ITERS vectors of a thread; `load` gives operand q (0 x, 1 residual, 2 dy, 3 dh)
+// of vector i, `sums` keeps the sums over rows (0 gamma, 1 post gamma, 2 a shared gate).  Operands are read again for each of the
+// three passes, between which the two reductions lie.
+template <typename T, typename P, bool VEC, int ITERS, bool SUM_GATE, typename Load, typename Sums>
+__device__ __forceinline__ void norm_grad_row(const NormGradArgs& a, const Place& at, int64_t row, int64_t gate_row, float rs1, float rs2,
+                                              const Load& load, Sums& sums, float (*red0)[32], float (*red1)[32], int barrier, bool ok) {
   const P* gamma = static_cast<const P*>(a.gamma);
   const P* post = static_cast<const P*>(a.post);
-  const float2 alpha = splat(a.alpha);
-  float2 sums[3][4];                                       // gamma, post gamma, gate; of the vector at hand when SHARED
+  const float2 alpha = splat(a.alpha), s1 = splat(rs1), s2 = splat(rs2);
+  float2 dot2 = splat(0.0f);
 #pragma unroll
-  for (int w = 0; w < 3; ++w)
+  for (int i = 0; i < ITERS; ++i) {
+    float2 g[4], w1[4], w2[4];
+    gate8<P, VEC>(a.gate, gate_row, i, a.width, at, g);
+    if (post != nullptr) param8<P, VEC>(post, i, a.width, at, w1);
+    param8<P, VEC>(gamma, i, a.width, at, w2);
+    const Pack8<T> xr = load(0, i), rr = load(1, i), yr = load(2, i);
+    float2(&acc)[4] = sums.open(0, i);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) sums[w][j] = splat(0.0f);
-  auto place = [&](int w, int half, int i) -> float4& { return column_sums[((2 * w + half) * ITERS + i) * threads_per_row + at.tid]; };
-  auto fetch = [&](int w, int i) {
-    if constexpr (SHARED) {
-      const float4 p = place(w, 0, i), q = place(w, 1, i);
-      sums[w][0] = make_float2(p.x, p.y), sums[w][1] = make_float2(p.z, p.w), sums[w][2] = make_float2(q.x, q.y), sums[w][3] = make_float2(q.z, q.w);
+    for (int j = 0; j < 4; ++j) {
+      float2 z = pair_of<T>(xr, j);
+      if (post != nullptr) z = __fmul2_rn(__fmul2_rn(z, s1), w1[j]);
+      const float2 hn = __fmul2_rn(__ffma2_rn(g[j], z, __fmul2_rn(alpha, pair_of<T>(rr, j))), s2);
+      const float2 d = __fmul2_rn(pair_of<T>(yr, j), hn);
+      dot2 = __ffma2_rn(d, w2[j], dot2);
+      acc[j] = __fadd2_rn(acc[j], d);
     }
-  };
-  auto put = [&](int w, int i) {
-    if constexpr (SHARED) {
-      place(w, 0, i) = make_float4(sums[w][0].x, sums[w][0].y, sums[w][1].x, sums[w][1].y);
-      place(w, 1, i) = make_float4(sums[w][2].x, sums[w][2].y, sums[w][3].x, sums[w][3].y);
-    }
-  };
-  auto clear = [&](int w) {
+    sums.close(0, i);
+  }
+  float dot[1] = {dot2.x + dot2.y};
+  row_sum<1>(dot, red0, at, barrier);
+  const float2 nc2 = splat(-dot[0] * a.inv_width);
+  float2 dots_v = splat(0.0f), dots_g = splat(0.0f);       // v . xn, dh . z
+  float2 keep[ITERS][4];                                   // v
 #pragma unroll
-    for (int j = 0; j < 4; ++j) sums[w][j] = splat(0.0f);
+  for (int i = 0; i < ITERS; ++i) {
+    float2 g[4], w1[4], w2[4], out[4], dg[4];
+    gate8<P, VEC>(a.gate, gate_row, i, a.width, at, g);
+    if (post != nullptr) param8<P, VEC>(post, i, a.width, at, w1);
+    param8<P, VEC>(gamma, i, a.width, at, w2);
+    const Pack8<T> xr = load(0, i), rr = load(1, i), yr = load(2, i);
+    Pack8<T> hr;
+    if (a.dh != nullptr) hr = load(3, i);
+    float2(&acc1)[4] = sums.open(1, i);
+    float2(&accg)[4] = sums.open(2, i);
 #pragma unroll
-    for (int i = 0; i < ITERS; ++i) put(w, i);
-  };
-  clear(0), clear(1), clear(2);
-  // Adds the groups' sums and stores them as one row; called by the whole CTA.
-  auto flush = [&](int w, float* to) {
-    if (!SHARED && groups > 1) {
-      float* joined = reinterpret_cast<float*>(column_sums);
-      for (int g = 0; g < groups; ++g) {
-        if (g == group) {
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const int c = at.col<VEC>(0, j);
-            const float v = (j & 1) ? sums[w][j >> 1].y : sums[w][j >> 1].x;
-            if (c < a.width) joined[c] = g == 0 ? v : joined[c] + v;
-          }
-        }
-        __syncthreads();
+    for (int j = 0; j < 4; ++j) {
+      const float2 xn = __fmul2_rn(pair_of<T>(xr, j), s1);
+      const float2 z = post != nullptr ? __fmul2_rn(xn, w1[j]) : xn;   // without post gamma s1 is 1
+      const float2 hn = __fmul2_rn(__ffma2_rn(g[j], z, __fmul2_rn(alpha, pair_of<T>(rr, j))), s2);
+      float2 dh = __fmul2_rn(s2, __ffma2_rn(hn, nc2, __fmul2_rn(pair_of<T>(yr, j), w2[j])));
+      if (a.dh != nullptr) dh = __fadd2_rn(dh, pair_of<T>(hr, j));
+      out[j] = __fmul2_rn(alpha, dh);
+      if (SUM_GATE) {
+        accg[j] = __ffma2_rn(dh, z, accg[j]);
+      } else {
+        dg[j] = __fmul2_rn(dh, z);
+        dots_g = __fadd2_rn(dots_g, dg[j]);
       }
-      for (int c = threadIdx.x; c < a.width; c += blockDim.x) to[c] = joined[c];
-      __syncthreads();
-    } else {
+      float2 dz = __fmul2_rn(dh, g[j]);
+      if (post != nullptr) {
+        const float2 t = __fmul2_rn(dz, xn);
+        acc1[j] = __fadd2_rn(acc1[j], t);
+        dots_v = __ffma2_rn(t, w1[j], dots_v);
+        dz = __fmul2_rn(dz, w1[j]);
+      }
+      keep[i][j] = dz;
+    }
+    if (post != nullptr) sums.close(1, i);
+    if (SUM_GATE) sums.close(2, i);
+    if (ok) {
+      store8<T, VEC>(static_cast<T*>(a.dres) + row * a.width, i, a.width, at, out);
+      // one gate a row: its gradient is dh * z itself
+      if (!SUM_GATE && a.dgate != nullptr && !a.gate.per_row) store8<P, VEC>(static_cast<P*>(a.dgate) + row * a.width, i, a.width, at, dg);
+    }
+  }
+  float dots[2] = {dots_v.x + dots_v.y, dots_g.x + dots_g.y};
+  if constexpr (SUM_GATE) {
+    float only[1] = {dots[0]};
+    row_sum<1>(only, red1, at, barrier);
+    dots[0] = only[0];
+  } else {
+    row_sum<2>(dots, red1, at, barrier);
+  }
+  const float2 nc1 = splat(-dots[0] * a.inv_width);
+  if (!ok) return;
+  if (!SUM_GATE && a.dgate != nullptr && a.gate.per_row && at.tid == 0) static_cast<P*>(a.dgate)[row] = narrow<P>(dots[1]);
+#pragma unroll
+  for (int i = 0; i < ITERS; ++i) {
+    if (post != nullptr) {
+      const Pack8<T> xr = load(0, i);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) keep[i][j] = __fmul2_rn(s1, __ffma2_rn(__fmul2_rn(pair_of<T>(xr, j), s1), nc1, keep[i][j]));
+    }
+    store8<T, VEC>(static_cast<T*>(a.dx) + row * a.width, i, a.width, at, keep[i]);
+  }
+}
+
+// Sums over rows in registers.
+template <int ITERS>
+struct RegisterSums {
+  float2 v[3][ITERS][4];
+  __device__ __forceinline__ float2 (&open(int w, int i))[4] { return v[w][i]; }
+  __device__ __forceinline__ void close(int, int) {}
+  __device__ __forceinline__ void clear(int w) {
+#pragma unroll
+    for (int i = 0; i < ITERS; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[w][i][j] = make_float2(0.0f, 0.0f);
+  }
+};
+// Sums over rows in shared memory, in two planes of four columns a vector, so that a warp's 16-byte accesses touch every bank
+// once.
+template <int ITERS>
+struct SharedSums {
+  float4* base;
+  int threads, tid;
+  float2 v[3][4];
+  __device__ __forceinline__ float4& place(int w, int half, int i) { return base[((2 * w + half) * ITERS + i) * threads + tid]; }
+  __device__ __forceinline__ float4 peek(int w, int half, int i, int further) const { return base[((2 * w + half) * ITERS + i) * threads + tid + further]; }
+  __device__ __forceinline__ float2 (&open(int w, int i))[4] {
+    const float4 p = place(w, 0, i), q = place(w, 1, i);
+    v[w][0] = make_float2(p.x, p.y), v[w][1] = make_float2(p.z, p.w), v[w][2] = make_float2(q.x, q.y), v[w][3] = make_float2(q.z, q.w);
+    return v[w];
+  }
+  __device__ __forceinline__ void close(int w, int i) {
+    place(w, 0, i) = make_float4(v[w][0].x, v[w][0].y, v[w][1].x, v[w][1].y);
+    place(w, 1, i) = make_float4(v[w][2].x, v[w][2].y, v[w][3].x, v[w][3].y);
+  }
+  __device__ __forceinline__ void clear(int w) {
+#pragma unroll
+    for (int i = 0; i < ITERS; ++i) place(w, 0, i) = place(w, 1, i) = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  }
+};
+
+// A CTA takes the rows [rows * c / CTAs, rows * (c + 1) / CTAs), `threads_per_row` threads a row and as many rows at a time as
+// fit into the CTA.  Its threads keep the same columns throughout, so the sums over its rows stay with them; at the end (for a
+// gate: at the end of the gate's rows) the CTA's row groups are joined in a fixed order and one partial row goes out.  SUM_GATE:
+// the gate's gradient is a sum over the rows that share a gate; without it there is no gate, or one value a row, or one gate a
+// row.  This form reads the rows straight from global memory, any width and alignment; the next row is on its way into L2.
+template <typename T, typename P, bool VEC, int ITERS, bool SUM_GATE, int MAX_THREADS, int MIN_CTAS>
+__global__ void __launch_bounds__(MAX_THREADS, MIN_CTAS)
+gated_norm_grad_kernel(const NormGradArgs a, int threads_per_row) {
+  constexpr bool KEEP = ITERS <= 2;
+  extern __shared__ float4 column_sums[];
+  __shared__ float red[2][MAX_THREADS / 32][2][32];
+  const int group = threadIdx.x / threads_per_row, groups = blockDim.x / threads_per_row;
+  const Place at{(int)threadIdx.x - group * threads_per_row, threads_per_row};
+  SharedSums<ITERS> sums{column_sums, (int)blockDim.x, (int)threadIdx.x};
+  sums.clear(0), sums.clear(1), sums.clear(2);
+  auto flush = [&](int w, float* to) {                     // by the whole CTA
+    if (groups > 1) __syncthreads();
+    if (group == 0) {
 #pragma unroll
       for (int i = 0; i < ITERS; ++i) {
-        fetch(w, i);
-        store8<float, VEC>(to, i, a.width, at, sums[w]);
+        float2(&v)[4] = sums.open(w, i);
+        for (int g = 1; g < groups; ++g) {
+          const float4 p = sums.peek(w, 0, i, g * threads_per_row), q = sums.peek(w, 1, i, g * threads_per_row);
+          v[0] = make_float2(v[0].x + p.x, v[0].y + p.y), v[1] = make_float2(v[1].x + p.z, v[1].y + p.w);
+          v[2] = make_float2(v[2].x + q.x, v[2].y + q.y), v[3] = make_float2(v[3].x + q.z, v[3].y + q.w);
+        }
+        store8<float, VEC>(to, i, a.width, at, v);
       }
     }
+    if (groups > 1) __syncthreads();
   };
   const int64_t r0 = a.rows * blockIdx.x / gridDim.x, r1 = a.rows * (blockIdx.x + 1) / gridDim.x;
-  int64_t seg = r0;
-  while (seg < r1) {
+  for (int64_t seg = r0; seg < r1;) {
     const int64_t gate = SUM_GATE ? seg / a.gate.rows_per : 0;
     const int64_t seg_end = SUM_GATE ? min(r1, (gate + 1) * a.gate.rows_per) : r1;
-    Pack8<T> xr[ITERS], rr[ITERS], yr[ITERS], hr[ITERS];
-    float rs2 = 0.0f, rs1 = 1.0f;
-    auto load_x = [&](int64_t row) {
-#pragma unroll
-      for (int i = 0; i < ITERS; ++i) load8<T, VEC>(x + row * a.width, i, a.width, at, xr[i]);
-      rs2 = a.rstd[row];
-      if (post != nullptr) rs1 = a.post_rstd[row];
-    };
-    auto load_rest = [&](int64_t row) {
-#pragma unroll
-      for (int i = 0; i < ITERS; ++i) {
-        load8<T, VEC>(res + row * a.width, i, a.width, at, rr[i]);
-        load8<T, VEC>(dy + row * a.width, i, a.width, at, yr[i]);
-        if (dhp != nullptr) load8<T, VEC>(dhp + row * a.width, i, a.width, at, hr[i]);
-      }
-    };
-    if (seg + group < seg_end) {
-      load_x(seg + group);
-      load_rest(seg + group);
-    }
-#pragma unroll 1
     for (int64_t row = seg + group; row < seg_end; row += groups) {
-      const int64_t gate_row = SUM_GATE ? gate : row;
-      const bool more = row + groups < seg_end;
-      const float2 s1 = splat(rs1), s2 = splat(rs2);
-      // xn, z and hn of one pair of columns
-      auto normed = [&](int i, int j, const float2(&g)[4], const float2(&w1)[4], float2& xn, float2& z) {
-        const float2 v = pair_of<T>(xr[i], j);
-        xn = __fmul2_rn(v, s1);
-        z = post != nullptr ? __fmul2_rn(xn, w1[j]) : v;
-        return __fmul2_rn(__ffma2_rn(g[j], z, __fmul2_rn(alpha, pair_of<T>(rr[i], j))), s2);
+      if (row + groups < r1) {
+        const int64_t next = (row + groups) * a.width;
+        for (int c = at.tid * (128 / (int)sizeof(T)); c < a.width; c += at.threads * (128 / (int)sizeof(T))) {
+          prefetch_l2(static_cast<const T*>(a.x) + next + c);
+          prefetch_l2(static_cast<const T*>(a.residual) + next + c);
+          prefetch_l2(static_cast<const T*>(a.dy) + next + c);
+          if (a.dh != nullptr) prefetch_l2(static_cast<const T*>(a.dh) + next + c);
+        }
+      }
+      // The row's operands stay in registers where there is room, else they are read again for each pass (from L1).
+      Pack8<T> kept[4][KEEP ? ITERS : 1];
+      auto fetch = [&](int q, int i) {
+        Pack8<T> raw;
+        load8<T, VEC, KEEP>(static_cast<const T*>(q == 0 ? a.x : q == 1 ? a.residual : q == 2 ? a.dy : a.dh) + row * a.width, i, a.width, at, raw);
+        return raw;
       };
-      float2 dot2 = splat(0.0f);
+      if constexpr (KEEP) {
 #pragma unroll
-      for (int i = 0; i < ITERS; ++i) {
-        float2 g[4], w1[4], w2[4];
-        gate8<P, VEC>(a.gate, gate_row, i, a.width, at, g);
-        if (post != nullptr) param8<P, VEC>(post, i, a.width, at, w1);
-        param8<P, VEC>(gamma, i, a.width, at, w2);
-        fetch(0, i);
+        for (int q = 0; q < 4; ++q)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          float2 xn, z;
-          const float2 hn = normed(i, j, g, w1, xn, z);
-          const float2 d = __fmul2_rn(pair_of<T>(yr[i], j), hn);
-          dot2 = __ffma2_rn(d, w2[j], dot2);
-          sums[0][j] = __fadd2_rn(sums[0][j], d);
-        }
-        put(0, i);
+          for (int i = 0; i < ITERS; ++i)
+            if (q < 3 || a.dh != nullptr) kept[q][i] = fetch(q, i);
       }
-      float dot[1] = {dot2.x + dot2.y};
-      row_sum<1>(dot, red[0][group], at, 1 + group);
-      const float2 nc2 = splat(-dot[0] * a.inv_width);
-      float2 dots_v = splat(0.0f), dots_g = splat(0.0f);   // v . xn, dh . z
-      float2 keep[ITERS][4];                               // v
-#pragma unroll
-      for (int i = 0; i < ITERS; ++i) {
-        float2 g[4], w1[4], w2[4], out[4], dg[4];
-        gate8<P, VEC>(a.gate, gate_row, i, a.width, at, g);
-        if (post != nullptr) param8<P, VEC>(post, i, a.width, at, w1);
-        param8<P, VEC>(gamma, i, a.width, at, w2);
-        if (post != nullptr) fetch(1, i);
-        if (SUM_GATE) fetch(2, i);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          float2 xn, z;
-          const float2 hn = normed(i, j, g, w1, xn, z);
-          const float2 u = __fmul2_rn(pair_of<T>(yr[i], j), w2[j]);
-          float2 dh = __fmul2_rn(s2, __ffma2_rn(hn, nc2, u));
-          if (dhp != nullptr) dh = __fadd2_rn(dh, pair_of<T>(hr[i], j));
-          out[j] = __fmul2_rn(alpha, dh);
-          if (SUM_GATE) {
-            sums[2][j] = __ffma2_rn(dh, z, sums[2][j]);
-          } else {
-            dg[j] = __fmul2_rn(dh, z);
-            dots_g = __fadd2_rn(dots_g, dg[j]);
-          }
-          float2 dz = __fmul2_rn(dh, g[j]);
-          if (post != nullptr) {
-            const float2 t = __fmul2_rn(dz, xn);
-            sums[1][j] = __fadd2_rn(sums[1][j], t);
-            dots_v = __ffma2_rn(t, w1[j], dots_v);
-            dz = __fmul2_rn(dz, w1[j]);
-          }
-          keep[i][j] = dz;
-        }
-        if (post != nullptr) put(1, i);
-        if (SUM_GATE) put(2, i);
-        store8<T, VEC>(static_cast<T*>(a.dres) + row * a.width, i, a.width, at, out);
-        // one gate a row: its gradient is dh * z itself
-        if (!SUM_GATE && a.dgate != nullptr && !a.gate.per_row) store8<P, VEC>(static_cast<P*>(a.dgate) + row * a.width, i, a.width, at, dg);
-      }
-      if (more) load_rest(row + groups);                   // in flight from here on
-      float dots[2] = {dots_v.x + dots_v.y, dots_g.x + dots_g.y};
-      row_sum<2>(dots, red[1][group], at, 1 + group);
-      const float2 nc1 = splat(-dots[0] * a.inv_width);
-      if (!SUM_GATE && a.dgate != nullptr && a.gate.per_row && at.tid == 0) static_cast<P*>(a.dgate)[row] = narrow<P>(dots[1]);
-#pragma unroll
-      for (int i = 0; i < ITERS; ++i) {
-        if (post != nullptr) {
-#pragma unroll
-          for (int j = 0; j < 4; ++j) keep[i][j] = __fmul2_rn(s1, __ffma2_rn(__fmul2_rn(pair_of<T>(xr[i], j), s1), nc1, keep[i][j]));
-        }
-        store8<T, VEC>(static_cast<T*>(a.dx) + row * a.width, i, a.width, at, keep[i]);
-      }
-      if (more) load_x(row + groups);
+      auto load = [&](int q, int i) {
+        if constexpr (KEEP) return kept[q][i];
+        else return fetch(q, i);
+      };
+      norm_grad_row<T, P, VEC, ITERS, SUM_GATE>(a, at, row, SUM_GATE ? gate : row, a.post != nullptr ? a.post_rstd[row] : 1.0f, a.rstd[row], load,
+                                                sums, red[0][group], red[1][group], 1 + group, true);
     }
-    if constexpr (SUM_GATE) {
+    if (SUM_GATE) {
       flush(2, a.part_gate + (blockIdx.x + gate) * a.width);
-      clear(2);
+      sums.clear(2);
     }
     seg = seg_end;
   }
   flush(0, a.part_gamma + (int64_t)blockIdx.x * a.width);
-  if (post != nullptr) flush(1, a.part_post + (int64_t)blockIdx.x * a.width);
+  if (a.post != nullptr) flush(1, a.part_post + (int64_t)blockIdx.x * a.width);
+}
+
+// The same for rows that do not come as full vectors, through shared memory; sums in registers, joined by the CTA's row groups in
+// shared memory in a fixed order.
+template <typename T, typename P, bool SUM_GATE>
+__global__ void __launch_bounds__(kRowPipeThreads, 1)
+gated_norm_grad_pipe_kernel(const NormGradArgs a, int threads_per_row, int stages) {
+  extern __shared__ __align__(16) uint8_t pipe_smem[];
+  constexpr bool VEC = false;
+  constexpr int ITERS = 1;
+  __shared__ float red[2][kRowPipeThreads / 32][2][32];
+  const int readers = blockDim.x, groups = readers / threads_per_row;
+  const RowPipe pipe = row_pipe_init(pipe_smem, stages, 4, groups, (int64_t)a.width * sizeof(T), a.rows, readers / 32);
+  float* joined = reinterpret_cast<float*>(pipe.slot(stages, 0));   // [width] behind the ring
+  const int64_t r0 = a.rows * blockIdx.x / gridDim.x, r1 = a.rows * (blockIdx.x + 1) / gridDim.x;
+  // Chunks do not cross the end of a gate's rows.
+  auto chunk_end = [&](int64_t row) {
+    int64_t end = min(row + groups, r1);
+    if (SUM_GATE) end = min(end, (row / a.gate.rows_per + 1) * a.gate.rows_per);
+    return end;
+  };
+  const void* const src[4] = {a.x, a.residual, a.dy, a.dh};
+  RowPipeFeed feed{r0, 0, 0, true};
+  auto fill = [&]() {                                      // by the first warp
+    if (feed.row >= r1 || !feed.ok) return;
+    const int64_t end = chunk_end(feed.row);
+    feed.ok = row_pipe_fill(pipe, src, feed.stage, feed.phase, feed.row, (int)(end - feed.row), threadIdx.x & 31);
+    feed.next(end, stages);
+  };
+  if (threadIdx.x < 32)
+    for (int i = 0; i < stages; ++i) fill();
+  int stage = 0;
+  uint32_t phase = 0;
+  {
+    const int group = threadIdx.x / threads_per_row;
+    const Place at{(int)threadIdx.x - group * threads_per_row, threads_per_row};
+    RegisterSums<ITERS> sums;
+    sums.clear(0), sums.clear(1), sums.clear(2);
+    auto flush = [&](int w, float* to) {                   // by the whole CTA
+      if (groups > 1) {
+        for (int g = 0; g < groups; ++g) {
+          if (g == group) {
+#pragma unroll
+            for (int i = 0; i < ITERS; ++i)
+#pragma unroll
+              for (int j = 0; j < 8; ++j) {
+                const int c = at.col<VEC>(i, j);
+                const float v = (j & 1) ? sums.v[w][i][j >> 1].y : sums.v[w][i][j >> 1].x;
+                if (c < a.width) joined[c] = g == 0 ? v : joined[c] + v;
+              }
+          }
+          __syncthreads();
+        }
+        for (int c = threadIdx.x; c < a.width; c += readers) to[c] = joined[c];
+        __syncthreads();
+      } else {
+#pragma unroll
+        for (int i = 0; i < ITERS; ++i) store8<float, VEC>(to, i, a.width, at, sums.v[w][i]);
+      }
+    };
+    // The statistics of this group's next row are loaded a chunk ahead.
+    float next1 = 1.0f, next2 = 0.0f;
+    auto look = [&](int64_t chunk) {
+      if (chunk < r1 && chunk + group < chunk_end(chunk)) {
+        next2 = a.rstd[chunk + group];
+        if (a.post != nullptr) next1 = a.post_rstd[chunk + group];
+      }
+    };
+    look(r0);
+    bool ok = true;
+    for (int64_t chunk = r0; chunk < r1;) {
+      const int64_t end = chunk_end(chunk), row = chunk + group;
+      const float rs1 = next1, rs2 = next2;
+      look(end);
+      ok = mbar_wait(&pipe.full[stage], phase, pipe.abort_flag, kDevTimeoutEpilogue) && ok;
+      if (threadIdx.x < 32 && chunk > r0) fill();
+      const int64_t gate = SUM_GATE ? chunk / a.gate.rows_per : row;
+      if (row < end) {                                     // the same for all threads of the row
+        const int64_t off = chunk * pipe.row_bytes - ((chunk * pipe.row_bytes) & ~int64_t(15)) + group * pipe.row_bytes;
+        auto load = [&](int q, int i) { return smem8<T, VEC>(pipe.slot(stage, q) + off, i, a.width, at); };
+        norm_grad_row<T, P, VEC, ITERS, SUM_GATE>(a, at, row, gate, rs1, rs2, load, sums, red[0][group], red[1][group], 1 + group, ok);
+      }
+      __syncwarp();
+      if ((threadIdx.x & 31) == 0) mbar_arrive(&pipe.empty[stage]);
+      if (++stage == stages) { stage = 0; phase ^= 1; }
+      if (SUM_GATE && (end == r1 || end / a.gate.rows_per != gate)) {
+        flush(2, a.part_gate + (blockIdx.x + gate) * a.width);
+        sums.clear(2);
+      }
+      chunk = end;
+    }
+    flush(0, a.part_gamma + (int64_t)blockIdx.x * a.width);
+    if (a.post != nullptr) flush(1, a.part_post + (int64_t)blockIdx.x * a.width);
+  }
+  // Give copies that are still in flight time to land before shared memory is released.
+  if (!feed.ok || *pipe.abort_flag)
+    for (int i = 0; i < 200; ++i) __nanosleep(1000);
+  __syncthreads();
 }
 
 // Adds the CTAs' partial sums: blockIdx.y 0 = gamma, 1 = post gamma, 2 + g = gate g.  A block owns 32 columns; its 32
@@ -565,64 +963,140 @@ gated_norm_sum_kernel(const NormSumArgs a) {
 
 constexpr int kNormMaxWidth = 16384;
 
-// Vectors of eight need a width that they divide and 16-byte aligned rows and parameters.
+// Vectors a thread takes of a row in the kernels that read rows straight into registers.
+inline int norm_iters(int64_t width, bool many) {
+  if (width > 8192) return 4;
+  if (!many || width % 512 != 0) return 1;
+  return width <= 4096 ? 2 : width % 1024 == 0 ? 4 : 1;
+}
+
+// Full vectors: a width that whole warps of vectors make up, however many vectors a thread takes, and 16-byte aligned rows and
+// parameters.
 inline bool norm_vec(int64_t width, std::initializer_list<const void*> ptrs) {
-  if (width % 8 != 0) return false;
+  const int64_t step = width > 8192 ? 1024 : width > 4096 ? 512 : 256;
+  if (width % step != 0) return false;
   for (const void* p : ptrs)
     if (!aligned(p, 16)) return false;
   return true;
 }
 
-// Few rows (no more than SMs): as many threads a row as it has vectors, for the shortest way through a row.  Otherwise
-// 256 threads or fewer with up to four vectors each, so that several rows are in flight on an SM.
+// Shape of a launch with rows through shared memory: threads a row (one vector each), groups of `rows` rows at a time, stages.
+struct RowPipePlan {
+  int threads, groups, stages, smem;
+  bool fits;
+};
+inline RowPipePlan row_pipe_plan(int64_t width, int element, int arrays, int rows, int64_t rows_per_cta, int extra) {
+  RowPipePlan p{};
+  p.threads = (int)ceil_div(ceil_div(width, 8), 32) * 32;
+  if (p.threads > kRowPipeThreads) return p;
+  p.groups = kRowPipeThreads / p.threads;
+  if (p.groups > 14) p.groups = 14;                         // named barriers 1 .. 14
+  if (p.groups * rows > rows_per_cta) p.groups = (int)ceil_div(rows_per_cta, rows);
+  const int stage = arrays * row_pipe_array_bytes(p.groups * rows, width * element);
+  p.stages = (kRowPipeSmem - extra) / stage;
+  if (p.stages > kRowPipeMaxStages) p.stages = kRowPipeMaxStages;
+  p.smem = p.stages * stage + extra;
+  p.fits = p.stages >= 2;
+  return p;
+}
+
+// Full vectors: a handful of rows (no more than two an SM) get as many threads a row as it has vectors, for the shortest way
+// through a row; more rows 256 threads (512 above 8192 columns) with two or four vectors each, four CTAs an SM.  Rows that are not
+// made of full vectors go through shared memory, up to 4096 columns and from a 16-byte boundary on.
 template <typename T, typename P, bool VEC, bool QUANT>
 int launch_norm(const NormArgs& a, cudaStream_t st) {
-  const int64_t vecs = ceil_div(a.width, 8);
-  int iters = vecs > 1024 ? 4 : 1;
-  if (a.rows > sm_count())
-    while (iters < 4 && vecs > iters * 256) iters *= 2;
-  const int threads = (int)ceil_div(ceil_div(vecs, iters), 32) * 32;
-#define B200Q_NORM(I, MAX)                                                                       \
+  const bool many = a.rows > 2 * sm_count();
+  if constexpr (!VEC) {
+    const int64_t ctas = a.rows < sm_count() ? a.rows : sm_count();
+    const RowPipePlan p = row_pipe_plan(a.width, sizeof(T), 2, 2, ceil_div(a.rows, ctas), 0);
+    if (many && p.fits && aligned(a.x, 16) && aligned(a.residual, 16)) {
+      constexpr auto kern = gated_norm_pipe_kernel<T, P, QUANT>;
+      if (int rc = ensure_dynamic_smem<kern>(kRowPipeSmem, "gated_add_rms_norm")) return rc;
+      kern<<<(unsigned)ctas, p.groups * p.threads, p.smem, st>>>(a, p.threads, p.stages);
+      return check_launch("gated_add_rms_norm");
+    }
+  }
+  const int iters = norm_iters(a.width, many && VEC);
+  const int threads = (int)ceil_div(ceil_div(a.width, 8 * iters), 32) * 32;
+#define B200Q_NORM(I, MAX, MIN)                                                                  \
   {                                                                                              \
-    constexpr auto kern = gated_norm_kernel<T, P, VEC, I, QUANT, MAX>;                           \
+    constexpr auto kern = gated_norm_kernel<T, P, VEC, I, QUANT, MAX, MIN>;                      \
     const int64_t cap = (int64_t)sm_count() * resident_ctas<kern>(threads);                      \
     kern<<<(unsigned)(a.rows < cap ? a.rows : cap), threads, 0, st>>>(a);                        \
   }
-  if (iters == 1) B200Q_NORM(1, 1024) else if (iters == 2) B200Q_NORM(2, 256) else B200Q_NORM(4, 512)
+  if (iters == 1) {
+    B200Q_NORM(1, 1024, 1)
+  } else if (iters == 2) {
+    if constexpr (VEC) B200Q_NORM(2, 256, 4)
+  } else {
+    B200Q_NORM(4, 512, 1)
+  }
 #undef B200Q_NORM
   return check_launch("gated_add_rms_norm");
 }
 
-// CTAs of the gradient kernel: one an SM, each of which writes one row of partial sums per parameter.
-inline int grad_ctas(int64_t rows) {
-  const int64_t cap = sm_count();
+// CTAs of the gradient kernels, each of which writes one row of partial sums per parameter: at most kNormGradCtas an SM.
+constexpr int kNormGradCtas = 2;
+inline int grad_ctas(int64_t rows, int per_sm) {
+  const int64_t cap = (int64_t)per_sm * sm_count();
   return (int)(rows < cap ? rows : cap);
 }
 
+// Full vectors: CTAs of 256 threads, two an SM, with two vectors a thread and row up to 4096 columns (measured for 8192 rows of 4096
+// bf16: 124 us with the row's operands in registers, 130 read again from L1, 151 from L2; three CTAs an SM at 80 registers
+// 147, rows through shared memory with the sums in registers 176 to 203); 512 threads with two (up to 8192) or four vectors above.  Else through shared memory, up to 4096 columns and from a
+// 16-byte boundary on.
 template <typename T, typename P, bool VEC>
-int launch_norm_grad(const NormGradArgs& a, const NormSumArgs& s, bool sum_gate, cudaStream_t st) {
-  // One vector a thread up to 4096 columns; the CTA's other threads take more rows at the same time.
-  const int64_t vecs = ceil_div(a.width, 8);
-  const int iters = vecs > 2 * kNormGradThreads ? 4 : vecs > kNormGradThreads ? 2 : 1;
-  const int threads = (int)ceil_div(ceil_div(vecs, iters), 32) * 32;
-  const int64_t most_rows = ceil_div(a.rows, s.ctas);
-  int groups = kNormGradThreads / threads;
-  if (groups > 15 && threads > 32) groups = 15;             // named barriers 1 .. 15
-  if (groups > most_rows) groups = (int)most_rows;
-  // Sums of every column (three, two planes of 16 bytes a vector: at most 192 KB), or one row for joining the groups.
-  const int smem = iters > 1 ? 3 * 2 * 16 * iters * threads : groups > 1 ? (int)a.width * 4 : 0;
-#define B200Q_NORM_GRAD_CASE(I)                                                                                                  \
-  {                                                                                                                              \
-    if (I > 1) {                                                                                                                 \
-      constexpr int most = 3 * 2 * 16 * I * kNormGradThreads;                                                                    \
-      if (int rc = ensure_dynamic_smem<gated_norm_grad_kernel<T, P, VEC, I, true>>(most, "gated_add_rms_norm_grad")) return rc;  \
-      if (int rc = ensure_dynamic_smem<gated_norm_grad_kernel<T, P, VEC, I, false>>(most, "gated_add_rms_norm_grad")) return rc; \
-    }                                                                                                                            \
-    if (sum_gate) gated_norm_grad_kernel<T, P, VEC, I, true><<<s.ctas, groups * threads, smem, st>>>(a, threads);                \
-    else gated_norm_grad_kernel<T, P, VEC, I, false><<<s.ctas, groups * threads, smem, st>>>(a, threads);                        \
+int launch_norm_grad(const NormGradArgs& a, NormSumArgs s, bool sum_gate, cudaStream_t st) {
+#define B200Q_NORM_GRAD(I, MAX, MIN, SUM)                                                                                \
+  {                                                                                                                      \
+    constexpr auto kern = gated_norm_grad_kernel<T, P, VEC, I, SUM, MAX, MIN>;                                           \
+    if (int rc = ensure_dynamic_smem<kern>(3 * 2 * 16 * I * MAX, "gated_add_rms_norm_grad")) return rc;                  \
+    int groups = MAX / threads;                                                                                          \
+    if (groups > 15) groups = 15;                          /* named barriers */                                          \
+    if (groups > ceil_div(a.rows, s.ctas)) groups = (int)ceil_div(a.rows, s.ctas);                                       \
+    /* three sums of every column: at most 192 KB */                                                                     \
+    kern<<<s.ctas, groups * threads, 3 * 2 * 16 * I * groups * threads, st>>>(a, threads);                               \
   }
-  if (iters == 1) B200Q_NORM_GRAD_CASE(1) else if (iters == 2) B200Q_NORM_GRAD_CASE(2) else B200Q_NORM_GRAD_CASE(4)
-#undef B200Q_NORM_GRAD_CASE
+#define B200Q_NORM_GRAD_BOTH(I, MAX, MIN)                                                                                \
+  if (sum_gate) B200Q_NORM_GRAD(I, MAX, MIN, true) else B200Q_NORM_GRAD(I, MAX, MIN, false)
+  if constexpr (VEC) {
+    // Whole warps of vectors: a multiple of 512 columns takes two vectors a thread, of 256 one, above 8192 columns four.
+    const int iters = a.width > 8192 ? 4 : a.width % 512 == 0 ? 2 : 1;
+    const int threads = (int)(a.width / (8 * iters));
+    s.ctas = grad_ctas(a.rows, threads <= 256 && iters < 4 ? 2 : 1);
+    if (iters == 4) {
+      B200Q_NORM_GRAD_BOTH(4, 512, 1)
+    } else if (threads > 256) {
+      if (iters == 2) {
+        B200Q_NORM_GRAD_BOTH(2, 512, 1)
+      } else {
+        B200Q_NORM_GRAD_BOTH(1, 512, 1)
+      }
+    } else if (iters == 2) {
+      B200Q_NORM_GRAD_BOTH(2, 256, 2)
+    } else {
+      B200Q_NORM_GRAD_BOTH(1, 256, 2)
+    }
+  } else {
+    s.ctas = grad_ctas(a.rows, 1);
+    const RowPipePlan p = row_pipe_plan(a.width, sizeof(T), 4, 1, ceil_div(a.rows, s.ctas), (int)((a.width * 4 + 15) & ~15));
+    if (p.fits && aligned(a.x, 16) && aligned(a.residual, 16) && aligned(a.dy, 16) && aligned(a.dh, 16)) {
+#define B200Q_NORM_GRAD_PIPE(SUM)                                                                                        \
+  {                                                                                                                      \
+    constexpr auto kern = gated_norm_grad_pipe_kernel<T, P, SUM>;                                                        \
+    if (int rc = ensure_dynamic_smem<kern>(kRowPipeSmem, "gated_add_rms_norm_grad")) return rc;                          \
+    kern<<<s.ctas, p.groups * p.threads, p.smem, st>>>(a, p.threads, p.stages);                                          \
+  }
+      if (sum_gate) B200Q_NORM_GRAD_PIPE(true) else B200Q_NORM_GRAD_PIPE(false)
+#undef B200Q_NORM_GRAD_PIPE
+    } else {
+      const int threads = (int)ceil_div(ceil_div(a.width, 32), 32) * 32;
+      B200Q_NORM_GRAD_BOTH(4, 512, 1)
+    }
+  }
+#undef B200Q_NORM_GRAD_BOTH
+#undef B200Q_NORM_GRAD
   if (int rc = check_launch("gated_add_rms_norm_grad")) return rc;
   const int64_t gates = sum_gate ? ceil_div(a.rows, s.rows_per) : 0;
   dim3 grid((unsigned)ceil_div(a.width, 32), (unsigned)(2 + gates));
@@ -709,7 +1183,7 @@ extern "C" int b200q_gated_norm(const b200q_gated_norm_args* a, void* stream) {
 extern "C" size_t b200q_gated_norm_grad_workspace_bytes(const b200q_gated_norm_args* a) {
   using namespace b200q;
   if (a == nullptr || a->rows <= 0 || a->width <= 0) return 0;
-  const int64_t ctas = grad_ctas(a->rows);
+  const int64_t ctas = grad_ctas(a->rows, kNormGradCtas);
   const int64_t gates = gate_is_shared(*a) ? ctas + ceil_div(a->rows, a->gate_rows) : 0;
   return (size_t)(2 * ctas + gates) * (size_t)a->width * 4;
 }
@@ -742,7 +1216,7 @@ extern "C" int b200q_gated_norm_grad(const b200q_gated_norm_args* a, const b200q
   const size_t need = b200q_gated_norm_grad_workspace_bytes(a);
   B200Q_REQUIRE(g->workspace != nullptr && g->workspace_bytes >= need && aligned(g->workspace, 256), B200Q_ERR_WORKSPACE,
                 "%s: needs %zu bytes of 256-byte aligned workspace, got %zu", op, need, g->workspace_bytes);
-  const int ctas = grad_ctas(a->rows);
+  const int ctas = grad_ctas(a->rows, kNormGradCtas);   // at most: the launch may use fewer
   // Partial rows lie `width` apart, so vectors of them are aligned exactly when the width allows vectors at all.
   float* part = static_cast<float*>(g->workspace);
   NormGradArgs n{};
@@ -756,7 +1230,7 @@ extern "C" int b200q_gated_norm_grad(const b200q_gated_norm_args* a, const b200q
   NormSumArgs s{};
   s.part_gamma = n.part_gamma; s.part_post = a->post_gamma != nullptr ? n.part_post : nullptr; s.part_gate = n.part_gate;
   s.dgamma = g->dgamma; s.dpost = g->dpost_gamma; s.dgate = g->dgate; s.dtype = a->param_dtype;
-  s.rows = a->rows; s.rows_per = shared ? a->gate_rows : 1; s.width = a->width; s.ctas = ctas;
+  s.rows = a->rows; s.rows_per = shared ? a->gate_rows : 1; s.width = a->width;
   const bool vec = norm_vec(a->width, {a->x, a->residual, g->dy, g->dh, g->dx, g->dresidual, a->gamma, a->post_gamma,
                                        a->gate_per_row ? nullptr : a->gate, a->gate_per_row || shared ? nullptr : g->dgate});
 #define B200Q_CALL(T, P) (vec ? launch_norm_grad<T, P, true>(n, s, shared, st) : launch_norm_grad<T, P, false>(n, s, shared, st))

@@ -449,12 +449,14 @@ moe_quant_direct_kernel(const RouteIds r, const T* __restrict__ x, int64_t width
 template <typename IdT, typename T, typename ST, int ITERS>
 __global__ void __launch_bounds__(512)
 moe_quant_kernel(const RouteIds r, const T* __restrict__ x, int64_t width, const ST* __restrict__ smooth, int smooth_rows,
-                 int8_t* __restrict__ out, float* __restrict__ out_scale, const int32_t* __restrict__ row_src) {
+                 int8_t* __restrict__ out, float* __restrict__ out_scale, const int32_t* __restrict__ row_src,
+                 const int32_t* __restrict__ valid_rows) {
   const IdT* ids = static_cast<const IdT*>(r.ids);
   __shared__ float red[2][32];
   wait_for_primary();
   const int nvec = (int)(width >> 3);
-  const int64_t r0 = r.n * blockIdx.x / gridDim.x, r1 = r.n * (blockIdx.x + 1) / gridDim.x;
+  const int64_t valid = *valid_rows;
+  const int64_t r0 = valid * blockIdx.x / gridDim.x, r1 = valid * (blockIdx.x + 1) / gridDim.x;
   uint4 raw[ITERS ? ITERS : 1], nxt[ITERS ? ITERS : 1];
   float2 sm_row[ITERS ? ITERS : 1][4];
   int sm_expert = -1;
@@ -473,6 +475,16 @@ moe_quant_kernel(const RouteIds r, const T* __restrict__ x, int64_t width, const
   int expert = src >= 0 ? expert_of(ids, src, r.begin, r.experts) : 0;
   if (src >= 0) load(src, nxt);
   int after = r0 + 1 < r1 ? row_src[r0 + 1] : -1;
+  // This CTA's share of the rows that no assignment owns.
+  const int64_t idle = r.n - valid;
+  for (int64_t row = valid + idle * blockIdx.x / gridDim.x; row < valid + idle * (blockIdx.x + 1) / gridDim.x; ++row) {
+    if constexpr (ITERS > 0) {
+      for (int v = threadIdx.x; v < nvec; v += blockDim.x) st_stream(reinterpret_cast<uint2*>(out + row * width) + v, make_uint2(0, 0));
+      if (threadIdx.x == 0) out_scale[row] = 0.0f;
+    } else {
+      zero_quant_row(out + row * width, out_scale + row, width);
+    }
+  }
   int par = 0;
   for (int64_t row = r0; row < r1; ++row) {
     if constexpr (ITERS > 0) {
@@ -484,10 +496,6 @@ moe_quant_kernel(const RouteIds r, const T* __restrict__ x, int64_t width, const
     src = after;
     if (src >= 0) expert = expert_of(ids, src, r.begin, r.experts);
     after = row + 2 < r1 ? row_src[row + 2] : -1;
-    if (here < 0) {
-      zero_quant_row(out + row * width, out_scale + row, width);
-      continue;
-    }
     par ^= 1;                                              // a buffer is written again only behind the other one's barrier
     const ST* sm = smooth == nullptr ? nullptr : smooth + (smooth_rows > 1 ? (int64_t)e * width : 0);
     if constexpr (ITERS > 0) {
@@ -912,7 +920,7 @@ int launch_route_quant_iters(const b200q_moe_route_args& a, const RouteIds& r, i
   if (int rc = launch_sort<IdT>(r, a.row_idx, row_src, a.expert_tokens, a.cumulative, valid_rows, st)) return rc;
   const int64_t cap = (int64_t)sm_count() * resident_ctas<moe_quant_kernel<IdT, T, ST, ITERS>>(threads);
   return launch_dependent(moe_quant_kernel<IdT, T, ST, ITERS>, (unsigned)(r.n < cap ? r.n : cap), threads, st, "moe_route (quantised)", r, x, a.hidden, sm,
-                          (int)a.scale_rows, out, a.out_scale, static_cast<const int32_t*>(row_src));
+                          (int)a.scale_rows, out, a.out_scale, static_cast<const int32_t*>(row_src), static_cast<const int32_t*>(valid_rows));
 }
 
 template <typename IdT, typename T, typename ST>

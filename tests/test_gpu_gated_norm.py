@@ -216,3 +216,46 @@ def test_captured_step_replays(npu):
         graph.replay()
         want = step()
         assert all(torch.equal(a, b) for a, b in zip(out, want))
+
+
+# Many rows, where the rows of a CTA overlap: full vectors of one, two and four a thread with one or several rows at a time, rows
+# that are not full vectors through shared memory (with odd starts, a last row that ends off the 16-byte grid, groups of
+# rows), gates that change within a CTA's rows, and storage off the vector grid.
+MANY = [((700, 256), "channel", True), ((1200, 512), "row", True), ((600, 768), "full", True), ((40, 31, 1024), "sample", True), ((333, 4096), "channel", True),
+        ((301, 5632), "channel", True), ((310, 8192), "sample2", True), ((299, 9216), "channel", True), ((150, 16384), "channel", True), ((905, 1111), "channel", True),
+        ((7, 131, 333), "sample", True), ((2500, 8), "sample2", True), ((777, 17), None, False), ((301, 4095), "full", False), ((300, 4097), "row", True)]
+
+
+@pytest.mark.parametrize("dtype,ptype", [(torch.bfloat16, torch.bfloat16), (torch.float16, torch.float32), (torch.float32, torch.float32)])
+@pytest.mark.parametrize("case", range(len(MANY)))
+def test_many_rows(npu, case, dtype, ptype):
+    shape, gate, post = MANY[case]
+    g = torch.Generator().manual_seed(case)
+    if gate == "sample2":                                          # a gate for every five rows
+        shape, gate = (shape[0] // 5, 5, shape[1]), "sample"
+    x, res, gamma, pg, gt = inputs(shape, dtype, ptype, gate, post, g)
+    dy, dh = torch.randn(shape, generator=g).to(dtype), (torch.randn(shape, generator=g) * 0.3).to(dtype)
+    width = shape[-1]
+    y64, h64, _, _ = oracle.gated_add_rms_norm(x, res, gamma, pg, gt, 0.5, EPS)
+    want, terms = oracle.gated_add_rms_norm_grad(x, res, gamma, pg, gt, 0.5, EPS, dy, dh)
+    for offset in (0, 1):
+        def place(t):                                              # the same values, one element off the allocation's start
+            if t is None or not offset:
+                return t if t is None else t.cuda()
+            wide = torch.empty(t.numel() + 1, dtype=t.dtype, device="cuda")
+            wide[1:] = t.reshape(-1).cuda()
+            return wide[1:].reshape(t.shape)
+        leaves = [place(t).requires_grad_() if t is not None else None for t in (x, res, gamma, pg, gt)]
+        y, _, h, _ = npu.npu_gated_add_rms_norm(leaves[0], leaves[1], leaves[2], post_gamma=leaves[3], gate=leaves[4], residual_scale=0.5, epsilon=EPS)
+        within(y.detach(), y64, width, "y")
+        within(h.detach(), h64, width, "h")
+        q, s, hq = npu.npu_gated_add_rms_norm_dynamic_quant(*(t.detach() for t in leaves[:3]), post_gamma=None if pg is None else leaves[3].detach(),
+                                                            gate=None if gt is None else leaves[4].detach(), residual_scale=0.5, epsilon=EPS)
+        s64 = y64.abs().amax(-1) / 127
+        assert torch.equal(hq, h) and bool(((s.cpu().double() - s64).abs() <= s64 * (width + 40) * 2.0 ** -24).all())
+        assert float((q.cpu().double() - y64 / s64[..., None]).abs().max()) <= 0.5 + 127 * (width + 40) * 2.0 ** -23
+        names = [n for n, t in zip(("x", "residual", "gamma", "post_gamma", "gate"), leaves) if t is not None]
+        have = [t for t in leaves if t is not None]
+        for n, t in zip(names, torch.autograd.grad((y, h), have, (place(dy), place(dh)))):
+            rows = x.numel() // width
+            within(t, want[n], width, n, rows=rows if n in ("gamma", "post_gamma", "gate") else 1, terms=terms[n])
