@@ -344,18 +344,27 @@ moe_copy_kernel(const VT* __restrict__ x, VT* __restrict__ out, int64_t tokens, 
 // ------------------------------------------------------------------------------------------------ routing + int8
 // One row: smooth multiply, row maximum, scale, quantised values, all with the helpers (and bits) of
 // npu_dynamic_quant.  The CTA owns the row; each thread holds ITERS vectors of eight values.
-template <typename ST, int ITERS>
+// FULL: every thread's every vector is inside the row (no predicates; this kernel is bound by instruction issue).
+template <typename ST, int ITERS, bool FULL>
 __device__ __forceinline__ void load_smooth_row(const ST* __restrict__ smooth, int nvec, float2 (&sm)[ITERS][4]) {
 #pragma unroll
   for (int i = 0; i < ITERS; ++i) {
     const int v = threadIdx.x + i * blockDim.x;
 #pragma unroll
     for (int j = 0; j < 4; ++j) sm[i][j] = make_float2(1.0f, 1.0f);
-    if (smooth != nullptr && v < nvec) load_smooth8(smooth + (int64_t)v * 8, sm[i]);
+    if (smooth != nullptr && (FULL || v < nvec)) load_smooth8(smooth + (int64_t)v * 8, sm[i]);
+  }
+}
+template <typename T, int ITERS, bool FULL>
+__device__ __forceinline__ void load_row(const T* __restrict__ x, int nvec, uint4 (&to)[ITERS]) {
+#pragma unroll
+  for (int q = 0; q < ITERS; ++q) {
+    const int v = threadIdx.x + q * blockDim.x;
+    to[q] = FULL || v < nvec ? __ldg(reinterpret_cast<const uint4*>(x) + v) : make_uint4(0, 0, 0, 0);
   }
 }
 
-template <typename T, int ITERS>
+template <typename T, int ITERS, bool FULL>
 __device__ __forceinline__ void quant_row_store(const uint4 (&raw)[ITERS], const float2 (&sm)[ITERS][4], int nvec,
                                                 int8_t* __restrict__ y, float* __restrict__ scale_out, float* red) {
   float2 f[ITERS][4];
@@ -367,10 +376,15 @@ __device__ __forceinline__ void quant_row_store(const uint4 (&raw)[ITERS], const
   if (threadIdx.x == 0) *scale_out = scale;
   const float inv = quant_inverse(scale);
   uint2* yr = reinterpret_cast<uint2*>(y) + threadIdx.x;
+  if (inv == inv) {
 #pragma unroll
-  for (int i = 0; i < ITERS; ++i)
-    if (threadIdx.x + i * blockDim.x < nvec)
-      st_stream(yr + i * blockDim.x, inv == inv ? quantize8<false>(f[i], scale, inv) : quantize8<true>(f[i], scale, inv));
+    for (int i = 0; i < ITERS; ++i)
+      if (FULL || threadIdx.x + i * blockDim.x < nvec) st_stream(yr + i * blockDim.x, quantize8<false>(f[i], scale, inv));
+  } else {
+#pragma unroll
+    for (int i = 0; i < ITERS; ++i)
+      if (FULL || threadIdx.x + i * blockDim.x < nvec) st_stream(yr + i * blockDim.x, quantize8<true>(f[i], scale, inv));
+  }
 }
 
 // The same for any width and alignment: two passes over the row.
@@ -422,12 +436,8 @@ moe_quant_direct_kernel(const RouteIds r, const T* __restrict__ x, int64_t width
   const int e = expert_of(ids, i, r.begin, r.experts);
   const ST* sm = smooth == nullptr ? nullptr : smooth + (smooth_rows > 1 ? (int64_t)max(e, 0) * width : 0);
   if constexpr (ITERS > 0) {                               // in flight while the row is being found
-    load_smooth_row<ST, ITERS>(sm, nvec, sm_row);
-#pragma unroll
-    for (int q = 0; q < ITERS; ++q) {
-      const int v = threadIdx.x + q * blockDim.x;
-      raw[q] = v < nvec ? __ldg(reinterpret_cast<const uint4*>(xr) + v) : make_uint4(0, 0, 0, 0);
-    }
+    load_smooth_row<ST, ITERS, false>(sm, nvec, sm_row);
+    load_row<T, ITERS, false>(xr, nvec, raw);
   }
   int rows[1];
   direct_rows(ids, n, r.begin, r.experts, i, red_i, rows);
@@ -440,13 +450,13 @@ moe_quant_direct_kernel(const RouteIds r, const T* __restrict__ x, int64_t width
     zero_quant_row(out + row * width, out_scale + row, width);
     return;
   }
-  if constexpr (ITERS > 0) quant_row_store<T, ITERS>(raw, sm_row, nvec, out + row * width, out_scale + row, red);
+  if constexpr (ITERS > 0) quant_row_store<T, ITERS, false>(raw, sm_row, nvec, out + row * width, out_scale + row, red);
   else quant_row_generic<T, ST>(xr, sm, width, out + row * width, out_scale + row, red);
 }
 
 // Many assignments: persistent CTAs take contiguous pieces of the sorted rows, so a piece mostly stays with one expert,
 // whose smooth scales stay in registers; the next row is in flight during the arithmetic of this one.
-template <typename IdT, typename T, typename ST, int ITERS>
+template <typename IdT, typename T, typename ST, int ITERS, bool FULL>
 __global__ void __launch_bounds__(512)
 moe_quant_kernel(const RouteIds r, const T* __restrict__ x, int64_t width, const ST* __restrict__ smooth, int smooth_rows,
                  int8_t* __restrict__ out, float* __restrict__ out_scale, const int32_t* __restrict__ row_src,
@@ -460,20 +470,13 @@ moe_quant_kernel(const RouteIds r, const T* __restrict__ x, int64_t width, const
   uint4 raw[ITERS ? ITERS : 1], nxt[ITERS ? ITERS : 1];
   float2 sm_row[ITERS ? ITERS : 1][4];
   int sm_expert = -1;
-  auto load = [&](int src, uint4(&to)[ITERS ? ITERS : 1]) {
-    if constexpr (ITERS > 0) {
-      const uint4* xr = reinterpret_cast<const uint4*>(x + (int64_t)(src / r.topk) * width);
-#pragma unroll
-      for (int q = 0; q < ITERS; ++q) {
-        const int v = threadIdx.x + q * blockDim.x;
-        to[q] = v < nvec ? __ldg(xr + v) : make_uint4(0, 0, 0, 0);
-      }
-    }
+  auto load = [&](int src) {
+    if constexpr (ITERS > 0) load_row<T, ITERS, FULL>(x + (int64_t)(src / r.topk) * width, nvec, nxt);
   };
   // Row r's assignment is read two rows ahead, its expert and x one row ahead.
   int src = r0 < r1 ? row_src[r0] : -1;
   int expert = src >= 0 ? expert_of(ids, src, r.begin, r.experts) : 0;
-  if (src >= 0) load(src, nxt);
+  if (src >= 0) load(src);
   int after = r0 + 1 < r1 ? row_src[r0 + 1] : -1;
   // This CTA's share of the rows that no assignment owns.
   const int64_t idle = r.n - valid;
@@ -490,7 +493,7 @@ moe_quant_kernel(const RouteIds r, const T* __restrict__ x, int64_t width, const
     if constexpr (ITERS > 0) {
 #pragma unroll
       for (int q = 0; q < ITERS; ++q) raw[q] = nxt[q];
-      if (after >= 0) load(after, nxt);
+      if (after >= 0) load(after);
     }
     const int here = src, e = expert;
     src = after;
@@ -500,10 +503,10 @@ moe_quant_kernel(const RouteIds r, const T* __restrict__ x, int64_t width, const
     const ST* sm = smooth == nullptr ? nullptr : smooth + (smooth_rows > 1 ? (int64_t)e * width : 0);
     if constexpr (ITERS > 0) {
       if (sm_expert < 0 || (smooth_rows > 1 && e != sm_expert)) {
-        load_smooth_row<ST, ITERS>(sm, nvec, sm_row);
+        load_smooth_row<ST, ITERS, FULL>(sm, nvec, sm_row);
         sm_expert = e;
       }
-      quant_row_store<T, ITERS>(raw, sm_row, nvec, out + row * width, out_scale + row, red[par]);
+      quant_row_store<T, ITERS, FULL>(raw, sm_row, nvec, out + row * width, out_scale + row, red[par]);
     } else {
       quant_row_generic<T, ST>(x + (int64_t)(here / r.topk) * width, sm, width, out + row * width, out_scale + row, red[par]);
     }
@@ -655,6 +658,39 @@ moe_combine_grad_kernel(const T* __restrict__ dy, const T* __restrict__ rows, in
   }
 }
 
+// Values of a 16-byte vector as pairs of floats, for the packed two-wide arithmetic, and back.
+template <typename T>
+__device__ __forceinline__ void unpack_pairs(const uint4& raw, float2 (&f)[16 / (2 * (int)sizeof(T))]) {
+  if constexpr (sizeof(T) == 4) {
+    f[0] = make_float2(__uint_as_float(raw.x), __uint_as_float(raw.y));
+    f[1] = make_float2(__uint_as_float(raw.z), __uint_as_float(raw.w));
+  } else {
+    f[0] = unpack2<T>(raw.x), f[1] = unpack2<T>(raw.y), f[2] = unpack2<T>(raw.z), f[3] = unpack2<T>(raw.w);
+  }
+}
+template <typename T>
+__device__ __forceinline__ uint4 pack_pairs(const float2 (&f)[16 / (2 * (int)sizeof(T))]) {
+  if constexpr (sizeof(T) == 4) {
+    return make_uint4(__float_as_uint(f[0].x), __float_as_uint(f[0].y), __float_as_uint(f[1].x), __float_as_uint(f[1].y));
+  } else if constexpr (std::is_same<T, __half>::value) {
+    uint32_t w[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const __half2 h = __float22half2_rn(f[j]);
+      w[j] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+  } else {
+    uint32_t w[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const __nv_bfloat162 h = __float22bfloat162_rn(f[j]);
+      w[j] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
+
 // Both directions for many tokens, as a pipeline: a producer warp brings the rows of a token (lane k the row of slot k) and,
 // for the gradient, dy into shared memory with bulk copies, kGatherBytes of every row a stage; eight warps work on them,
 // a 16-byte vector of every row a thread.  The rows lie all over HBM and their indices have to be read first; the ring of
@@ -673,8 +709,8 @@ struct GatherLayout {
   static constexpr int kFit = (kGatherSmem - 1024) / kStageBytes;
   static constexpr int kStages = kFit < 16 ? kFit : 16;
   static constexpr int kBarOff = kStages * kStageBytes;        // full[S], empty[S]
-  static constexpr int kMetaOff = kBarOff + 2 * kStages * 8;   // per stage and slot: row, weight
-  static constexpr int kDynamic = kMetaOff + kStages * KC * 8 + 128;
+  static constexpr int kMetaOff = kBarOff + 2 * kStages * 8;   // per stage and slot: row, weight; then whether all slots have rows
+  static constexpr int kDynamic = kMetaOff + kStages * (KC + 1) * 8 + 128;
 };
 
 template <typename T, int KC, bool GRAD>
@@ -730,11 +766,13 @@ moe_gather_kernel(const T* __restrict__ dy, const T* __restrict__ rows, int64_t 
       }
       if (GRAD && lane == KC) src = reinterpret_cast<const uint8_t*>(dy) + t * row_bytes;
       const int copies = __popc(__ballot_sync(0xffffffffu, src != nullptr));
+      const int all = copies == KC + (GRAD ? 1 : 0);
       for (int sg = 0; sg < segs; ++sg) {
         const uint32_t bytes = (uint32_t)min((int64_t)kGatherBytes, row_bytes - (int64_t)sg * kGatherBytes);
         ok = __all_sync(0xffffffffu, mbar_wait(&empty[stage], phase ^ 1, abort_flag, kDevTimeoutProducer));
         if (!ok) break;
-        if (lane < KC) meta[stage * KC + lane] = make_int2((int)row, __float_as_int(w));
+        if (lane < KC) meta[stage * (KC + 1) + lane] = make_int2((int)row, __float_as_int(w));
+        if (lane == KC) meta[stage * (KC + 1) + KC] = make_int2(all, 0);
         __syncwarp();
         if (lane == 0) mbar_arrive_expect_tx(&full[stage], bytes * copies);
         __syncwarp();
@@ -751,46 +789,57 @@ moe_gather_kernel(const T* __restrict__ dy, const T* __restrict__ rows, int64_t 
     bool ok = true;
     int par = 0;
     for (int64_t t = blockIdx.x; t < tokens; t += gridDim.x, par ^= 1) {
-      float dot[KC];
+      float2 dot[KC];
 #pragma unroll
-      for (int k = 0; k < KC; ++k) dot[k] = 0.0f;
+      for (int k = 0; k < KC; ++k) dot[k] = make_float2(0.0f, 0.0f);
       for (int sg = 0; sg < segs; ++sg) {
         ok = mbar_wait(&full[stage], phase, abort_flag, kDevTimeoutEpilogue) && ok;
         const int64_t at = (int64_t)sg * kGatherBytes + threadIdx.x * 16;
         if (ok && at < row_bytes) {
           const uint8_t* in = smem + stage * L::kStageBytes + threadIdx.x * 16;
+          const int2* slots = meta + stage * (KC + 1);
           if constexpr (GRAD) {
-            float g[E::N];
-            E::unpack(*reinterpret_cast<const uint4*>(in + KC * kGatherBytes), g);
+            float2 g[E::N / 2];
+            unpack_pairs<T>(*reinterpret_cast<const uint4*>(in + KC * kGatherBytes), g);
+            auto slot = [&](int k, int2 m) {
+              float2 f[E::N / 2];
+              unpack_pairs<T>(*reinterpret_cast<const uint4*>(in + k * kGatherBytes), f);
+              const float2 w = make_float2(__int_as_float(m.y), __int_as_float(m.y));
 #pragma unroll
-            for (int k = 0; k < KC; ++k) {
-              const int2 m = meta[stage * KC + k];
-              if (m.x < 0) continue;
-              const float w = __int_as_float(m.y);
-              float f[E::N];
-              E::unpack(*reinterpret_cast<const uint4*>(in + k * kGatherBytes), f);
-#pragma unroll
-              for (int j = 0; j < E::N; ++j) {
-                dot[k] = fmaf(f[j], g[j], dot[k]);
-                f[j] = w * g[j];
+              for (int j = 0; j < E::N / 2; ++j) {
+                dot[k] = __ffma2_rn(f[j], g[j], dot[k]);
+                f[j] = __fmul2_rn(w, g[j]);
               }
-              __stcs(reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(out) + m.x * row_bytes + at), E::pack(f));
+              __stcs(reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(out) + m.x * row_bytes + at), pack_pairs<T>(f));
+            };
+            if (slots[KC].x) {                             // the same for all threads
+#pragma unroll
+              for (int k = 0; k < KC; ++k) slot(k, slots[k]);
+            } else {
+#pragma unroll
+              for (int k = 0; k < KC; ++k)
+                if (slots[k].x >= 0) slot(k, slots[k]);
             }
           } else {
-            float acc[E::N];
+            float2 acc[E::N / 2];
 #pragma unroll
-            for (int j = 0; j < E::N; ++j) acc[j] = 0.0f;
+            for (int j = 0; j < E::N / 2; ++j) acc[j] = make_float2(0.0f, 0.0f);
+            auto slot = [&](int k) {
+              float2 f[E::N / 2];
+              unpack_pairs<T>(*reinterpret_cast<const uint4*>(in + k * kGatherBytes), f);
+              const float w = __int_as_float(slots[k].y);
 #pragma unroll
-            for (int k = 0; k < KC; ++k) {
-              const int2 m = meta[stage * KC + k];
-              if (m.x < 0) continue;
-              const float w = __int_as_float(m.y);
-              float f[E::N];
-              E::unpack(*reinterpret_cast<const uint4*>(in + k * kGatherBytes), f);
+              for (int j = 0; j < E::N / 2; ++j) acc[j] = __ffma2_rn(make_float2(w, w), f[j], acc[j]);
+            };
+            if (slots[KC].x) {                             // the same for all threads: no branch between the loads
 #pragma unroll
-              for (int j = 0; j < E::N; ++j) acc[j] = fmaf(w, f[j], acc[j]);
+              for (int k = 0; k < KC; ++k) slot(k);
+            } else {
+#pragma unroll
+              for (int k = 0; k < KC; ++k)
+                if (slots[k].x >= 0) slot(k);
             }
-            __stcs(reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(out) + t * row_bytes + at), E::pack(acc));
+            __stcs(reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(out) + t * row_bytes + at), pack_pairs<T>(acc));
           }
         }
         __syncwarp();
@@ -800,9 +849,10 @@ moe_gather_kernel(const T* __restrict__ dy, const T* __restrict__ rows, int64_t 
       if constexpr (GRAD) {
 #pragma unroll
         for (int k = 0; k < KC; ++k) {
+          float d = dot[k].x + dot[k].y;
 #pragma unroll
-          for (int o = 16; o > 0; o >>= 1) dot[k] += __shfl_xor_sync(0xffffffffu, dot[k], o);
-          if (lane == 0) red[par][k][warp] = dot[k];
+          for (int o = 16; o > 0; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
+          if (lane == 0) red[par][k][warp] = d;
         }
         named_barrier_sync(1, 32 * kGatherWarps);
         if (ok && (int)threadIdx.x < topk) {
@@ -918,9 +968,19 @@ int launch_route_quant_iters(const b200q_moe_route_args& a, const RouteIds& r, i
     return check_launch("moe_route (quantised, few tokens)");
   }
   if (int rc = launch_sort<IdT>(r, a.row_idx, row_src, a.expert_tokens, a.cumulative, valid_rows, st)) return rc;
-  const int64_t cap = (int64_t)sm_count() * resident_ctas<moe_quant_kernel<IdT, T, ST, ITERS>>(threads);
-  return launch_dependent(moe_quant_kernel<IdT, T, ST, ITERS>, (unsigned)(r.n < cap ? r.n : cap), threads, st, "moe_route (quantised)", r, x, a.hidden, sm,
-                          (int)a.scale_rows, out, a.out_scale, static_cast<const int32_t*>(row_src), static_cast<const int32_t*>(valid_rows));
+#define B200Q_ROUTE_QUANT(FULL)                                                                                                        \
+  {                                                                                                                                    \
+    constexpr auto kern = moe_quant_kernel<IdT, T, ST, ITERS, FULL>;                                                                   \
+    const int64_t cap = (int64_t)sm_count() * resident_ctas<kern>(threads);                                                            \
+    return launch_dependent(kern, (unsigned)(r.n < cap ? r.n : cap), threads, st, "moe_route (quantised)", r, x, a.hidden, sm,         \
+                            (int)a.scale_rows, out, a.out_scale, static_cast<const int32_t*>(row_src),                                 \
+                            static_cast<const int32_t*>(valid_rows));                                                                  \
+  }
+  if constexpr (ITERS > 0) {
+    if (a.hidden == (int64_t)threads * ITERS * 8) B200Q_ROUTE_QUANT(true)
+  }
+  B200Q_ROUTE_QUANT(false)
+#undef B200Q_ROUTE_QUANT
 }
 
 template <typename IdT, typename T, typename ST>
@@ -928,9 +988,10 @@ int launch_route_quant(const b200q_moe_route_args& a, const RouteIds& r, int32_t
   const bool vec = a.hidden % 8 == 0 && a.hidden > 0 && a.hidden <= 8 * 512 * 4 && aligned(a.x, 16) && aligned(a.out, 8) &&
                    (a.scale == nullptr || aligned(a.scale, 16));
   if (!vec) return launch_route_quant_iters<IdT, T, ST, 0>(a, r, 256, row_src, valid_rows, st);
+  // Two vectors a thread up to 8192 columns: with four, the row, the next row and the smooth scales take so many registers that half
+  // as many warps fit on an SM.
   const int nvec = (int)(a.hidden / 8);
-  int iters = 1;
-  while (iters < 4 && nvec > iters * 256) iters *= 2;
+  const int iters = nvec <= 128 ? 1 : nvec <= 1024 ? 2 : 4;
   const int threads = (int)ceil_div(ceil_div(nvec, iters), 32) * 32;
   switch (iters) {
     case 1: return launch_route_quant_iters<IdT, T, ST, 1>(a, r, threads, row_src, valid_rows, st);
@@ -1005,6 +1066,7 @@ int gather(const void* dy, const void* rows, int64_t num_rows, const int32_t* ro
   if (topk == 1) B200Q_GATHER(1);
   if (topk == 2) B200Q_GATHER(2);
   if (topk <= 4) B200Q_GATHER(4);
+  if (topk <= 6) B200Q_GATHER(6);
   B200Q_GATHER(8);
 #undef B200Q_GATHER
 }
