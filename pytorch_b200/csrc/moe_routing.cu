@@ -43,7 +43,8 @@ __device__ __forceinline__ int expert_of(const IdT* __restrict__ ids, int64_t i,
 // memory; a prefix over warps, over the CTAs of the cluster (through distributed shared memory) and over the experts
 // turns the counts into first rows; pass 2 walks the indices again, 32 a step, and hands the rows out: the lanes with the
 // same expert find one another by a ballot for each bit of the expert's number, and one of them moves the expert's next
-// row on.  No global scratch, no atomics outside shared memory, no waiting but the cluster's barrier.
+// row on.  row_info, when wanted, gets the token and the expert of every row that has an owner.  No global scratch, no atomics
+// outside shared memory, no waiting but the cluster's barrier.
 constexpr int kSortThreads = 1024;
 constexpr int kSortWarps = kSortThreads / 32;
 constexpr int kSortBatch = 8;             // index loads in flight per lane
@@ -52,7 +53,7 @@ template <typename IdT, int BITS>           // BITS hold the numbers 0 .. expert
 __global__ void __launch_bounds__(kSortThreads, 1)
 moe_sort_kernel(const IdT* __restrict__ ids, int64_t n, int64_t begin, int experts, int strict_limit,
                 int32_t* __restrict__ row_idx, int32_t* __restrict__ row_src, int64_t* __restrict__ expert_tokens,
-                int cumulative, int32_t* __restrict__ valid_rows) {
+                int cumulative, int32_t* __restrict__ valid_rows, int2* __restrict__ row_info, int topk) {
   extern __shared__ int sort_smem[];
   int* hist = sort_smem;                                   // [kSortWarps][experts]
   int* total = hist + kSortWarps * experts;                // [experts] this CTA's counts
@@ -172,6 +173,7 @@ moe_sort_kernel(const IdT* __restrict__ ids, int64_t n, int64_t begin, int exper
       const int row = e[b] >= 0 ? base + __popc(same & ((1u << lane) - 1)) : -1;
       if (i < n) row_idx[i] = row;
       if (row >= 0 && row_src != nullptr) row_src[row] = (int32_t)i;
+      if (row >= 0 && row_info != nullptr) row_info[row] = make_int2((int)i / topk, key);
       __syncwarp();
     }
     s += kSortBatch;
@@ -456,12 +458,10 @@ moe_quant_direct_kernel(const RouteIds r, const T* __restrict__ x, int64_t width
 
 // Many assignments: persistent CTAs take contiguous pieces of the sorted rows, so a piece mostly stays with one expert,
 // whose smooth scales stay in registers; the next row is in flight during the arithmetic of this one.
-template <typename IdT, typename T, typename ST, int ITERS, bool FULL>
+template <typename T, typename ST, int ITERS, bool FULL>
 __global__ void __launch_bounds__(512)
-moe_quant_kernel(const RouteIds r, const T* __restrict__ x, int64_t width, const ST* __restrict__ smooth, int smooth_rows,
-                 int8_t* __restrict__ out, float* __restrict__ out_scale, const int32_t* __restrict__ row_src,
-                 const int32_t* __restrict__ valid_rows) {
-  const IdT* ids = static_cast<const IdT*>(r.ids);
+moe_quant_kernel(int64_t n, const T* __restrict__ x, int64_t width, const ST* __restrict__ smooth, int smooth_rows, int8_t* __restrict__ out,
+                 float* __restrict__ out_scale, const int2* __restrict__ row_info, const int32_t* __restrict__ valid_rows) {
   __shared__ float red[2][32];
   wait_for_primary();
   const int nvec = (int)(width >> 3);
@@ -470,16 +470,18 @@ moe_quant_kernel(const RouteIds r, const T* __restrict__ x, int64_t width, const
   uint4 raw[ITERS ? ITERS : 1], nxt[ITERS ? ITERS : 1];
   float2 sm_row[ITERS ? ITERS : 1][4];
   int sm_expert = -1;
-  auto load = [&](int src) {
-    if constexpr (ITERS > 0) load_row<T, ITERS, FULL>(x + (int64_t)(src / r.topk) * width, nvec, nxt);
+  auto load = [&](int token) {
+    if constexpr (ITERS > 0) load_row<T, ITERS, FULL>(x + token * width, nvec, nxt);
   };
-  // Row r's assignment is read two rows ahead, its expert and x one row ahead.
-  int src = r0 < r1 ? row_src[r0] : -1;
-  int expert = src >= 0 ? expert_of(ids, src, r.begin, r.experts) : 0;
-  if (src >= 0) load(src);
-  int after = r0 + 1 < r1 ? row_src[r0 + 1] : -1;
+  // A row's token and expert are read two rows ahead, its x one row ahead.
+  int2 here = make_int2(0, 0), after = make_int2(0, 0);
+  if (r0 < r1) {
+    after = row_info[r0];
+    load(after.x);
+  }
+  int2 later = r0 + 1 < r1 ? row_info[r0 + 1] : make_int2(0, 0);
   // This CTA's share of the rows that no assignment owns.
-  const int64_t idle = r.n - valid;
+  const int64_t idle = n - valid;
   for (int64_t row = valid + idle * blockIdx.x / gridDim.x; row < valid + idle * (blockIdx.x + 1) / gridDim.x; ++row) {
     if constexpr (ITERS > 0) {
       for (int v = threadIdx.x; v < nvec; v += blockDim.x) st_stream(reinterpret_cast<uint2*>(out + row * width) + v, make_uint2(0, 0));
@@ -490,25 +492,24 @@ moe_quant_kernel(const RouteIds r, const T* __restrict__ x, int64_t width, const
   }
   int par = 0;
   for (int64_t row = r0; row < r1; ++row) {
+    here = after;
+    after = later;
     if constexpr (ITERS > 0) {
 #pragma unroll
       for (int q = 0; q < ITERS; ++q) raw[q] = nxt[q];
-      if (after >= 0) load(after);
+      if (row + 1 < r1) load(after.x);
     }
-    const int here = src, e = expert;
-    src = after;
-    if (src >= 0) expert = expert_of(ids, src, r.begin, r.experts);
-    after = row + 2 < r1 ? row_src[row + 2] : -1;
+    if (row + 2 < r1) later = row_info[row + 2];
     par ^= 1;                                              // a buffer is written again only behind the other one's barrier
-    const ST* sm = smooth == nullptr ? nullptr : smooth + (smooth_rows > 1 ? (int64_t)e * width : 0);
+    const ST* sm = smooth == nullptr ? nullptr : smooth + (smooth_rows > 1 ? here.y * width : 0);
     if constexpr (ITERS > 0) {
-      if (sm_expert < 0 || (smooth_rows > 1 && e != sm_expert)) {
+      if (sm_expert < 0 || (smooth_rows > 1 && here.y != sm_expert)) {
         load_smooth_row<ST, ITERS, FULL>(sm, nvec, sm_row);
-        sm_expert = e;
+        sm_expert = here.y;
       }
       quant_row_store<T, ITERS, FULL>(raw, sm_row, nvec, out + row * width, out_scale + row, red[par]);
     } else {
-      quant_row_generic<T, ST>(x + (int64_t)(here / r.topk) * width, sm, width, out + row * width, out_scale + row, red[par]);
+      quant_row_generic<T, ST>(x + here.x * width, sm, width, out + row * width, out_scale + row, red[par]);
     }
   }
 }
@@ -903,7 +904,7 @@ constexpr int kSortClusterMax = 16;
 
 template <typename IdT, int BITS>
 int launch_sort_bits(const RouteIds& r, int32_t* row_idx, int32_t* row_src, int64_t* expert_tokens, int cumulative, int32_t* valid_rows,
-                     cudaStream_t st) {
+                     int2* row_info, cudaStream_t st) {
   constexpr auto kern = moe_sort_kernel<IdT, BITS>;
   const int smem = (kSortWarps + 1) * r.experts * (int)sizeof(int);
   if (int rc = ensure_dynamic_smem<kern>((kSortWarps + 1) * kMaxExperts * (int)sizeof(int), "moe_route (sort)")) return rc;
@@ -923,17 +924,17 @@ int launch_sort_bits(const RouteIds& r, int32_t* row_idx, int32_t* row_src, int6
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   cudaError_t err = cudaLaunchKernelEx(&cfg, kern, static_cast<const IdT*>(r.ids), r.n, r.begin, r.experts, r.strict_limit,
-                                       row_idx, row_src, expert_tokens, cumulative, valid_rows);
+                                       row_idx, row_src, expert_tokens, cumulative, valid_rows, row_info, r.topk);
   if (err != cudaSuccess) return fail(B200Q_ERR_LAUNCH, "moe_route (sort): %s", cudaGetErrorString(err));
   return check_launch("moe_route (sort)");
 }
 
 template <typename IdT>
 int launch_sort(const RouteIds& r, int32_t* row_idx, int32_t* row_src, int64_t* expert_tokens, int cumulative, int32_t* valid_rows,
-                cudaStream_t st) {
-  if (r.experts < 64) return launch_sort_bits<IdT, 6>(r, row_idx, row_src, expert_tokens, cumulative, valid_rows, st);
-  if (r.experts < 256) return launch_sort_bits<IdT, 8>(r, row_idx, row_src, expert_tokens, cumulative, valid_rows, st);
-  return launch_sort_bits<IdT, 11>(r, row_idx, row_src, expert_tokens, cumulative, valid_rows, st);
+                int2* row_info, cudaStream_t st) {
+  if (r.experts < 64) return launch_sort_bits<IdT, 6>(r, row_idx, row_src, expert_tokens, cumulative, valid_rows, row_info, st);
+  if (r.experts < 256) return launch_sort_bits<IdT, 8>(r, row_idx, row_src, expert_tokens, cumulative, valid_rows, row_info, st);
+  return launch_sort_bits<IdT, 11>(r, row_idx, row_src, expert_tokens, cumulative, valid_rows, row_info, st);
 }
 
 template <typename IdT, int BYTES>
@@ -948,7 +949,7 @@ int launch_copy(const b200q_moe_route_args& a, const RouteIds& r, int64_t row_by
                                                                               a.row_src, a.expert_tokens, a.cumulative);
     return check_launch("moe_route (copy, few tokens)");
   }
-  if (int rc = launch_sort<IdT>(r, a.row_idx, a.row_src, a.expert_tokens, a.cumulative, valid_rows, st)) return rc;
+  if (int rc = launch_sort<IdT>(r, a.row_idx, a.row_src, a.expert_tokens, a.cumulative, valid_rows, nullptr, st)) return rc;
   constexpr int U = 4;
   const int64_t segs = nvec == 0 ? 1 : ceil_div(nvec, 32 * U);
   const int64_t move_blocks = ceil_div(a.tokens * segs, 8), blocks = move_blocks + 2 * sm_count();
@@ -958,7 +959,7 @@ int launch_copy(const b200q_moe_route_args& a, const RouteIds& r, int64_t row_by
 }
 
 template <typename IdT, typename T, typename ST, int ITERS>
-int launch_route_quant_iters(const b200q_moe_route_args& a, const RouteIds& r, int threads, int32_t* row_src, int32_t* valid_rows, cudaStream_t st) {
+int launch_route_quant_iters(const b200q_moe_route_args& a, const RouteIds& r, int threads, int2* row_info, int32_t* valid_rows, cudaStream_t st) {
   const T* x = static_cast<const T*>(a.x);
   const ST* sm = static_cast<const ST*>(a.scale);
   int8_t* out = static_cast<int8_t*>(a.out);
@@ -967,13 +968,13 @@ int launch_route_quant_iters(const b200q_moe_route_args& a, const RouteIds& r, i
                                                                                         a.row_idx, a.row_src, a.expert_tokens, a.cumulative);
     return check_launch("moe_route (quantised, few tokens)");
   }
-  if (int rc = launch_sort<IdT>(r, a.row_idx, row_src, a.expert_tokens, a.cumulative, valid_rows, st)) return rc;
+  if (int rc = launch_sort<IdT>(r, a.row_idx, a.row_src, a.expert_tokens, a.cumulative, valid_rows, row_info, st)) return rc;
 #define B200Q_ROUTE_QUANT(FULL)                                                                                                        \
   {                                                                                                                                    \
-    constexpr auto kern = moe_quant_kernel<IdT, T, ST, ITERS, FULL>;                                                                   \
+    constexpr auto kern = moe_quant_kernel<T, ST, ITERS, FULL>;                                                                        \
     const int64_t cap = (int64_t)sm_count() * resident_ctas<kern>(threads);                                                            \
-    return launch_dependent(kern, (unsigned)(r.n < cap ? r.n : cap), threads, st, "moe_route (quantised)", r, x, a.hidden, sm,         \
-                            (int)a.scale_rows, out, a.out_scale, static_cast<const int32_t*>(row_src),                                 \
+    return launch_dependent(kern, (unsigned)(r.n < cap ? r.n : cap), threads, st, "moe_route (quantised)", r.n, x, a.hidden, sm,       \
+                            (int)a.scale_rows, out, a.out_scale, static_cast<const int2*>(row_info),                                   \
                             static_cast<const int32_t*>(valid_rows));                                                                  \
   }
   if constexpr (ITERS > 0) {
@@ -984,24 +985,24 @@ int launch_route_quant_iters(const b200q_moe_route_args& a, const RouteIds& r, i
 }
 
 template <typename IdT, typename T, typename ST>
-int launch_route_quant(const b200q_moe_route_args& a, const RouteIds& r, int32_t* row_src, int32_t* valid_rows, cudaStream_t st) {
+int launch_route_quant(const b200q_moe_route_args& a, const RouteIds& r, int2* row_info, int32_t* valid_rows, cudaStream_t st) {
   const bool vec = a.hidden % 8 == 0 && a.hidden > 0 && a.hidden <= 8 * 512 * 4 && aligned(a.x, 16) && aligned(a.out, 8) &&
                    (a.scale == nullptr || aligned(a.scale, 16));
-  if (!vec) return launch_route_quant_iters<IdT, T, ST, 0>(a, r, 256, row_src, valid_rows, st);
+  if (!vec) return launch_route_quant_iters<IdT, T, ST, 0>(a, r, 256, row_info, valid_rows, st);
   // Two vectors a thread up to 8192 columns: with four, the row, the next row and the smooth scales take so many registers that half
   // as many warps fit on an SM.
   const int nvec = (int)(a.hidden / 8);
   const int iters = nvec <= 128 ? 1 : nvec <= 1024 ? 2 : 4;
   const int threads = (int)ceil_div(ceil_div(nvec, iters), 32) * 32;
   switch (iters) {
-    case 1: return launch_route_quant_iters<IdT, T, ST, 1>(a, r, threads, row_src, valid_rows, st);
-    case 2: return launch_route_quant_iters<IdT, T, ST, 2>(a, r, threads, row_src, valid_rows, st);
-    default: return launch_route_quant_iters<IdT, T, ST, 4>(a, r, threads, row_src, valid_rows, st);
+    case 1: return launch_route_quant_iters<IdT, T, ST, 1>(a, r, threads, row_info, valid_rows, st);
+    case 2: return launch_route_quant_iters<IdT, T, ST, 2>(a, r, threads, row_info, valid_rows, st);
+    default: return launch_route_quant_iters<IdT, T, ST, 4>(a, r, threads, row_info, valid_rows, st);
   }
 }
 
 template <typename IdT>
-int route(const b200q_moe_route_args& a, const RouteIds& r, int32_t* row_src, int32_t* valid_rows, cudaStream_t st) {
+int route(const b200q_moe_route_args& a, const RouteIds& r, int2* row_info, int32_t* valid_rows, cudaStream_t st) {
   if (!a.quantise) {
     const int64_t bytes = a.hidden * element_bytes(a.x_dtype);
     switch (chunk_bytes(bytes, {a.x, a.out})) {
@@ -1014,16 +1015,16 @@ int route(const b200q_moe_route_args& a, const RouteIds& r, int32_t* row_src, in
   }
   const bool f32 = a.scale == nullptr || a.scale_dtype == B200Q_F32;
   if (a.x_dtype == B200Q_BF16)
-    return f32 ? launch_route_quant<IdT, __nv_bfloat16, float>(a, r, row_src, valid_rows, st)
-               : launch_route_quant<IdT, __nv_bfloat16, __nv_bfloat16>(a, r, row_src, valid_rows, st);
-  return f32 ? launch_route_quant<IdT, __half, float>(a, r, row_src, valid_rows, st)
-             : launch_route_quant<IdT, __half, __half>(a, r, row_src, valid_rows, st);
+    return f32 ? launch_route_quant<IdT, __nv_bfloat16, float>(a, r, row_info, valid_rows, st)
+               : launch_route_quant<IdT, __nv_bfloat16, __nv_bfloat16>(a, r, row_info, valid_rows, st);
+  return f32 ? launch_route_quant<IdT, __half, float>(a, r, row_info, valid_rows, st)
+             : launch_route_quant<IdT, __half, __half>(a, r, row_info, valid_rows, st);
 }
 
-// [valid rows: 1 word, padded to 256 bytes][row -> assignment: n words, quantised form only]
+// [valid rows: 1 word, padded to 256 bytes][row -> token and expert: 2 n words, quantised form only]
 size_t route_workspace(int64_t n, int quantise) {
   if (n <= kDirectIds) return 0;
-  return 256 + (quantise ? (size_t)n * 4 : 0);
+  return 256 + (quantise ? (size_t)n * 8 : 0);
 }
 
 template <typename T, bool VEC>
@@ -1173,10 +1174,9 @@ extern "C" int b200q_moe_route(const b200q_moe_route_args* a, void* stream) {
   B200Q_REQUIRE(need == 0 || (a->workspace != nullptr && a->workspace_bytes >= need && aligned(a->workspace, 256)), B200Q_ERR_WORKSPACE,
                 "moe_route: needs %zu bytes of 256-byte aligned workspace, got %zu", need, a->workspace_bytes);
   int32_t* valid_rows = static_cast<int32_t*>(a->workspace);
-  int32_t* row_src = a->row_src != nullptr || !a->quantise || need == 0 ? a->row_src
-                                                                         : reinterpret_cast<int32_t*>(static_cast<uint8_t*>(a->workspace) + 256);
+  int2* row_info = a->quantise && need != 0 ? reinterpret_cast<int2*>(static_cast<uint8_t*>(a->workspace) + 256) : nullptr;
   RouteIds r{a->expert_idx, n, a->expert_begin, (int)(a->expert_end - a->expert_begin), (int)a->topk, a->strict ? (int)a->expert_end : 0};
-  return a->idx_dtype == B200Q_I64 ? route<int64_t>(*a, r, row_src, valid_rows, st) : route<int32_t>(*a, r, row_src, valid_rows, st);
+  return a->idx_dtype == B200Q_I64 ? route<int64_t>(*a, r, row_info, valid_rows, st) : route<int32_t>(*a, r, row_info, valid_rows, st);
 }
 
 extern "C" int b200q_moe_combine(const void* rows, int dtype, int64_t num_rows, const int32_t* row_idx, const void* weights, int weight_dtype,

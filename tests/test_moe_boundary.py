@@ -101,7 +101,7 @@ def test_route_argument_checks(lib):
         assert lib.b200q_moe_route(args(**kw), None) == status and what in last(), (kw, last())
     assert lib.b200q_moe_route(args(tokens=0, out_rows=0), None) == cabi.OK
     assert lib.b200q_moe_route_workspace_bytes(2048, 1) == 0 and lib.b200q_moe_route_workspace_bytes(0, 1) == 0
-    assert lib.b200q_moe_route_workspace_bytes(4096, 1) == 256 + 4 * 4096 and lib.b200q_moe_route_workspace_bytes(4096, 0) == 256
+    assert lib.b200q_moe_route_workspace_bytes(4096, 1) == 256 + 8 * 4096 and lib.b200q_moe_route_workspace_bytes(4096, 0) == 256
 
 
 def test_combine_argument_checks(lib):
