@@ -601,12 +601,36 @@ std::vector<Tensor> grouped_matmul_meta(at::TensorList x, at::TensorList weight,
 }
 
 // ---------------------------------------------------------------------------------------------
-// Autograd
+// Autograd.  Both directions go through the dispatcher below the autograd keys, so that a dispatch mode (fake tensors, a profiler of
+// operators) sees the operators that run, the gradients among them.
+template <typename F>
+c10::TypedOperatorHandle<F> operator_handle(const char* name) {
+  return c10::Dispatcher::singleton().findSchemaOrThrow(name, "").typed<F>();
+}
+
+std::tuple<Tensor, Tensor> permute_below(const Tensor& tokens, const Tensor& indices, optional<int64_t> num_out, bool padded_mode) {
+  static const auto op = operator_handle<decltype(permute_cuda)>("npu::npu_moe_token_permute");
+  at::AutoDispatchBelowADInplaceOrView below;
+  return op.call(tokens, indices, num_out, padded_mode);
+}
+
+Tensor unpermute_below(const Tensor& rows, const Tensor& sorted, const optional<Tensor>& probs, bool padded_mode, at::OptionalIntArrayRef restore_shape) {
+  static const auto op = operator_handle<decltype(unpermute_cuda)>("npu::npu_moe_token_unpermute");
+  at::AutoDispatchBelowADInplaceOrView below;
+  return op.call(rows, sorted, probs, padded_mode, restore_shape);
+}
+
+NormOutputs norm_below(const Tensor& x, const Tensor& residual, const Tensor& gamma, const optional<Tensor>& post, const optional<Tensor>& gate,
+                       double residual_scale, double epsilon) {
+  static const auto op = operator_handle<decltype(norm_cuda)>("npu::npu_gated_add_rms_norm");
+  at::AutoDispatchBelowADInplaceOrView below;
+  return op.call(x, residual, gamma, post, gate, residual_scale, epsilon);
+}
+
 class PermuteFunction : public torch::autograd::Function<PermuteFunction> {
  public:
   static variable_list forward(AutogradContext* ctx, const Tensor& tokens, const Tensor& indices, optional<int64_t> num_out, bool padded_mode) {
-    at::AutoDispatchBelowADInplaceOrView below;
-    auto [rows, sorted] = permute_cuda(tokens, indices, num_out, padded_mode);
+    auto [rows, sorted] = permute_below(tokens, indices, num_out, padded_mode);
     ctx->set_materialize_grads(false);
     ctx->mark_non_differentiable({sorted});
     ctx->save_for_backward({sorted});
@@ -616,21 +640,21 @@ class PermuteFunction : public torch::autograd::Function<PermuteFunction> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     if (!grads[0].defined()) return {Tensor(), Tensor(), Tensor(), Tensor()};
-    constexpr const char* op = "npu_moe_token_permute_grad";
-    no_second_derivative(op);
+    no_second_derivative("npu_moe_token_permute_grad");
+    static const auto op = operator_handle<decltype(permute_grad_cuda)>("npu::npu_moe_token_permute_grad");
+    at::AutoDispatchBelowADInplaceOrView below;
     const Tensor sorted = ctx->get_saved_variables()[0];
     const int64_t tokens = ctx->saved_data["tokens"].toInt(), topk = ctx->saved_data["topk"].toInt();
-    c10::cuda::CUDAGuard guard(grads[0].device());
-    surface_device_error(op, grads[0]);
-    Tensor g = topk == 0 ? at::zeros({tokens, grads[0].size(1)}, grads[0].options()) : combine_cuda(op, grads[0], sorted, {}, tokens, topk);
+    // The operator takes the shapes of tokens and indices only: neither is kept for it.
+    const Tensor shape = at::empty({1, 1}, grads[0].options()).expand({tokens, grads[0].size(1)});
+    Tensor g = op.call(shape, grads[0], sorted.view({tokens, topk}), sorted, false);
     return {g, Tensor(), Tensor(), Tensor()};
   }
 };
 
 std::tuple<Tensor, Tensor> permute_autograd(const Tensor& tokens, const Tensor& indices, optional<int64_t> num_out, bool padded_mode) {
   if (!(at::GradMode::is_enabled() && tokens.requires_grad())) {
-    at::AutoDispatchBelowADInplaceOrView below;
-    return permute_cuda(tokens, indices, num_out, padded_mode);
+    return permute_below(tokens, indices, num_out, padded_mode);
   }
   auto out = PermuteFunction::apply(tokens, indices, num_out, padded_mode);
   return {out[0], out[1]};
@@ -640,8 +664,7 @@ class UnpermuteFunction : public torch::autograd::Function<UnpermuteFunction> {
  public:
   static variable_list forward(AutogradContext* ctx, const Tensor& rows, const Tensor& sorted, const optional<Tensor>& probs, bool padded_mode,
                                at::OptionalIntArrayRef restore_shape) {
-    at::AutoDispatchBelowADInplaceOrView below;
-    Tensor out = unpermute_cuda(rows, sorted, probs, padded_mode, restore_shape);
+    Tensor out = unpermute_below(rows, sorted, probs, padded_mode, restore_shape);
     ctx->set_materialize_grads(false);
     ctx->save_for_backward({rows, sorted, probs.value_or(Tensor())});
     return {out};
@@ -649,9 +672,11 @@ class UnpermuteFunction : public torch::autograd::Function<UnpermuteFunction> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     if (!grads[0].defined()) return {Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
     no_second_derivative("npu_moe_token_unpermute_grad");
+    static const auto op = operator_handle<decltype(unpermute_grad_cuda)>("npu::npu_moe_token_unpermute_grad");
+    at::AutoDispatchBelowADInplaceOrView below;
     auto saved = ctx->get_saved_variables();
     const optional<Tensor> probs = saved[2].defined() ? optional<Tensor>(saved[2]) : optional<Tensor>();
-    auto [drows, dprobs] = unpermute_grad_cuda(saved[0], grads[0], saved[1], probs, false, c10::nullopt);
+    auto [drows, dprobs] = op.call(saved[0], grads[0], saved[1], probs, false, c10::nullopt);
     return {drows, Tensor(), probs.has_value() ? dprobs : Tensor(), Tensor(), Tensor()};
   }
 };
@@ -659,8 +684,7 @@ class UnpermuteFunction : public torch::autograd::Function<UnpermuteFunction> {
 Tensor unpermute_autograd(const Tensor& rows, const Tensor& sorted, const optional<Tensor>& probs, bool padded_mode,
                           at::OptionalIntArrayRef restore_shape) {
   if (!(at::GradMode::is_enabled() && (rows.requires_grad() || (probs.has_value() && probs->requires_grad())))) {
-    at::AutoDispatchBelowADInplaceOrView below;
-    return unpermute_cuda(rows, sorted, probs, padded_mode, restore_shape);
+    return unpermute_below(rows, sorted, probs, padded_mode, restore_shape);
   }
   return UnpermuteFunction::apply(rows, sorted, probs, padded_mode, restore_shape)[0];
 }
@@ -669,8 +693,7 @@ class NormFunction : public torch::autograd::Function<NormFunction> {
  public:
   static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& residual, const Tensor& gamma, const optional<Tensor>& post,
                                const optional<Tensor>& gate, double residual_scale, double epsilon) {
-    at::AutoDispatchBelowADInplaceOrView below;
-    auto [y, rstd, h, post_rstd] = norm_cuda(x, residual, gamma, post, gate, residual_scale, epsilon);
+    auto [y, rstd, h, post_rstd] = norm_below(x, residual, gamma, post, gate, residual_scale, epsilon);
     ctx->set_materialize_grads(false);
     ctx->mark_non_differentiable({rstd, post_rstd});
     ctx->save_for_backward({x, residual, gamma, post.value_or(Tensor()), gate.value_or(Tensor()), rstd, post_rstd});
@@ -681,12 +704,13 @@ class NormFunction : public torch::autograd::Function<NormFunction> {
     variable_list out(7);
     if (!grads[0].defined() && !grads[2].defined()) return out;
     no_second_derivative("npu_gated_add_rms_norm_grad");
+    static const auto op = operator_handle<decltype(norm_grad_cuda)>("npu::npu_gated_add_rms_norm_grad");
+    at::AutoDispatchBelowADInplaceOrView below;
     auto s = ctx->get_saved_variables();
     auto opt = [](const Tensor& t) { return t.defined() ? optional<Tensor>(t) : optional<Tensor>(); };
-    c10::cuda::CUDAGuard guard(s[0].device());
     const Tensor dy = grads[0].defined() ? grads[0] : at::zeros(s[0].sizes(), s[0].options());
-    auto [dx, dres, dgamma, dpost, dgate] = norm_grad_cuda(dy, opt(grads[2]), s[0], s[1], s[2], s[5], opt(s[3]), opt(s[4]), opt(s[6]),
-                                                           ctx->saved_data["residual_scale"].toDouble());
+    auto [dx, dres, dgamma, dpost, dgate] = op.call(dy, opt(grads[2]), s[0], s[1], s[2], s[5], opt(s[3]), opt(s[4]), opt(s[6]),
+                                                   ctx->saved_data["residual_scale"].toDouble());
     out[0] = dx;
     out[1] = dres;
     out[2] = dgamma;
@@ -701,8 +725,7 @@ NormOutputs norm_autograd(const Tensor& x, const Tensor& residual, const Tensor&
   const bool wanted = x.requires_grad() || residual.requires_grad() || gamma.requires_grad() || (post.has_value() && post->requires_grad()) ||
                       (gate.has_value() && gate->requires_grad());
   if (!(at::GradMode::is_enabled() && wanted)) {
-    at::AutoDispatchBelowADInplaceOrView below;
-    return norm_cuda(x, residual, gamma, post, gate, residual_scale, epsilon);
+    return norm_below(x, residual, gamma, post, gate, residual_scale, epsilon);
   }
   auto o = NormFunction::apply(x, residual, gamma, post, gate, residual_scale, epsilon);
   return {o[0], o[1], o[2], o[3]};

@@ -136,3 +136,18 @@ def test_training_step(pb):
     for name, u, v in zip(leaves, got, want):
         # the padded tokens' last norm has a mean of squares of zero: epsilon makes its factor 1000
         assert bool(((u.cpu().double() - v).abs() <= 1e-4 * v.abs().max()).all()), name
+
+
+def test_fake_tensors_in_both_directions(pb):
+    """Under a dispatch mode a training step runs on shapes alone: the gradients are operators that the mode sees."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    with FakeTensorMode():
+        def leaf(*shape, dtype=torch.bfloat16):
+            return torch.empty(*shape, dtype=dtype, device="cuda", requires_grad=True)
+
+        x, res, w, post, gate, probs = leaf(6, 64), leaf(6, 64), leaf(64), leaf(64), leaf(6, 1), leaf(6, 2, dtype=torch.float32)
+        y, _, h, _ = pb.npu_gated_add_rms_norm(x, res, w, post_gamma=post, gate=gate)
+        rows, place = pb.npu_moe_token_permute(y, torch.empty(6, 2, dtype=torch.int64, device="cuda"))
+        (pb.npu_moe_token_unpermute(rows, place, probs).sum() + h.sum()).backward()
+        for t in (x, res, w, post, gate, probs):
+            assert t.grad.shape == t.shape and t.grad.dtype == t.dtype and t.grad.device.type == "cuda"

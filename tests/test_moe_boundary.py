@@ -252,3 +252,33 @@ def test_grouped_matmul_argument_checks(lib):
             (dict(out=p + 1), cabi.ERR_BAD_ARG, "misaligned")]:
         assert run(**kw) == status and what in last(), (kw, last())
     assert run(m=0) == cabi.OK and run(n=0) == cabi.OK
+
+
+def test_fake_tensors():
+    """Under a dispatch mode the operators run on shapes alone, also where autograd is on (the backward pass itself needs a
+    device for its thread)."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    import pytorch_b200 as pkg
+    with FakeTensorMode():
+        def leaf(*shape, dtype=torch.bfloat16):
+            return torch.empty(*shape, dtype=dtype, device="cuda", requires_grad=True)
+
+        x, res, w, post, gate = leaf(6, 64), leaf(6, 64), leaf(64), leaf(64), leaf(6, 1)
+        y, rstd, h, post_rstd = pkg.npu_gated_add_rms_norm(x, res, w, post_gamma=post, gate=gate)
+        assert y.requires_grad and h.requires_grad and not rstd.requires_grad and not post_rstd.requires_grad
+        rows, sorted_idx = pkg.npu_moe_token_permute(y, torch.empty(6, 2, dtype=torch.int64, device="cuda"))
+        assert rows.shape == (12, 64) and sorted_idx.shape == (12,) and sorted_idx.dtype == torch.int32
+        probs = leaf(6, 2, dtype=torch.float32)
+        out = pkg.npu_moe_token_unpermute(rows, sorted_idx, probs)
+        assert out.shape == (6, 64) and out.dtype == torch.bfloat16
+        assert out.requires_grad
+        grads = torch.ops.npu.npu_gated_add_rms_norm_grad(torch.empty_like(y), None, x, res, w, rstd, post_gamma=post, gate=gate, post_rstd=post_rstd)
+        assert [g.shape for g in grads] == [t.shape for t in (x, res, w, post, gate)]
+        grads = torch.ops.npu.npu_moe_token_unpermute_grad(rows, torch.empty_like(out), sorted_idx, probs)
+        assert grads[0].shape == rows.shape and grads[1].shape == probs.shape
+        q, ri, et, sc = pkg.npu_moe_init_routing_v2(y.detach(), torch.empty(6, 2, dtype=torch.int32, device="cuda"), expert_num=4, active_num=12,
+                                                    quant_mode=1, expert_tokens_num_flag=True, expert_tokens_num_type=0)
+        assert q.shape == (12, 64) and q.dtype == torch.int8 and ri.shape == (12,) and et.shape == (4,) and sc.shape == (12,)
+        got = pkg.npu_grouped_matmul([q], [torch.empty(4, 64, 32, dtype=torch.int8, device="cuda")], scale=[torch.empty(4, 32, device="cuda")],
+                                     per_token_scale=[sc], group_list=et, split_item=3, group_type=0, group_list_type=0)
+        assert got[0].shape == (12, 32) and got[0].dtype == torch.bfloat16
