@@ -482,12 +482,12 @@ template <int CTAS, int MAX_TOKENS, int STAGES>
 int launch_grouped(const b200q_grouped_matmul_args& in, const GroupedArgs& a, cudaStream_t st) {
   using L = GroupedLayout<CTAS, MAX_TOKENS, STAGES>;
   GroupedMaps<L::kBRows> maps;
-  if (int rc = make_tmap_3d_cached(&maps.w, in.weight, (uint64_t)in.k, (uint64_t)in.n, (uint64_t)in.groups, (uint64_t)in.w_stride_n,
-                                   (uint64_t)in.w_stride_g, kBK, kTileA, "grouped_matmul (weight)"))
+  if (int rc = make_tmap_3d(&maps.w, in.weight, (uint64_t)in.k, (uint64_t)in.n, (uint64_t)in.groups, (uint64_t)in.w_stride_n,
+                            (uint64_t)in.w_stride_g, kBK, kTileA, "grouped_matmul (weight)"))
     return rc;
   for (int i = 0; i < L::kBRows / 16; ++i)
-    if (int rc = make_tmap_2d_cached(&maps.x[i], CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, in.x, (uint64_t)in.k, (uint64_t)in.m, (uint64_t)in.k, kBK,
-                                     16 * (i + 1), CU_TENSOR_MAP_SWIZZLE_128B, "grouped_matmul (x)"))
+    if (int rc = make_tmap_2d(&maps.x[i], CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, in.x, (uint64_t)in.k, (uint64_t)in.m, (uint64_t)in.k, kBK,
+                              16 * (i + 1), CU_TENSOR_MAP_SWIZZLE_128B, "grouped_matmul (x)"))
       return rc;
   // No more CTAs than there can be units.
   const int64_t tiles = in.m / MAX_TOKENS + (in.groups < in.m ? in.groups : in.m);

@@ -87,46 +87,20 @@ inline int make_tmap_2d_cached(CUtensorMap* out, CUtensorMapDataType dt, int ele
 
 // Stack of row-major int8 matrices [count, outer, inner] with a row pitch and a matrix pitch in bytes; box
 // [1, box_outer, box_inner], 128-byte swizzle.  A box that runs over the last row of one matrix reads zeros there.
-// Cached like the two-dimensional maps.
-inline int make_tmap_3d_cached(CUtensorMap* out, const void* base, uint64_t inner, uint64_t outer, uint64_t count, uint64_t pitch_bytes,
-                               uint64_t matrix_bytes, uint32_t box_inner, uint32_t box_outer, const char* what) {
-  struct Entry {
-    const void* base;
-    uint64_t inner, outer, count, pitch, matrix;
-    uint32_t box_inner, box_outer;
-    bool valid;
-    CUtensorMap map;
-  };
-  static std::mutex mu;
-  static Entry table[64];
-  if (count == 1) matrix_bytes = pitch_bytes * outer;          // the stride of a single matrix is never used
-  uint64_t h = reinterpret_cast<uint64_t>(base) * 0x9E3779B97F4A7C15ull;
-  h ^= (inner * 31 + outer + count * 977) * 0xC2B2AE3D27D4EB4Full + pitch_bytes * 0x165667B19E3779F9ull + box_outer * 131 + box_inner;
-  std::lock_guard<std::mutex> lock(mu);
-  Entry& e = table[(h >> 24) & 63];
-  if (e.valid && e.base == base && e.inner == inner && e.outer == outer && e.count == count && e.pitch == pitch_bytes && e.matrix == matrix_bytes &&
-      e.box_inner == box_inner && e.box_outer == box_outer) {
-    *out = e.map;
-    return B200Q_OK;
-  }
+inline int make_tmap_3d(CUtensorMap* out, const void* base, uint64_t inner, uint64_t outer, uint64_t count, uint64_t pitch_bytes,
+                        uint64_t matrix_bytes, uint32_t box_inner, uint32_t box_outer, const char* what) {
   EncodeTiledFn fn = encode_tiled_fn();
   if (!fn) return fail(B200Q_ERR_LAUNCH, "%s: cuTensorMapEncodeTiled is not available from this driver", what);
+  if (count == 1) matrix_bytes = pitch_bytes * outer;          // the stride of a single matrix is never used
   if (!aligned(base, 16) || pitch_bytes % 16 != 0 || matrix_bytes % 16 != 0 || box_inner % 16 != 0 || box_inner > 128 || box_outer > 256)
     return fail(B200Q_ERR_BAD_ARG, "%s: operand does not meet the TMA alignment rules", what);
   cuuint64_t dims[3] = {inner, outer, count};
   cuuint64_t strides[2] = {pitch_bytes, matrix_bytes};
   cuuint32_t box[3] = {box_inner, box_outer, 1};
   cuuint32_t estr[3] = {1, 1, 1};
-  CUresult r = fn(&e.map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+  CUresult r = fn(out, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  if (r != CUDA_SUCCESS) {
-    e.valid = false;
-    return fail(B200Q_ERR_LAUNCH, "%s: cuTensorMapEncodeTiled failed (CUresult %d)", what, (int)r);
-  }
-  e.base = base; e.inner = inner; e.outer = outer; e.count = count; e.pitch = pitch_bytes; e.matrix = matrix_bytes;
-  e.box_inner = box_inner; e.box_outer = box_outer;
-  e.valid = true;
-  *out = e.map;
+  if (r != CUDA_SUCCESS) return fail(B200Q_ERR_LAUNCH, "%s: cuTensorMapEncodeTiled failed (CUresult %d)", what, (int)r);
   return B200Q_OK;
 }
 
