@@ -13,8 +13,8 @@
 // Bound by HBM: the forward pass reads x and the residual and writes y and h, the gradient reads x, the residual and both
 // gradients and writes two, each once; a row stays in its CTA's registers between the reductions.  Everything between
 // loading and storing is fp32: h is not rounded before its norm, and the gradient computes it again from x and the
-// residual instead of reading the rounded one.  Sums over rows (dw1, dw2, a shared gate) are kept in registers by CTAs
-// that take contiguous rows, written once per CTA as fp32 and added by a second kernel in a fixed order.
+// residual instead of reading the rounded one.  Sums over rows (dw1, dw2, a shared gate) are kept in shared memory or registers
+// by CTAs that take contiguous rows, written once per CTA as fp32 and added by a second kernel in a fixed order.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -206,11 +206,11 @@ constexpr int kRowPipeMaxStages = 4;
 
 // Where the filling of the ring stands: next row, stage, and whether every wait was met.
 struct RowPipeFeed {
-  int64_t row;
+  int row;
   int stage;
   uint32_t phase;
   bool ok;
-  __device__ __forceinline__ void next(int64_t to, int stages) {
+  __device__ __forceinline__ void next(int to, int stages) {
     row = to;
     if (++stage == stages) { stage = 0; phase ^= 1; }
   }
@@ -347,7 +347,7 @@ gated_norm_kernel(const NormArgs a) {
   }
   const float2 alpha = splat(a.alpha);
   for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
-    const int64_t gate_row = a.gate.rows_per == 1 ? row : row / a.gate.rows_per;
+    const int64_t gate_row = a.gate.rows_per == 1 ? row : a.gate.rows_per >= a.rows ? 0 : row / a.gate.rows_per;
     float2 early_gate[4];
     if constexpr (EARLY) gate8<P, VEC>(a.gate, gate_row, 0, a.width, at, early_gate);
     float r1 = 1.0f;
@@ -437,12 +437,12 @@ gated_norm_pipe_kernel(const NormArgs a, int threads_per_row, int stages) {
   __shared__ float red[3][kRowPipeThreads / 32][ROWS][32];
   const int groups = blockDim.x / threads_per_row, chunk_rows = groups * ROWS;
   const RowPipe pipe = row_pipe_init(pipe_smem, stages, 2, chunk_rows, (int64_t)a.width * sizeof(T), a.rows, blockDim.x / 32);
-  const int64_t r0 = a.rows * blockIdx.x / gridDim.x, r1 = a.rows * (blockIdx.x + 1) / gridDim.x;
+  const int r0 = (int)(a.rows * blockIdx.x / gridDim.x), r1 = (int)(a.rows * (blockIdx.x + 1) / gridDim.x);   // fewer than 2^30 rows
   const void* const src[2] = {a.x, a.residual};
   RowPipeFeed feed{r0, 0, 0, true};
   auto fill = [&]() {                                      // by the first warp
     if (feed.row >= r1 || !feed.ok) return;
-    feed.ok = row_pipe_fill(pipe, src, feed.stage, feed.phase, feed.row, (int)min((int64_t)chunk_rows, r1 - feed.row), threadIdx.x & 31);
+    feed.ok = row_pipe_fill(pipe, src, feed.stage, feed.phase, feed.row, min(chunk_rows, r1 - feed.row), threadIdx.x & 31);
     feed.next(feed.row + chunk_rows, stages);
   };
   if (threadIdx.x < 32)
@@ -451,30 +451,48 @@ gated_norm_pipe_kernel(const NormArgs a, int threads_per_row, int stages) {
   uint32_t phase = 0;
   const int group = threadIdx.x / threads_per_row;
   const Place at{(int)threadIdx.x - group * threads_per_row, threads_per_row};
-  const P* gamma = static_cast<const P*>(a.gamma);
   const P* post = static_cast<const P*>(a.post);
   const float2 alpha = splat(a.alpha);
+  // A thread's columns stay the same: so do its parameters, but for the gate.
+  float2 w_post[4], w_gamma[4], w_smooth[4], g[4];
+  if (post != nullptr) param8<P, VEC>(post, 0, a.width, at, w_post);
+  param8<P, VEC>(static_cast<const P*>(a.gamma), 0, a.width, at, w_gamma);
+  if (QUANT && a.smooth != nullptr) {
+    if (a.smooth_f32) param8<float, VEC>(static_cast<const float*>(a.smooth), 0, a.width, at, w_smooth);
+    else param8<T, VEC>(static_cast<const T*>(a.smooth), 0, a.width, at, w_smooth);
+  }
+  // The gate of the group's rows, walked along; rows_per 1: the row itself.
+  const int rows_per = (int)min(a.gate.rows_per, a.rows);
+  int have_gate = -1, gate_at = (r0 + group * ROWS) / rows_per, gate_end = (gate_at + 1) * rows_per;
   bool ok = true;
-  for (int64_t chunk = r0; chunk < r1; chunk += chunk_rows) {
+  for (int chunk = r0; chunk < r1; chunk += chunk_rows) {
     ok = mbar_wait(&pipe.full[stage], phase, pipe.abort_flag, kDevTimeoutEpilogue) && ok;
     if (threadIdx.x < 32 && chunk > r0) fill();
-    const int64_t row = chunk + group * ROWS;
+    const int row = chunk + group * ROWS;
     if (row < r1) {                                        // the same for all threads of the row
       // Past the CTA's last row the row before is worked on again and not stored.
-      const int live = (int)min((int64_t)ROWS, r1 - row);
+      const int live = min(ROWS, r1 - row);
       const uint8_t *xs[ROWS], *rs[ROWS];
-      int64_t gate_row[ROWS];
-      const int64_t off = chunk * pipe.row_bytes - ((chunk * pipe.row_bytes) & ~int64_t(15)) + (int64_t)group * ROWS * pipe.row_bytes;
+      int gate_row[ROWS];
+      const int off = (int)((chunk * pipe.row_bytes) & 15) + group * ROWS * (int)pipe.row_bytes;
 #pragma unroll
       for (int k = 0; k < ROWS; ++k) {
         const int kk = min(k, live - 1);
-        xs[k] = pipe.slot(stage, 0) + off + kk * pipe.row_bytes;
-        rs[k] = pipe.slot(stage, 1) + off + kk * pipe.row_bytes;
-        gate_row[k] = a.gate.rows_per == 1 ? row + kk : (row + kk) / a.gate.rows_per;
+        xs[k] = pipe.slot(stage, 0) + off + kk * (int)pipe.row_bytes;
+        rs[k] = pipe.slot(stage, 1) + off + kk * (int)pipe.row_bytes;
+        if (rows_per == 1) {
+          gate_row[k] = row + kk;
+        } else {
+          while (row + kk >= gate_end) ++gate_at, gate_end += rows_per;
+          gate_row[k] = gate_at;
+        }
       }
       float r1s[ROWS];
 #pragma unroll
       for (int k = 0; k < ROWS; ++k) r1s[k] = 1.0f;
+      Pack8<T> xr[ROWS];
+#pragma unroll
+      for (int k = 0; k < ROWS; ++k) xr[k] = smem8<T, VEC>(xs[k], 0, a.width, at);
       if (post != nullptr) {
         float2 s2[ROWS];
         float s[ROWS];
@@ -482,13 +500,9 @@ gated_norm_pipe_kernel(const NormArgs a, int threads_per_row, int stages) {
         for (int k = 0; k < ROWS; ++k) {
           s2[k] = splat(0.0f);
 #pragma unroll
-          for (int i = 0; i < ITERS; ++i) {
-            const Pack8<T> xr = smem8<T, VEC>(xs[k], i, a.width, at);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const float2 v = pair_of<T>(xr, j);
-              s2[k] = __ffma2_rn(v, v, s2[k]);
-            }
+          for (int j = 0; j < 4; ++j) {
+            const float2 v = pair_of<T>(xr[k], j);
+            s2[k] = __ffma2_rn(v, v, s2[k]);
           }
           s[k] = s2[k].x + s2[k].y;
         }
@@ -504,20 +518,19 @@ gated_norm_pipe_kernel(const NormArgs a, int threads_per_row, int stages) {
       for (int k = 0; k < ROWS; ++k) s2[k] = splat(0.0f);
 #pragma unroll
       for (int i = 0; i < ITERS; ++i) {
-        float2 g[4], w[4];
-        if (post != nullptr) param8<P, VEC>(post, i, a.width, at, w);
 #pragma unroll
         for (int k = 0; k < ROWS; ++k) {
-          if (k == 0 || gate_row[k] != gate_row[0]) gate8<P, VEC>(a.gate, gate_row[k], i, a.width, at, g);
-          const Pack8<T> xr = smem8<T, VEC>(xs[k], i, a.width, at), rr = smem8<T, VEC>(rs[k], i, a.width, at);
+          if (gate_row[k] != have_gate) gate8<P, VEC>(a.gate, gate_row[k], i, a.width, at, g);
+          have_gate = gate_row[k];
+          const Pack8<T> rr = smem8<T, VEC>(rs[k], i, a.width, at);
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            float2 z = pair_of<T>(xr, j);
-            if (post != nullptr) z = __fmul2_rn(__fmul2_rn(z, splat(r1s[k])), w[j]);
+            float2 z = pair_of<T>(xr[k], j);
+            if (post != nullptr) z = __fmul2_rn(__fmul2_rn(z, splat(r1s[k])), w_post[j]);
             h[k][i][j] = __ffma2_rn(g[j], z, __fmul2_rn(alpha, pair_of<T>(rr, j)));
             s2[k] = __ffma2_rn(h[k][i][j], h[k][i][j], s2[k]);
           }
-          if (ok && k < live) store8<T, VEC>(static_cast<T*>(a.h) + (row + k) * a.width, i, a.width, at, h[k][i]);
+          if (ok && k < live) store8<T, VEC>(static_cast<T*>(a.h) + (int64_t)(row + k) * a.width, i, a.width, at, h[k][i]);
         }
       }
       float s[ROWS], r2[ROWS], amax[ROWS];
@@ -532,24 +545,18 @@ gated_norm_pipe_kernel(const NormArgs a, int threads_per_row, int stages) {
       }
 #pragma unroll
       for (int i = 0; i < ITERS; ++i) {
-        float2 w[4], sm[4];
-        param8<P, VEC>(gamma, i, a.width, at, w);
-        if (QUANT && a.smooth != nullptr) {
-          if (a.smooth_f32) param8<float, VEC>(static_cast<const float*>(a.smooth), i, a.width, at, sm);
-          else param8<T, VEC>(static_cast<const T*>(a.smooth), i, a.width, at, sm);
-        }
 #pragma unroll
         for (int k = 0; k < ROWS; ++k) {
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            float2 y = __fmul2_rn(__fmul2_rn(h[k][i][j], splat(r2[k])), w[j]);
+            float2 y = __fmul2_rn(__fmul2_rn(h[k][i][j], splat(r2[k])), w_gamma[j]);
             if (QUANT) {
-              if (a.smooth != nullptr) y = __fmul2_rn(y, sm[j]);
+              if (a.smooth != nullptr) y = __fmul2_rn(y, w_smooth[j]);
               amax[k] = fmaxf(amax[k], fmaxf(fabsf(y.x), fabsf(y.y)));
             }
             h[k][i][j] = y;
           }
-          if (!QUANT && ok && k < live) store8<T, VEC>(static_cast<T*>(a.y) + (row + k) * a.width, i, a.width, at, h[k][i]);
+          if (!QUANT && ok && k < live) store8<T, VEC>(static_cast<T*>(a.y) + (int64_t)(row + k) * a.width, i, a.width, at, h[k][i]);
         }
       }
       if constexpr (QUANT) {
@@ -562,7 +569,7 @@ gated_norm_pipe_kernel(const NormArgs a, int threads_per_row, int stages) {
           const float inv = quant_inverse(scale);
 #pragma unroll
           for (int i = 0; i < ITERS; ++i)
-            store8_int8<VEC>(static_cast<int8_t*>(a.y) + (row + k) * a.width, i, a.width, at,
+            store8_int8<VEC>(static_cast<int8_t*>(a.y) + (int64_t)(row + k) * a.width, i, a.width, at,
                              inv == inv ? quantize8<false>(h[k][i], scale, inv) : quantize8<true>(h[k][i], scale, inv));
         }
       } else if (post == nullptr) {
@@ -604,27 +611,26 @@ struct NormGradArgs {
 constexpr int kNormGradThreads = 512;
 
 // The arithmetic of one row of the gradient for ITERS vectors of a thread; `load` gives operand q (0 x, 1 residual, 2 dy, 3 dh)
-// of vector i, `sums` keeps the sums over rows (0 gamma, 1 post gamma, 2 a shared gate).  Operands are read again for each of the
-// three passes, between which the two reductions lie.
-template <typename T, typename P, bool VEC, int ITERS, bool SUM_GATE, typename Load, typename Sums>
-__device__ __forceinline__ void norm_grad_row(const NormGradArgs& a, const Place& at, int64_t row, int64_t gate_row, float rs1, float rs2,
-                                              const Load& load, Sums& sums, float (*red0)[32], float (*red1)[32], int barrier, bool ok) {
-  const P* gamma = static_cast<const P*>(a.gamma);
-  const P* post = static_cast<const P*>(a.post);
+// of vector i, `params` gamma, post gamma and the row's gate, `sums` keeps the sums over rows (0 gamma, 1 post gamma, 2 a shared
+// gate).  Operands and parameters are asked for again in each of the three passes, between which the two reductions lie.
+template <typename T, typename P, bool VEC, int ITERS, bool SUM_GATE, typename Load, typename Params, typename Sums>
+__device__ __forceinline__ void norm_grad_row(const NormGradArgs& a, const Place& at, int64_t row, float rs1, float rs2, const Load& load,
+                                              const Params& params, Sums& sums, float (*red0)[32], float (*red1)[32], int barrier, bool ok) {
+  const bool post = a.post != nullptr;
   const float2 alpha = splat(a.alpha), s1 = splat(rs1), s2 = splat(rs2);
   float2 dot2 = splat(0.0f);
 #pragma unroll
   for (int i = 0; i < ITERS; ++i) {
     float2 g[4], w1[4], w2[4];
-    gate8<P, VEC>(a.gate, gate_row, i, a.width, at, g);
-    if (post != nullptr) param8<P, VEC>(post, i, a.width, at, w1);
-    param8<P, VEC>(gamma, i, a.width, at, w2);
+    params.gate(i, g);
+    if (post) params.post(i, w1);
+    params.gamma(i, w2);
     const Pack8<T> xr = load(0, i), rr = load(1, i), yr = load(2, i);
     float2(&acc)[4] = sums.open(0, i);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       float2 z = pair_of<T>(xr, j);
-      if (post != nullptr) z = __fmul2_rn(__fmul2_rn(z, s1), w1[j]);
+      if (post) z = __fmul2_rn(__fmul2_rn(z, s1), w1[j]);
       const float2 hn = __fmul2_rn(__ffma2_rn(g[j], z, __fmul2_rn(alpha, pair_of<T>(rr, j))), s2);
       const float2 d = __fmul2_rn(pair_of<T>(yr, j), hn);
       dot2 = __ffma2_rn(d, w2[j], dot2);
@@ -640,9 +646,9 @@ __device__ __forceinline__ void norm_grad_row(const NormGradArgs& a, const Place
 #pragma unroll
   for (int i = 0; i < ITERS; ++i) {
     float2 g[4], w1[4], w2[4], out[4], dg[4];
-    gate8<P, VEC>(a.gate, gate_row, i, a.width, at, g);
-    if (post != nullptr) param8<P, VEC>(post, i, a.width, at, w1);
-    param8<P, VEC>(gamma, i, a.width, at, w2);
+    params.gate(i, g);
+    if (post) params.post(i, w1);
+    params.gamma(i, w2);
     const Pack8<T> xr = load(0, i), rr = load(1, i), yr = load(2, i);
     Pack8<T> hr;
     if (a.dh != nullptr) hr = load(3, i);
@@ -651,7 +657,7 @@ __device__ __forceinline__ void norm_grad_row(const NormGradArgs& a, const Place
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const float2 xn = __fmul2_rn(pair_of<T>(xr, j), s1);
-      const float2 z = post != nullptr ? __fmul2_rn(xn, w1[j]) : xn;   // without post gamma s1 is 1
+      const float2 z = post ? __fmul2_rn(xn, w1[j]) : xn;   // without post gamma s1 is 1
       const float2 hn = __fmul2_rn(__ffma2_rn(g[j], z, __fmul2_rn(alpha, pair_of<T>(rr, j))), s2);
       float2 dh = __fmul2_rn(s2, __ffma2_rn(hn, nc2, __fmul2_rn(pair_of<T>(yr, j), w2[j])));
       if (a.dh != nullptr) dh = __fadd2_rn(dh, pair_of<T>(hr, j));
@@ -663,7 +669,7 @@ __device__ __forceinline__ void norm_grad_row(const NormGradArgs& a, const Place
         dots_g = __fadd2_rn(dots_g, dg[j]);
       }
       float2 dz = __fmul2_rn(dh, g[j]);
-      if (post != nullptr) {
+      if (post) {
         const float2 t = __fmul2_rn(dz, xn);
         acc1[j] = __fadd2_rn(acc1[j], t);
         dots_v = __ffma2_rn(t, w1[j], dots_v);
@@ -671,7 +677,7 @@ __device__ __forceinline__ void norm_grad_row(const NormGradArgs& a, const Place
       }
       keep[i][j] = dz;
     }
-    if (post != nullptr) sums.close(1, i);
+    if (post) sums.close(1, i);
     if (SUM_GATE) sums.close(2, i);
     if (ok) {
       store8<T, VEC>(static_cast<T*>(a.dres) + row * a.width, i, a.width, at, out);
@@ -692,7 +698,7 @@ __device__ __forceinline__ void norm_grad_row(const NormGradArgs& a, const Place
   if (!SUM_GATE && a.dgate != nullptr && a.gate.per_row && at.tid == 0) static_cast<P*>(a.dgate)[row] = narrow<P>(dots[1]);
 #pragma unroll
   for (int i = 0; i < ITERS; ++i) {
-    if (post != nullptr) {
+    if (post) {
       const Pack8<T> xr = load(0, i);
 #pragma unroll
       for (int j = 0; j < 4; ++j) keep[i][j] = __fmul2_rn(s1, __ffma2_rn(__fmul2_rn(pair_of<T>(xr, j), s1), nc1, keep[i][j]));
@@ -700,6 +706,27 @@ __device__ __forceinline__ void norm_grad_row(const NormGradArgs& a, const Place
     store8<T, VEC>(static_cast<T*>(a.dx) + row * a.width, i, a.width, at, keep[i]);
   }
 }
+
+// Parameters read where they are wanted (from L1), and parameters that stay in registers.
+template <typename P, bool VEC>
+struct GlobalParams {
+  const NormGradArgs& a;
+  const Place& at;
+  int64_t gate_row;
+  __device__ __forceinline__ void gate(int i, float2 (&f)[4]) const { gate8<P, VEC>(a.gate, gate_row, i, a.width, at, f); }
+  __device__ __forceinline__ void post(int i, float2 (&f)[4]) const { param8<P, VEC>(static_cast<const P*>(a.post), i, a.width, at, f); }
+  __device__ __forceinline__ void gamma(int i, float2 (&f)[4]) const { param8<P, VEC>(static_cast<const P*>(a.gamma), i, a.width, at, f); }
+};
+struct RegisterParams {
+  float2 g[4], w1[4], w2[4];
+  static __device__ __forceinline__ void copy(const float2 (&from)[4], float2 (&f)[4]) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) f[j] = from[j];
+  }
+  __device__ __forceinline__ void gate(int, float2 (&f)[4]) const { copy(g, f); }
+  __device__ __forceinline__ void post(int, float2 (&f)[4]) const { copy(w1, f); }
+  __device__ __forceinline__ void gamma(int, float2 (&f)[4]) const { copy(w2, f); }
+};
 
 // Sums over rows in registers.
 template <int ITERS>
@@ -801,8 +828,9 @@ gated_norm_grad_kernel(const NormGradArgs a, int threads_per_row) {
         if constexpr (KEEP) return kept[q][i];
         else return fetch(q, i);
       };
-      norm_grad_row<T, P, VEC, ITERS, SUM_GATE>(a, at, row, SUM_GATE ? gate : row, a.post != nullptr ? a.post_rstd[row] : 1.0f, a.rstd[row], load,
-                                                sums, red[0][group], red[1][group], 1 + group, true);
+      const GlobalParams<P, VEC> params{a, at, SUM_GATE ? gate : row};
+      norm_grad_row<T, P, VEC, ITERS, SUM_GATE>(a, at, row, a.post != nullptr ? a.post_rstd[row] : 1.0f, a.rstd[row], load, params, sums,
+                                                red[0][group], red[1][group], 1 + group, true);
     }
     if (SUM_GATE) {
       flush(2, a.part_gate + (blockIdx.x + gate) * a.width);
@@ -826,19 +854,25 @@ gated_norm_grad_pipe_kernel(const NormGradArgs a, int threads_per_row, int stage
   const int readers = blockDim.x, groups = readers / threads_per_row;
   const RowPipe pipe = row_pipe_init(pipe_smem, stages, 4, groups, (int64_t)a.width * sizeof(T), a.rows, readers / 32);
   float* joined = reinterpret_cast<float*>(pipe.slot(stages, 0));   // [width] behind the ring
-  const int64_t r0 = a.rows * blockIdx.x / gridDim.x, r1 = a.rows * (blockIdx.x + 1) / gridDim.x;
-  // Chunks do not cross the end of a gate's rows.
-  auto chunk_end = [&](int64_t row) {
-    int64_t end = min(row + groups, r1);
-    if (SUM_GATE) end = min(end, (row / a.gate.rows_per + 1) * a.gate.rows_per);
+  const int r0 = (int)(a.rows * blockIdx.x / gridDim.x), r1 = (int)(a.rows * (blockIdx.x + 1) / gridDim.x);   // fewer than 2^30 rows
+  // Chunks do not cross the end of a gate's rows, which the feed and the rows walk along (a division for every chunk cost more).
+  const int rows_per = (int)min(a.gate.rows_per, a.rows);
+  const int gate0 = SUM_GATE ? r0 / rows_per : 0, gate0_end = SUM_GATE ? (gate0 + 1) * rows_per : 0;
+  auto chunk_end = [&](int row, int& gate_end) {
+    int end = min(row + groups, r1);
+    if (SUM_GATE) {
+      if (row == gate_end) gate_end += rows_per;
+      end = min(end, gate_end);
+    }
     return end;
   };
   const void* const src[4] = {a.x, a.residual, a.dy, a.dh};
   RowPipeFeed feed{r0, 0, 0, true};
+  int feed_gate_end = gate0_end;
   auto fill = [&]() {                                      // by the first warp
     if (feed.row >= r1 || !feed.ok) return;
-    const int64_t end = chunk_end(feed.row);
-    feed.ok = row_pipe_fill(pipe, src, feed.stage, feed.phase, feed.row, (int)(end - feed.row), threadIdx.x & 31);
+    const int end = chunk_end(feed.row, feed_gate_end);
+    feed.ok = row_pipe_fill(pipe, src, feed.stage, feed.phase, feed.row, end - feed.row, threadIdx.x & 31);
     feed.next(end, stages);
   };
   if (threadIdx.x < 32)
@@ -874,34 +908,50 @@ gated_norm_grad_pipe_kernel(const NormGradArgs a, int threads_per_row, int stage
     };
     // The statistics of this group's next row are loaded a chunk ahead.
     float next1 = 1.0f, next2 = 0.0f;
-    auto look = [&](int64_t chunk) {
-      if (chunk < r1 && chunk + group < chunk_end(chunk)) {
+    auto look = [&](int chunk, int end) {
+      if (chunk + group < end) {
         next2 = a.rstd[chunk + group];
         if (a.post != nullptr) next1 = a.post_rstd[chunk + group];
       }
     };
-    look(r0);
+    int gate = gate0, gate_end = gate0_end, end = r0 < r1 ? chunk_end(r0, gate_end) : r0;
+    look(r0, end);
+    // A thread's columns stay the same: so do its parameters, but for the gate.
+    RegisterParams params;
+    if (a.post != nullptr) param8<P, VEC>(static_cast<const P*>(a.post), 0, a.width, at, params.w1);
+    param8<P, VEC>(static_cast<const P*>(a.gamma), 0, a.width, at, params.w2);
+    int have_gate = -1;
     bool ok = true;
-    for (int64_t chunk = r0; chunk < r1;) {
-      const int64_t end = chunk_end(chunk), row = chunk + group;
+    for (int chunk = r0; chunk < r1;) {
+      const int row = chunk + group;
       const float rs1 = next1, rs2 = next2;
-      look(end);
+      const bool last_of_gate = SUM_GATE && (end == r1 || end == gate_end);
+      const int next_end = end < r1 ? chunk_end(end, gate_end) : end;
+      look(end, next_end);
       ok = mbar_wait(&pipe.full[stage], phase, pipe.abort_flag, kDevTimeoutEpilogue) && ok;
       if (threadIdx.x < 32 && chunk > r0) fill();
-      const int64_t gate = SUM_GATE ? chunk / a.gate.rows_per : row;
+      const int row_gate = SUM_GATE ? gate : row;
       if (row < end) {                                     // the same for all threads of the row
-        const int64_t off = chunk * pipe.row_bytes - ((chunk * pipe.row_bytes) & ~int64_t(15)) + group * pipe.row_bytes;
-        auto load = [&](int q, int i) { return smem8<T, VEC>(pipe.slot(stage, q) + off, i, a.width, at); };
-        norm_grad_row<T, P, VEC, ITERS, SUM_GATE>(a, at, row, gate, rs1, rs2, load, sums, red[0][group], red[1][group], 1 + group, ok);
+        const int off = (int)((chunk * pipe.row_bytes) & 15) + group * (int)pipe.row_bytes;
+        Pack8<T> kept[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          if (q < 3 || a.dh != nullptr) kept[q] = smem8<T, VEC>(pipe.slot(stage, q) + off, 0, a.width, at);
+        auto load = [&](int q, int) { return kept[q]; };
+        if (row_gate != have_gate) gate8<P, VEC>(a.gate, row_gate, 0, a.width, at, params.g);
+        have_gate = row_gate;
+        norm_grad_row<T, P, VEC, ITERS, SUM_GATE>(a, at, row, rs1, rs2, load, params, sums, red[0][group], red[1][group], 1 + group, ok);
       }
       __syncwarp();
       if ((threadIdx.x & 31) == 0) mbar_arrive(&pipe.empty[stage]);
       if (++stage == stages) { stage = 0; phase ^= 1; }
-      if (SUM_GATE && (end == r1 || end / a.gate.rows_per != gate)) {
-        flush(2, a.part_gate + (blockIdx.x + gate) * a.width);
+      if (last_of_gate) {
+        flush(2, a.part_gate + (int64_t)(blockIdx.x + gate) * a.width);
         sums.clear(2);
+        ++gate;
       }
       chunk = end;
+      end = next_end;
     }
     flush(0, a.part_gamma + (int64_t)blockIdx.x * a.width);
     if (a.post != nullptr) flush(1, a.part_post + (int64_t)blockIdx.x * a.width);
@@ -985,8 +1035,10 @@ struct RowPipePlan {
   int threads, groups, stages, smem;
   bool fits;
 };
-inline RowPipePlan row_pipe_plan(int64_t width, int element, int arrays, int rows, int64_t rows_per_cta, int extra) {
+inline RowPipePlan row_pipe_plan(int64_t width, int element, int arrays, int rows, int64_t all_rows, int64_t ctas, int extra) {
   RowPipePlan p{};
+  if (all_rows >= (1LL << 30)) return p;                   // rows are counted in 32 bits
+  const int64_t rows_per_cta = ceil_div(all_rows, ctas);
   p.threads = (int)ceil_div(ceil_div(width, 8), 32) * 32;
   if (p.threads > kRowPipeThreads) return p;
   p.groups = kRowPipeThreads / p.threads;
@@ -1008,7 +1060,7 @@ int launch_norm(const NormArgs& a, cudaStream_t st) {
   const bool many = a.rows > 2 * sm_count();
   if constexpr (!VEC) {
     const int64_t ctas = a.rows < sm_count() ? a.rows : sm_count();
-    const RowPipePlan p = row_pipe_plan(a.width, sizeof(T), 2, 2, ceil_div(a.rows, ctas), 0);
+    const RowPipePlan p = row_pipe_plan(a.width, sizeof(T), 2, 2, a.rows, ctas, 0);
     if (many && p.fits && aligned(a.x, 16) && aligned(a.residual, 16)) {
       constexpr auto kern = gated_norm_pipe_kernel<T, P, QUANT>;
       if (int rc = ensure_dynamic_smem<kern>(kRowPipeSmem, "gated_add_rms_norm")) return rc;
@@ -1080,7 +1132,7 @@ int launch_norm_grad(const NormGradArgs& a, NormSumArgs s, bool sum_gate, cudaSt
     }
   } else {
     s.ctas = grad_ctas(a.rows, 1);
-    const RowPipePlan p = row_pipe_plan(a.width, sizeof(T), 4, 1, ceil_div(a.rows, s.ctas), (int)((a.width * 4 + 15) & ~15));
+    const RowPipePlan p = row_pipe_plan(a.width, sizeof(T), 4, 1, a.rows, s.ctas, (int)((a.width * 4 + 15) & ~15));
     if (p.fits && aligned(a.x, 16) && aligned(a.residual, 16) && aligned(a.dy, 16) && aligned(a.dh, 16)) {
 #define B200Q_NORM_GRAD_PIPE(SUM)                                                                                        \
   {                                                                                                                      \
