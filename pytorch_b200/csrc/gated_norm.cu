@@ -1053,15 +1053,18 @@ inline RowPipePlan row_pipe_plan(int64_t width, int element, int arrays, int row
 }
 
 // Full vectors: a handful of rows (no more than two an SM) get as many threads a row as it has vectors, for the shortest way
-// through a row; more rows 256 threads (512 above 8192 columns) with two or four vectors each, four CTAs an SM.  Rows that are not
-// made of full vectors go through shared memory, up to 4096 columns and from a 16-byte boundary on.
+// through a row; more rows 256 threads (512 above 8192 columns) with two or four vectors each, four CTAs an SM (4096 bf16 columns,
+// one vector a thread against two: 16 rows 6.1 / 8.2 us, 296 8.2 / 10.2, 600 10.2 / 10.2, 4096 32.8 / 30.7).  Many rows that are not
+// made of full vectors go through shared memory from a few hundred columns up to 4096 and from a 16-byte boundary on (f16, straight
+// from global memory against through shared memory: 600 rows of 1111 8.2 / 10.2 us, 6124 32.8 / 30.7, 3000 of 4000 51.2 / 45.1;
+// 6124 of 264 16.4 / 16.4, 20000 of 96 18.4 / 20.5).
 template <typename T, typename P, bool VEC, bool QUANT>
 int launch_norm(const NormArgs& a, cudaStream_t st) {
   const bool many = a.rows > 2 * sm_count();
   if constexpr (!VEC) {
     const int64_t ctas = a.rows < sm_count() ? a.rows : sm_count();
     const RowPipePlan p = row_pipe_plan(a.width, sizeof(T), 2, 2, a.rows, ctas, 0);
-    if (many && p.fits && aligned(a.x, 16) && aligned(a.residual, 16)) {
+    if (a.rows > 8 * sm_count() && a.width >= 512 && p.fits && aligned(a.x, 16) && aligned(a.residual, 16)) {
       constexpr auto kern = gated_norm_pipe_kernel<T, P, QUANT>;
       if (int rc = ensure_dynamic_smem<kern>(kRowPipeSmem, "gated_add_rms_norm")) return rc;
       kern<<<(unsigned)ctas, p.groups * p.threads, p.smem, st>>>(a, p.threads, p.stages);
@@ -1096,8 +1099,9 @@ inline int grad_ctas(int64_t rows, int per_sm) {
 
 // Full vectors: CTAs of 256 threads, two an SM, with two vectors a thread and row up to 4096 columns (measured for 8192 rows of 4096
 // bf16: 124 us with the row's operands in registers, 130 read again from L1, 151 from L2; three CTAs an SM at 80 registers
-// 147, rows through shared memory with the sums in registers 176 to 203); 512 threads with two (up to 8192) or four vectors above.  Else through shared memory, up to 4096 columns and from a
-// 16-byte boundary on.
+// 147, rows through shared memory with the sums in registers 176 to 203); 512 threads with two (up to 8192) or four vectors above.
+// Else through shared memory, up to 4096 columns and from a 16-byte boundary on (f16, read three times from global memory against
+// that: 100 rows of 1111 65 / 16 us, 6124 309 / 59, 3000 of 4000 342 / 84, 20000 of 96 364 / 47), and straight for what is left.
 template <typename T, typename P, bool VEC>
 int launch_norm_grad(const NormGradArgs& a, NormSumArgs s, bool sum_gate, cudaStream_t st) {
 #define B200Q_NORM_GRAD(I, MAX, MIN, SUM)                                                                                \

@@ -25,7 +25,10 @@ namespace b200q {
 namespace {
 
 constexpr int kMaxExperts = 1024;
-constexpr int kDirectIds = 2048;          // assignments up to which every CTA counts for itself
+// Assignments up to which every CTA counts for itself instead of a sort in front.  With 4096 columns and 64 experts, one launch
+// against two: copied 128 rows 8.2 / 10.2 us, 1024 10.2 / 12.3, 4096 18.4 / 18.4; quantised 128 6.1 / 12.3, 2048 16.4 / 18.4,
+// 4096 34.8 / 22.5.
+constexpr int kDirectIds = 2048;
 constexpr int kKeyShift = 12;             // (expert, assignment) in one word on that path: 1025 keys x 4096 places
 static_assert(kDirectIds <= (1 << kKeyShift), "an assignment's number fits below the expert");
 constexpr int kNoExpert = -1;
@@ -48,8 +51,10 @@ __device__ __forceinline__ int expert_of(const IdT* __restrict__ ids, int64_t i,
 constexpr int kSortThreads = 1024;
 constexpr int kSortWarps = kSortThreads / 32;
 constexpr int kSortBatch = 8;             // index loads in flight per lane
+constexpr int kExpertBits = 11;           // hold the numbers 0 .. kMaxExperts (fewer ballots for fewer experts gained nothing: 18.4 us with 6 and 11)
+static_assert(kMaxExperts < (1 << kExpertBits), "an expert's number and the one for none");
 
-template <typename IdT, int BITS>           // BITS hold the numbers 0 .. experts
+template <typename IdT>
 __global__ void __launch_bounds__(kSortThreads, 1)
 moe_sort_kernel(const IdT* __restrict__ ids, int64_t n, int64_t begin, int experts, int strict_limit,
                 int32_t* __restrict__ row_idx, int32_t* __restrict__ row_src, int64_t* __restrict__ expert_tokens,
@@ -157,7 +162,7 @@ moe_sort_kernel(const IdT* __restrict__ ids, int64_t n, int64_t begin, int exper
       const int key = e[b] < 0 ? experts : e[b];
       unsigned same = 0xffffffffu;
 #pragma unroll
-      for (int q = 0; q < BITS; ++q) {
+      for (int q = 0; q < kExpertBits; ++q) {
         const bool one = (key >> q) & 1;
         const unsigned ballot = __ballot_sync(0xffffffffu, one);
         same &= one ? ballot : ~ballot;
@@ -898,14 +903,15 @@ inline int element_bytes(int dtype) {
   }
 }
 
-// Launches the sort: one cluster of a CTA for every 2048 indices, up to sixteen (the ballots of pass 2 keep an SM's
-// schedulers busy for about 4 us per 4096 indices, the cluster's barriers cost less).
+// Launches the sort: one cluster of a CTA for every 2048 indices, up to sixteen (sort and a copy of 16-byte rows with 1 / 4 / 16
+// CTAs: 8192 indices of 64 experts 18.4 / 12.3 / 12.3 us, 32768 51.2 / 20.4 / 14.3, 65536 94.2 / 36.9 / 18.4, of 1000 experts
+// 108.5 / 38.9 / 22.5).
 constexpr int kSortClusterMax = 16;
 
-template <typename IdT, int BITS>
-int launch_sort_bits(const RouteIds& r, int32_t* row_idx, int32_t* row_src, int64_t* expert_tokens, int cumulative, int32_t* valid_rows,
+template <typename IdT>
+int launch_sort(const RouteIds& r, int32_t* row_idx, int32_t* row_src, int64_t* expert_tokens, int cumulative, int32_t* valid_rows,
                      int2* row_info, cudaStream_t st) {
-  constexpr auto kern = moe_sort_kernel<IdT, BITS>;
+  constexpr auto kern = moe_sort_kernel<IdT>;
   const int smem = (kSortWarps + 1) * r.experts * (int)sizeof(int);
   if (int rc = ensure_dynamic_smem<kern>((kSortWarps + 1) * kMaxExperts * (int)sizeof(int), "moe_route (sort)")) return rc;
   if (int rc = ensure_wide_clusters<kern>("moe_route (sort)")) return rc;
@@ -927,14 +933,6 @@ int launch_sort_bits(const RouteIds& r, int32_t* row_idx, int32_t* row_src, int6
                                        row_idx, row_src, expert_tokens, cumulative, valid_rows, row_info, r.topk);
   if (err != cudaSuccess) return fail(B200Q_ERR_LAUNCH, "moe_route (sort): %s", cudaGetErrorString(err));
   return check_launch("moe_route (sort)");
-}
-
-template <typename IdT>
-int launch_sort(const RouteIds& r, int32_t* row_idx, int32_t* row_src, int64_t* expert_tokens, int cumulative, int32_t* valid_rows,
-                int2* row_info, cudaStream_t st) {
-  if (r.experts < 64) return launch_sort_bits<IdT, 6>(r, row_idx, row_src, expert_tokens, cumulative, valid_rows, row_info, st);
-  if (r.experts < 256) return launch_sort_bits<IdT, 8>(r, row_idx, row_src, expert_tokens, cumulative, valid_rows, row_info, st);
-  return launch_sort_bits<IdT, 11>(r, row_idx, row_src, expert_tokens, cumulative, valid_rows, row_info, st);
 }
 
 template <typename IdT, int BYTES>
@@ -959,46 +957,46 @@ int launch_copy(const b200q_moe_route_args& a, const RouteIds& r, int64_t row_by
 }
 
 template <typename IdT, typename T, typename ST, int ITERS>
-int launch_route_quant_iters(const b200q_moe_route_args& a, const RouteIds& r, int threads, int2* row_info, int32_t* valid_rows, cudaStream_t st) {
-  const T* x = static_cast<const T*>(a.x);
-  const ST* sm = static_cast<const ST*>(a.scale);
-  int8_t* out = static_cast<int8_t*>(a.out);
-  if (r.n <= kDirectIds) {
-    moe_quant_direct_kernel<IdT, T, ST, ITERS><<<(unsigned)(r.n + 1), threads, 0, st>>>(r, x, a.hidden, sm, (int)a.scale_rows, out, a.out_scale,
-                                                                                        a.row_idx, a.row_src, a.expert_tokens, a.cumulative);
-    return check_launch("moe_route (quantised, few tokens)");
-  }
-  if (int rc = launch_sort<IdT>(r, a.row_idx, a.row_src, a.expert_tokens, a.cumulative, valid_rows, row_info, st)) return rc;
-#define B200Q_ROUTE_QUANT(FULL)                                                                                                        \
-  {                                                                                                                                    \
-    constexpr auto kern = moe_quant_kernel<T, ST, ITERS, FULL>;                                                                        \
-    const int64_t cap = (int64_t)sm_count() * resident_ctas<kern>(threads);                                                            \
-    return launch_dependent(kern, (unsigned)(r.n < cap ? r.n : cap), threads, st, "moe_route (quantised)", r.n, x, a.hidden, sm,       \
-                            (int)a.scale_rows, out, a.out_scale, static_cast<const int2*>(row_info),                                   \
-                            static_cast<const int32_t*>(valid_rows));                                                                  \
-  }
-  if constexpr (ITERS > 0) {
-    if (a.hidden == (int64_t)threads * ITERS * 8) B200Q_ROUTE_QUANT(true)
-  }
-  B200Q_ROUTE_QUANT(false)
-#undef B200Q_ROUTE_QUANT
+int launch_route_quant_direct(const b200q_moe_route_args& a, const RouteIds& r, int threads, cudaStream_t st) {
+  moe_quant_direct_kernel<IdT, T, ST, ITERS><<<(unsigned)(r.n + 1), threads, 0, st>>>(
+      r, static_cast<const T*>(a.x), a.hidden, static_cast<const ST*>(a.scale), (int)a.scale_rows, static_cast<int8_t*>(a.out), a.out_scale, a.row_idx,
+      a.row_src, a.expert_tokens, a.cumulative);
+  return check_launch("moe_route (quantised, few tokens)");
+}
+
+template <typename T, typename ST, int ITERS, bool FULL>
+int launch_route_quant_sorted(const b200q_moe_route_args& a, int64_t n, int threads, const int2* row_info, const int32_t* valid_rows, cudaStream_t st) {
+  constexpr auto kern = moe_quant_kernel<T, ST, ITERS, FULL>;
+  const int64_t cap = (int64_t)sm_count() * resident_ctas<kern>(threads);
+  return launch_dependent(kern, (unsigned)(n < cap ? n : cap), threads, st, "moe_route (quantised)", n, static_cast<const T*>(a.x), a.hidden,
+                          static_cast<const ST*>(a.scale), (int)a.scale_rows, static_cast<int8_t*>(a.out), a.out_scale, row_info, valid_rows);
 }
 
 template <typename IdT, typename T, typename ST>
 int launch_route_quant(const b200q_moe_route_args& a, const RouteIds& r, int2* row_info, int32_t* valid_rows, cudaStream_t st) {
   const bool vec = a.hidden % 8 == 0 && a.hidden > 0 && a.hidden <= 8 * 512 * 4 && aligned(a.x, 16) && aligned(a.out, 8) &&
                    (a.scale == nullptr || aligned(a.scale, 16));
-  if (!vec) return launch_route_quant_iters<IdT, T, ST, 0>(a, r, 256, row_info, valid_rows, st);
-  // Two vectors a thread up to 8192 columns: with four, the row, the next row and the smooth scales take so many registers that half
-  // as many warps fit on an SM.
-  const int nvec = (int)(a.hidden / 8);
-  const int iters = nvec <= 128 ? 1 : nvec <= 1024 ? 2 : 4;
-  const int threads = (int)ceil_div(ceil_div(nvec, iters), 32) * 32;
-  switch (iters) {
-    case 1: return launch_route_quant_iters<IdT, T, ST, 1>(a, r, threads, row_info, valid_rows, st);
-    case 2: return launch_route_quant_iters<IdT, T, ST, 2>(a, r, threads, row_info, valid_rows, st);
-    default: return launch_route_quant_iters<IdT, T, ST, 4>(a, r, threads, row_info, valid_rows, st);
+  const int nvec = vec ? (int)(a.hidden / 8) : 0;
+  auto threads_for = [&](int iters) { return (int)ceil_div(ceil_div(nvec, iters), 32) * 32; };
+  if (r.n <= kDirectIds) {
+    // Latency counts: few vectors a thread.
+    if (!vec) return launch_route_quant_direct<IdT, T, ST, 0>(a, r, 256, st);
+    if (nvec <= 128) return launch_route_quant_direct<IdT, T, ST, 1>(a, r, threads_for(1), st);
+    if (nvec <= 1024) return launch_route_quant_direct<IdT, T, ST, 2>(a, r, threads_for(2), st);
+    return launch_route_quant_direct<IdT, T, ST, 4>(a, r, threads_for(4), st);
   }
+  if (int rc = launch_sort<IdT>(r, a.row_idx, a.row_src, a.expert_tokens, a.cumulative, valid_rows, row_info, st)) return rc;
+  // What a row costs besides its vectors (the maximum's way through the warps, the scale) is shared by fewer warps with four vectors
+  // a thread.  4096 tokens to six rows each, with 1 / 2 / 4: 512 columns 24.6 / 22.5 / 24.6 us, 1024 34.8 / 28.7 / 26.6, 2048 55.3 /
+  // 41.0 / 38.9, 4096 102.4 / 69.6 / 63.5, 8192 - / 139.2 / 133.1.
+  if (!vec) return launch_route_quant_sorted<T, ST, 0, false>(a, r.n, 256, row_info, valid_rows, st);
+  const int iters = nvec < 128 ? 2 : 4, threads = threads_for(iters);
+  const bool full = nvec == threads * iters;
+  if (iters == 2)
+    return full ? launch_route_quant_sorted<T, ST, 2, true>(a, r.n, threads, row_info, valid_rows, st)
+                : launch_route_quant_sorted<T, ST, 2, false>(a, r.n, threads, row_info, valid_rows, st);
+  return full ? launch_route_quant_sorted<T, ST, 4, true>(a, r.n, threads, row_info, valid_rows, st)
+              : launch_route_quant_sorted<T, ST, 4, false>(a, r.n, threads, row_info, valid_rows, st);
 }
 
 template <typename IdT>
@@ -1043,9 +1041,12 @@ int launch_combine(const void* rows, int64_t num_rows, const int32_t* row_idx, c
   return check_launch("moe_combine");
 }
 
-// The pipeline pays from a few tokens a CTA on and for rows of at least a stage's length; up to eight slots.
+// The pipeline pays from one token a CTA on and for rows that fill a quarter of a stage; it has up to eight slots.  A thread a
+// vector against the pipeline, eight bf16 rows a token, forward and gradient: 148 tokens of 4096 columns 8.2 / 8.2 and 18.4 /
+// 16.4 us, 300 14.3 / 12.3 and 24.6 / 20.5, 2048 57.3 / 32.8 and 79.9 / 59.4, 8192 190.5 / 108.5 and 278.5 / 200.7; 8192 tokens
+// of 256 columns 20.5 / 24.6 and 43.0 / 55.3, of 512 32.7 / 28.7 and 63.5 / 59.4.
 inline bool use_gather(int64_t tokens, int64_t topk, int64_t row_bytes) {
-  return topk <= 8 && tokens >= 4 * sm_count() && row_bytes >= 1024;
+  return topk <= 8 && tokens >= 2 * sm_count() && row_bytes >= 1024;
 }
 
 template <typename T, int KC, bool GRAD>
