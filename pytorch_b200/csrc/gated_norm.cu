@@ -158,6 +158,27 @@ __device__ __forceinline__ void row_sum(float (&v)[N], float (*red)[32], const P
   }
 }
 
+// The same for up to 16 warps, with one round of 16-byte loads in place of the second round of shuffles; `red` holds zeros behind the
+// row's warps.
+template <int N>
+__device__ __forceinline__ void row_sum16(float (&v)[N], float (*red)[32], const Place& at, int barrier) {
+#pragma unroll
+  for (int k = 0; k < N; ++k)
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v[k] += __shfl_xor_sync(0xffffffffu, v[k], o);
+  if (at.threads == 32) return;
+#pragma unroll
+  for (int k = 0; k < N; ++k)
+    if ((at.tid & 31) == 0) red[k][at.tid >> 5] = v[k];
+  named_barrier_sync(barrier, at.threads);
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    const float4* p = reinterpret_cast<const float4*>(red[k]);
+    const float4 a = p[0], b = p[1], c = p[2], d = p[3];
+    v[k] = (((a.x + a.y) + (a.z + a.w)) + ((b.x + b.y) + (b.z + b.w))) + (((c.x + c.y) + (c.z + c.w)) + ((d.x + d.y) + (d.z + d.w)));
+  }
+}
+
 // Maxima of N non-negative values over the threads of a row.
 template <int N>
 __device__ __forceinline__ void row_max(float (&v)[N], float (*red)[32], const Place& at, int barrier) {
@@ -610,7 +631,7 @@ struct NormGradArgs {
 
 constexpr int kNormGradThreads = 512;
 
-// The arithmetic of one row of the gradient for ITERS vectors of a thread; `load` gives operand q (0 x, 1 residual, 2 dy, 3 dh)
+// The arithmetic of one row of the gradient for ITERS vectors of a thread (with one, hn stays in registers between the passes); `load` gives operand q (0 x, 1 residual, 2 dy, 3 dh)
 // of vector i, `params` gamma, post gamma and the row's gate, `sums` keeps the sums over rows (0 gamma, 1 post gamma, 2 a shared
 // gate).  Operands and parameters are asked for again in each of the three passes, between which the two reductions lie.
 template <typename T, typename P, bool VEC, int ITERS, bool SUM_GATE, typename Load, typename Params, typename Sums>
@@ -618,6 +639,8 @@ __device__ __forceinline__ void norm_grad_row(const NormGradArgs& a, const Place
                                               const Params& params, Sums& sums, float (*red0)[32], float (*red1)[32], int barrier, bool ok) {
   const bool post = a.post != nullptr;
   const float2 alpha = splat(a.alpha), s1 = splat(rs1), s2 = splat(rs2);
+  constexpr bool KEEP_HN = ITERS == 1;
+  float2 hn_kept[KEEP_HN ? 4 : 1];
   float2 dot2 = splat(0.0f);
 #pragma unroll
   for (int i = 0; i < ITERS; ++i) {
@@ -632,6 +655,7 @@ __device__ __forceinline__ void norm_grad_row(const NormGradArgs& a, const Place
       float2 z = pair_of<T>(xr, j);
       if (post) z = __fmul2_rn(__fmul2_rn(z, s1), w1[j]);
       const float2 hn = __fmul2_rn(__ffma2_rn(g[j], z, __fmul2_rn(alpha, pair_of<T>(rr, j))), s2);
+      if constexpr (KEEP_HN) hn_kept[j] = hn;
       const float2 d = __fmul2_rn(pair_of<T>(yr, j), hn);
       dot2 = __ffma2_rn(d, w2[j], dot2);
       acc[j] = __fadd2_rn(acc[j], d);
@@ -639,7 +663,7 @@ __device__ __forceinline__ void norm_grad_row(const NormGradArgs& a, const Place
     sums.close(0, i);
   }
   float dot[1] = {dot2.x + dot2.y};
-  row_sum<1>(dot, red0, at, barrier);
+  row_sum16<1>(dot, red0, at, barrier);
   const float2 nc2 = splat(-dot[0] * a.inv_width);
   float2 dots_v = splat(0.0f), dots_g = splat(0.0f);       // v . xn, dh . z
   float2 keep[ITERS][4];                                   // v
@@ -658,7 +682,7 @@ __device__ __forceinline__ void norm_grad_row(const NormGradArgs& a, const Place
     for (int j = 0; j < 4; ++j) {
       const float2 xn = __fmul2_rn(pair_of<T>(xr, j), s1);
       const float2 z = post ? __fmul2_rn(xn, w1[j]) : xn;   // without post gamma s1 is 1
-      const float2 hn = __fmul2_rn(__ffma2_rn(g[j], z, __fmul2_rn(alpha, pair_of<T>(rr, j))), s2);
+      const float2 hn = KEEP_HN ? hn_kept[KEEP_HN ? j : 0] : __fmul2_rn(__ffma2_rn(g[j], z, __fmul2_rn(alpha, pair_of<T>(rr, j))), s2);
       float2 dh = __fmul2_rn(s2, __ffma2_rn(hn, nc2, __fmul2_rn(pair_of<T>(yr, j), w2[j])));
       if (a.dh != nullptr) dh = __fadd2_rn(dh, pair_of<T>(hr, j));
       out[j] = __fmul2_rn(alpha, dh);
@@ -688,10 +712,10 @@ __device__ __forceinline__ void norm_grad_row(const NormGradArgs& a, const Place
   float dots[2] = {dots_v.x + dots_v.y, dots_g.x + dots_g.y};
   if constexpr (SUM_GATE) {
     float only[1] = {dots[0]};
-    row_sum<1>(only, red1, at, barrier);
+    row_sum16<1>(only, red1, at, barrier);
     dots[0] = only[0];
   } else {
-    row_sum<2>(dots, red1, at, barrier);
+    row_sum16<2>(dots, red1, at, barrier);
   }
   const float2 nc1 = splat(-dots[0] * a.inv_width);
   if (!ok) return;
@@ -775,7 +799,9 @@ __global__ void __launch_bounds__(MAX_THREADS, MIN_CTAS)
 gated_norm_grad_kernel(const NormGradArgs a, int threads_per_row) {
   constexpr bool KEEP = ITERS <= 2;
   extern __shared__ float4 column_sums[];
-  __shared__ float red[2][MAX_THREADS / 32][2][32];
+  __shared__ __align__(16) float red[2][MAX_THREADS / 32][2][32];
+  for (int i = threadIdx.x; i < 2 * (MAX_THREADS / 32) * 64; i += blockDim.x) (&red[0][0][0][0])[i] = 0.0f;
+  __syncthreads();
   const int group = threadIdx.x / threads_per_row, groups = blockDim.x / threads_per_row;
   const Place at{(int)threadIdx.x - group * threads_per_row, threads_per_row};
   SharedSums<ITERS> sums{column_sums, (int)blockDim.x, (int)threadIdx.x};
@@ -842,6 +868,91 @@ gated_norm_grad_kernel(const NormGradArgs a, int threads_per_row) {
   if (a.post != nullptr) flush(1, a.part_post + (int64_t)blockIdx.x * a.width);
 }
 
+// Full vectors, one a thread, so that everything fits into registers: the row's operands, those of the next row on their way, the
+// parameters and the sums.
+template <typename T, typename P, bool SUM_GATE>
+__global__ void __launch_bounds__(kNormGradThreads, 1)
+gated_norm_grad_vector_kernel(const NormGradArgs a, int threads_per_row) {
+  constexpr bool VEC = true;
+  constexpr bool AHEAD = sizeof(T) == 2;                   // fp32 rows have no registers to wait in: they wait in L2
+  extern __shared__ float4 joined[];                       // [2][threads]
+  __shared__ __align__(16) float red[2][kNormGradThreads / 32][2][32];
+  for (int i = threadIdx.x; i < 2 * (kNormGradThreads / 32) * 64; i += blockDim.x) (&red[0][0][0][0])[i] = 0.0f;
+  __syncthreads();
+  const int group = threadIdx.x / threads_per_row, groups = blockDim.x / threads_per_row;
+  const Place at{(int)threadIdx.x - group * threads_per_row, threads_per_row};
+  RegisterSums<1> sums;
+  sums.clear(0), sums.clear(1), sums.clear(2);
+  auto flush = [&](int w, float* to) {                     // by the whole CTA
+    float2(&v)[4] = sums.open(w, 0);
+    if (groups > 1) {
+      __syncthreads();
+      if (group > 0) {
+        joined[threadIdx.x] = make_float4(v[0].x, v[0].y, v[1].x, v[1].y);
+        joined[blockDim.x + threadIdx.x] = make_float4(v[2].x, v[2].y, v[3].x, v[3].y);
+      }
+      __syncthreads();
+    }
+    if (group == 0) {
+      for (int g = 1; g < groups; ++g) {
+        const float4 p = joined[threadIdx.x + g * threads_per_row], q = joined[blockDim.x + threadIdx.x + g * threads_per_row];
+        v[0] = make_float2(v[0].x + p.x, v[0].y + p.y), v[1] = make_float2(v[1].x + p.z, v[1].y + p.w);
+        v[2] = make_float2(v[2].x + q.x, v[2].y + q.y), v[3] = make_float2(v[3].x + q.z, v[3].y + q.w);
+      }
+      store8<float, VEC>(to, 0, a.width, at, v);
+    }
+  };
+  auto fetch = [&](int64_t row, Pack8<T>(&to)[4], float& rs1, float& rs2) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      if (q < 3 || a.dh != nullptr)
+        load8<T, VEC>(static_cast<const T*>(q == 0 ? a.x : q == 1 ? a.residual : q == 2 ? a.dy : a.dh) + row * a.width, 0, a.width, at, to[q]);
+    rs2 = a.rstd[row];
+    rs1 = a.post != nullptr ? a.post_rstd[row] : 1.0f;
+  };
+  RegisterParams params;
+  if (a.post != nullptr) param8<P, VEC>(static_cast<const P*>(a.post), 0, a.width, at, params.w1);
+  param8<P, VEC>(static_cast<const P*>(a.gamma), 0, a.width, at, params.w2);
+  const int64_t r0 = a.rows * blockIdx.x / gridDim.x, r1 = a.rows * (blockIdx.x + 1) / gridDim.x;
+  for (int64_t seg = r0; seg < r1;) {
+    const int64_t gate = SUM_GATE ? seg / a.gate.rows_per : 0;
+    const int64_t seg_end = SUM_GATE ? min(r1, (gate + 1) * a.gate.rows_per) : r1;
+    if (SUM_GATE) gate8<P, VEC>(a.gate, gate, 0, a.width, at, params.g);
+    Pack8<T> kept[4], next[4];
+    float rs1 = 1.0f, rs2 = 0.0f, next1 = 1.0f, next2 = 0.0f;
+    if (AHEAD && seg + group < seg_end) fetch(seg + group, next, next1, next2);
+    for (int64_t row = seg + group; row < seg_end; row += groups) {
+      if constexpr (AHEAD) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) kept[q] = next[q];
+        rs1 = next1, rs2 = next2;
+        if (row + groups < seg_end) fetch(row + groups, next, next1, next2);
+      } else {
+        if (row + groups < r1) {
+          const int64_t ahead = (row + groups) * a.width + at.tid * 8;
+          if (at.tid % 4 == 0) {                           // one of the four threads of a 128-byte line
+            prefetch_l2(static_cast<const T*>(a.x) + ahead);
+            prefetch_l2(static_cast<const T*>(a.residual) + ahead);
+            prefetch_l2(static_cast<const T*>(a.dy) + ahead);
+            if (a.dh != nullptr) prefetch_l2(static_cast<const T*>(a.dh) + ahead);
+          }
+        }
+        fetch(row, kept, rs1, rs2);
+      }
+      if (!SUM_GATE) gate8<P, VEC>(a.gate, row, 0, a.width, at, params.g);
+      auto load = [&](int q, int) { return kept[q]; };
+      norm_grad_row<T, P, VEC, 1, SUM_GATE>(a, at, row, rs1, rs2, load, params, sums, red[0][group], red[1][group], 1 + group, true);
+    }
+    if (SUM_GATE) {
+      flush(2, a.part_gate + (blockIdx.x + gate) * a.width);
+      sums.clear(2);
+    }
+    seg = seg_end;
+  }
+  flush(0, a.part_gamma + (int64_t)blockIdx.x * a.width);
+  if (a.post != nullptr) flush(1, a.part_post + (int64_t)blockIdx.x * a.width);
+}
+
 // The same for rows that do not come as full vectors, through shared memory; sums in registers, joined by the CTA's row groups in
 // shared memory in a fixed order.
 template <typename T, typename P, bool SUM_GATE>
@@ -850,7 +961,8 @@ gated_norm_grad_pipe_kernel(const NormGradArgs a, int threads_per_row, int stage
   extern __shared__ __align__(16) uint8_t pipe_smem[];
   constexpr bool VEC = false;
   constexpr int ITERS = 1;
-  __shared__ float red[2][kRowPipeThreads / 32][2][32];
+  __shared__ __align__(16) float red[2][kRowPipeThreads / 32][2][32];
+  for (int i = threadIdx.x; i < 2 * (kRowPipeThreads / 32) * 64; i += blockDim.x) (&red[0][0][0][0])[i] = 0.0f;   // behind the next barrier
   const int readers = blockDim.x, groups = readers / threads_per_row;
   const RowPipe pipe = row_pipe_init(pipe_smem, stages, 4, groups, (int64_t)a.width * sizeof(T), a.rows, readers / 32);
   float* joined = reinterpret_cast<float*>(pipe.slot(stages, 0));   // [width] behind the ring
@@ -1090,20 +1202,17 @@ int launch_norm(const NormArgs& a, cudaStream_t st) {
   return check_launch("gated_add_rms_norm");
 }
 
-// CTAs of the gradient kernels, each of which writes one row of partial sums per parameter: at most kNormGradCtas an SM.
-constexpr int kNormGradCtas = 2;
-inline int grad_ctas(int64_t rows, int per_sm) {
-  const int64_t cap = (int64_t)per_sm * sm_count();
-  return (int)(rows < cap ? rows : cap);
-}
+// CTAs of the gradient kernels, each of which writes one row of partial sums per parameter: one an SM.
+inline int grad_ctas(int64_t rows) { return (int)(rows < sm_count() ? rows : sm_count()); }
 
-// Full vectors: CTAs of 256 threads, two an SM, with two vectors a thread and row up to 4096 columns (measured for 8192 rows of 4096
-// bf16: 124 us with the row's operands in registers, 130 read again from L1, 151 from L2; three CTAs an SM at 80 registers
-// 147, rows through shared memory with the sums in registers 176 to 203); 512 threads with two (up to 8192) or four vectors above.
+// Full vectors: one CTA of 512 threads an SM.  Up to 4096 columns a thread has one vector of a row, and everything fits into its
+// registers (8192 rows of 4096 bf16 with all three sums: 93 us, 4.3 TB/s, bound by instruction issue and the packed fp32
+// pipe; two vectors a thread with the sums in shared memory took 121, rows through shared memory 176 to 203; 16384 rows of 1024
+// 45 against 61); above two (4096 rows of 8192: 125 us) or four vectors a thread.
 // Else through shared memory, up to 4096 columns and from a 16-byte boundary on (f16, read three times from global memory against
 // that: 100 rows of 1111 65 / 16 us, 6124 309 / 59, 3000 of 4000 342 / 84, 20000 of 96 364 / 47), and straight for what is left.
 template <typename T, typename P, bool VEC>
-int launch_norm_grad(const NormGradArgs& a, NormSumArgs s, bool sum_gate, cudaStream_t st) {
+int launch_norm_grad(const NormGradArgs& a, const NormSumArgs& s, bool sum_gate, cudaStream_t st) {
 #define B200Q_NORM_GRAD(I, MAX, MIN, SUM)                                                                                \
   {                                                                                                                      \
     constexpr auto kern = gated_norm_grad_kernel<T, P, VEC, I, SUM, MAX, MIN>;                                           \
@@ -1117,25 +1226,24 @@ int launch_norm_grad(const NormGradArgs& a, NormSumArgs s, bool sum_gate, cudaSt
 #define B200Q_NORM_GRAD_BOTH(I, MAX, MIN)                                                                                \
   if (sum_gate) B200Q_NORM_GRAD(I, MAX, MIN, true) else B200Q_NORM_GRAD(I, MAX, MIN, false)
   if constexpr (VEC) {
-    // Whole warps of vectors: a multiple of 512 columns takes two vectors a thread, of 256 one, above 8192 columns four.
-    const int iters = a.width > 8192 ? 4 : a.width % 512 == 0 ? 2 : 1;
-    const int threads = (int)(a.width / (8 * iters));
-    s.ctas = grad_ctas(a.rows, threads <= 256 && iters < 4 ? 2 : 1);
-    if (iters == 4) {
-      B200Q_NORM_GRAD_BOTH(4, 512, 1)
-    } else if (threads > 256) {
-      if (iters == 2) {
-        B200Q_NORM_GRAD_BOTH(2, 512, 1)
-      } else {
-        B200Q_NORM_GRAD_BOTH(1, 512, 1)
-      }
-    } else if (iters == 2) {
-      B200Q_NORM_GRAD_BOTH(2, 256, 2)
+    if (a.width <= 8 * kNormGradThreads) {
+      const int threads = (int)(a.width / 8);
+      int groups = kNormGradThreads / threads;
+      if (groups > 15) groups = 15;                        // named barriers
+      if (groups > ceil_div(a.rows, s.ctas)) groups = (int)ceil_div(a.rows, s.ctas);
+      const int smem = 2 * 16 * groups * threads;
+      if (sum_gate) gated_norm_grad_vector_kernel<T, P, true><<<s.ctas, groups * threads, smem, st>>>(a, threads);
+      else gated_norm_grad_vector_kernel<T, P, false><<<s.ctas, groups * threads, smem, st>>>(a, threads);
     } else {
-      B200Q_NORM_GRAD_BOTH(1, 256, 2)
+      const int iters = a.width > 8192 ? 4 : 2;
+      const int threads = (int)(a.width / (8 * iters));
+      if (iters == 4) {
+        B200Q_NORM_GRAD_BOTH(4, 512, 1)
+      } else {
+        B200Q_NORM_GRAD_BOTH(2, 512, 1)
+      }
     }
   } else {
-    s.ctas = grad_ctas(a.rows, 1);
     const RowPipePlan p = row_pipe_plan(a.width, sizeof(T), 4, 1, a.rows, s.ctas, (int)((a.width * 4 + 15) & ~15));
     if (p.fits && aligned(a.x, 16) && aligned(a.residual, 16) && aligned(a.dy, 16) && aligned(a.dh, 16)) {
 #define B200Q_NORM_GRAD_PIPE(SUM)                                                                                        \
@@ -1239,7 +1347,7 @@ extern "C" int b200q_gated_norm(const b200q_gated_norm_args* a, void* stream) {
 extern "C" size_t b200q_gated_norm_grad_workspace_bytes(const b200q_gated_norm_args* a) {
   using namespace b200q;
   if (a == nullptr || a->rows <= 0 || a->width <= 0) return 0;
-  const int64_t ctas = grad_ctas(a->rows, kNormGradCtas);
+  const int64_t ctas = grad_ctas(a->rows);
   const int64_t gates = gate_is_shared(*a) ? ctas + ceil_div(a->rows, a->gate_rows) : 0;
   return (size_t)(2 * ctas + gates) * (size_t)a->width * 4;
 }
@@ -1272,7 +1380,7 @@ extern "C" int b200q_gated_norm_grad(const b200q_gated_norm_args* a, const b200q
   const size_t need = b200q_gated_norm_grad_workspace_bytes(a);
   B200Q_REQUIRE(g->workspace != nullptr && g->workspace_bytes >= need && aligned(g->workspace, 256), B200Q_ERR_WORKSPACE,
                 "%s: needs %zu bytes of 256-byte aligned workspace, got %zu", op, need, g->workspace_bytes);
-  const int ctas = grad_ctas(a->rows, kNormGradCtas);   // at most: the launch may use fewer
+  const int ctas = grad_ctas(a->rows);
   // Partial rows lie `width` apart, so vectors of them are aligned exactly when the width allows vectors at all.
   float* part = static_cast<float*>(g->workspace);
   NormGradArgs n{};
@@ -1286,7 +1394,7 @@ extern "C" int b200q_gated_norm_grad(const b200q_gated_norm_args* a, const b200q
   NormSumArgs s{};
   s.part_gamma = n.part_gamma; s.part_post = a->post_gamma != nullptr ? n.part_post : nullptr; s.part_gate = n.part_gate;
   s.dgamma = g->dgamma; s.dpost = g->dpost_gamma; s.dgate = g->dgate; s.dtype = a->param_dtype;
-  s.rows = a->rows; s.rows_per = shared ? a->gate_rows : 1; s.width = a->width;
+  s.rows = a->rows; s.rows_per = shared ? a->gate_rows : 1; s.width = a->width; s.ctas = ctas;
   const bool vec = norm_vec(a->width, {a->x, a->residual, g->dy, g->dh, g->dx, g->dresidual, a->gamma, a->post_gamma,
                                        a->gate_per_row ? nullptr : a->gate, a->gate_per_row || shared ? nullptr : g->dgate});
 #define B200Q_CALL(T, P) (vec ? launch_norm_grad<T, P, true>(n, s, shared, st) : launch_norm_grad<T, P, false>(n, s, shared, st))
