@@ -223,7 +223,9 @@ def test_captured_step_replays(npu):
 # rows), gates that change within a CTA's rows, and storage off the vector grid.
 MANY = [((700, 256), "channel", True), ((1200, 512), "row", True), ((600, 768), "full", True), ((40, 31, 1024), "sample", True), ((333, 4096), "channel", True),
         ((301, 5632), "channel", True), ((310, 8192), "sample2", True), ((299, 9216), "channel", True), ((150, 16384), "channel", True), ((905, 1111), "channel", True),
-        ((7, 131, 333), "sample", True), ((2500, 8), "sample2", True), ((777, 17), None, False), ((301, 4095), "full", False), ((300, 4097), "row", True)]
+        ((7, 131, 333), "sample", True), ((2500, 8), "sample2", True), ((777, 17), None, False), ((301, 4095), "full", False), ((300, 4097), "row", True),
+        ((1301, 1111), "channel", True), ((3, 431, 555), "sample", False), ((1250, 2047), "full", True), ((6, 200, 513), "sample", True),
+        ((1500, 700), "sample2", True), ((1600, 256), "sample2", True), ((905, 2048), "sample2", False)]
 
 
 @pytest.mark.parametrize("dtype,ptype", [(torch.bfloat16, torch.bfloat16), (torch.float16, torch.float32), (torch.float32, torch.float32)])
@@ -259,3 +261,26 @@ def test_many_rows(npu, case, dtype, ptype):
         for n, t in zip(names, torch.autograd.grad((y, h), have, (place(dy), place(dh)))):
             rows = x.numel() // width
             within(t, want[n], width, n, rows=rows if n in ("gamma", "post_gamma", "gate") else 1, terms=terms[n])
+
+
+def test_one_tensor_twice_and_expanded_inputs(npu):
+    """x as its own residual, one row expanded over all rows, one gamma for both norms: the gradients of what is shared are the sums
+    that autograd adds up; nothing is written through an expanded input."""
+    g = torch.Generator().manual_seed(11)
+    for width, dtype in ((512, torch.float32), (77, torch.float32)):
+        x, res, gamma, _, gt = inputs((40, width), dtype, torch.float32, "channel", True, g)
+        dy, dh = torch.randn((40, width), generator=g), torch.randn((40, width), generator=g)
+        a, w = x.cuda().requires_grad_(), gamma.cuda().requires_grad_()
+        y, _, h, _ = npu.npu_gated_add_rms_norm(a, a, w, post_gamma=w, gate=gt.cuda(), residual_scale=0.5, epsilon=EPS)
+        torch.autograd.backward((y, h), (dy.cuda(), dh.cuda()))
+        want, terms = oracle.gated_add_rms_norm_grad(x, x, gamma, gamma, gt, 0.5, EPS, dy, dh)
+        within(a.grad, want["x"] + want["residual"], width, "x", terms=terms["x"] + terms["residual"])
+        within(w.grad, want["gamma"] + want["post_gamma"], width, "gamma", rows=40, terms=terms["gamma"] + terms["post_gamma"])
+        row = x[:1].clone()
+        leaf = row.cuda().requires_grad_()
+        y, _, h, _ = npu.npu_gated_add_rms_norm(leaf.expand(40, width), res.cuda(), gamma.cuda(), gate=gt.cuda(), residual_scale=0.5, epsilon=EPS)
+        torch.autograd.backward((y, h), (dy.cuda(), dh.cuda()[:1].expand(40, width)))
+        want, terms = oracle.gated_add_rms_norm_grad(row.expand(40, width).contiguous(), res, gamma, None, gt, 0.5, EPS, dy,
+                                                     dh[:1].expand(40, width).contiguous())
+        assert torch.equal(leaf.detach().cpu(), row)
+        within(leaf.grad, want["x"].sum(0, keepdim=True), width, "row", rows=40, terms=terms["x"].max() * 40)

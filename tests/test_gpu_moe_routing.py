@@ -267,3 +267,24 @@ def test_refusals(npu):
         a = x.float().requires_grad_()
         y, _ = npu.npu_moe_token_permute(a, i)
         torch.autograd.grad(y.sum(), a, create_graph=True)
+
+
+def test_expanded_inputs_and_one_set_of_rows_twice(npu):
+    """One token's row and one row of weights expanded over all tokens; the rows of one permute used by two unpermutes."""
+    g = torch.Generator().manual_seed(12)
+    t, k, h = 700, 4, 264
+    idx = ids_of(t, k, 16, g)
+    x, w, dy = torch.randn((1, h), generator=g), torch.rand((1, k), generator=g), torch.randn((t, h), generator=g)
+    row, _, _ = oracle.sorted_rows(idx, 0, 1024)
+    lx, lw = x.cuda().requires_grad_(), w.cuda().requires_grad_()
+    rows, place = npu.npu_moe_token_permute(lx.expand(t, h), idx.cuda())
+    assert torch.equal(place.cpu(), row) and torch.equal(rows.detach().cpu(), x.expand(t * k, h))
+    first = npu.npu_moe_token_unpermute(rows, place, lw.expand(t, k))
+    second = npu.npu_moe_token_unpermute(rows, place, lw.expand(t, k).flip(1))
+    (first + second).backward(dy.cuda())
+    sum_w = float(w.double().sum())
+    # y = 2 * sum(w) * x for every token, through fp32 sums of k products, added up over t tokens and 2 k slots
+    assert bool(((lx.grad.cpu().double() - 2 * sum_w * dy.double().sum(0)).abs() <= dy.double().abs().sum(0) * 2 * sum_w * (t + 4 * k) * 2.0 ** -24).all())
+    dots = (dy.double() @ x.double().t()).sum()
+    size = (dy.double().abs() @ x.double().abs().t()).sum()
+    assert bool(((lw.grad.cpu().double() - 2 * dots).abs() <= 2 * size * (t + h) * 2.0 ** -24).all())
