@@ -1206,8 +1206,8 @@ int launch_norm(const NormArgs& a, cudaStream_t st) {
 inline int grad_ctas(int64_t rows) { return (int)(rows < sm_count() ? rows : sm_count()); }
 
 // Full vectors: one CTA of 512 threads an SM.  Up to 4096 columns a thread has one vector of a row, and everything fits into its
-// registers (8192 rows of 4096 bf16 with all three sums: 93 us, 4.3 TB/s, bound by instruction issue and the packed fp32
-// pipe; two vectors a thread with the sums in shared memory took 121, rows through shared memory 176 to 203; 16384 rows of 1024
+// registers (8192 rows of 4096 bf16 with all three sums: 93 us, 4.3 TB/s, half of the issue slots, the packed fp32 pipe and the
+// row sums' shuffles; two vectors a thread with the sums in shared memory took 121, rows through shared memory 176 to 203; 16384 rows of 1024
 // 45 against 61); above two (4096 rows of 8192: 125 us) or four vectors a thread.
 // Else through shared memory, up to 4096 columns and from a 16-byte boundary on (f16, read three times from global memory against
 // that: 100 rows of 1111 65 / 16 us, 6124 309 / 59, 3000 of 4000 342 / 84, 20000 of 96 364 / 47), and straight for what is left.
