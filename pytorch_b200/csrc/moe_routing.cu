@@ -313,13 +313,13 @@ moe_copy_direct_kernel(const RouteIds r, const VT* __restrict__ x, VT* __restric
 template <typename VT, int U>
 __global__ void __launch_bounds__(256)
 moe_copy_kernel(const VT* __restrict__ x, VT* __restrict__ out, int64_t tokens, int topk, int64_t nvec, int segs, int64_t out_rows,
-                const float* __restrict__ token_scale, float* __restrict__ out_scale, const int32_t* __restrict__ row_idx,
-                const int32_t* __restrict__ valid_rows, int64_t move_blocks) {
+                const float* __restrict__ token_scale, float* __restrict__ out_scale, const int32_t* row_idx,
+                const int32_t* valid_rows, int64_t move_blocks) {
   const int lane = threadIdx.x & 31;
   if ((int64_t)blockIdx.x >= move_blocks) {
     wait_for_primary();
     const int64_t zb = blockIdx.x - move_blocks, zn = gridDim.x - move_blocks;
-    for (int64_t row = *valid_rows + zb; row < out_rows; row += zn) {
+    for (int64_t row = ld_of_primary(valid_rows) + zb; row < out_rows; row += zn) {
       for (int64_t v = threadIdx.x; v < nvec; v += blockDim.x) out[row * nvec + v] = VT{};
       if (out_scale != nullptr && threadIdx.x == 0) out_scale[row] = 0.0f;
     }
@@ -336,7 +336,7 @@ moe_copy_kernel(const VT* __restrict__ x, VT* __restrict__ out, int64_t tokens, 
     if (v0 + 32 * u < nvec) val[u] = x[t * nvec + v0 + 32 * u];
   wait_for_primary();                                      // the sort's rows; x does not depend on it
   for (int k0 = 0; k0 < topk; k0 += 32) {
-    const int mine = k0 + lane < topk ? row_idx[t * topk + k0 + lane] : -1;
+    const int mine = k0 + lane < topk ? ld_of_primary(row_idx + t * topk + k0 + lane) : -1;
     const int kc = min(32, topk - k0);
     for (int k = 0; k < kc; ++k) {
       const int64_t row = __shfl_sync(0xffffffffu, mine, k);
@@ -472,11 +472,11 @@ moe_quant_direct_kernel(const RouteIds r, const T* __restrict__ x, int64_t width
 template <typename T, typename ST, int ITERS, bool FULL>
 __global__ void __launch_bounds__(512)
 moe_quant_kernel(int64_t n, const T* __restrict__ x, int64_t width, const ST* __restrict__ smooth, int smooth_rows, int8_t* __restrict__ out,
-                 float* __restrict__ out_scale, const int2* __restrict__ row_info, const int32_t* __restrict__ valid_rows) {
+                 float* __restrict__ out_scale, const int2* row_info, const int32_t* valid_rows) {
   __shared__ float red[2][32];
   wait_for_primary();
   const int nvec = (int)(width >> 3);
-  const int64_t valid = *valid_rows;
+  const int64_t valid = ld_of_primary(valid_rows);
   const int64_t r0 = valid * blockIdx.x / gridDim.x, r1 = valid * (blockIdx.x + 1) / gridDim.x;
   constexpr int N = ITERS ? ITERS : 1;
   uint4 raw[N], nxt[FULL ? 1 : N];
@@ -489,10 +489,10 @@ moe_quant_kernel(int64_t n, const T* __restrict__ x, int64_t width, const ST* __
   // A row's token and expert are read two rows ahead, its x one row ahead.
   int2 here = make_int2(0, 0), after = make_int2(0, 0);
   if (r0 < r1) {
-    after = row_info[r0];
+    after = ld_of_primary(row_info + r0);
     load(after.x);
   }
-  int2 later = r0 + 1 < r1 ? row_info[r0 + 1] : make_int2(0, 0);
+  int2 later = r0 + 1 < r1 ? ld_of_primary(row_info + r0 + 1) : make_int2(0, 0);
   // This CTA's share of the rows that no assignment owns.
   const int64_t idle = n - valid;
   for (int64_t row = valid + idle * blockIdx.x / gridDim.x; row < valid + idle * (blockIdx.x + 1) / gridDim.x; ++row) {
@@ -512,7 +512,7 @@ moe_quant_kernel(int64_t n, const T* __restrict__ x, int64_t width, const ST* __
       for (int q = 0; q < ITERS; ++q) raw[q] = nxt[q];
       if (row + 1 < r1) load(after.x);
     }
-    if (row + 2 < r1) later = row_info[row + 2];
+    if (row + 2 < r1) later = ld_of_primary(row_info + row + 2);
     par ^= 1;                                              // a buffer is written again only behind the other one's barrier
     const ST* sm = smooth == nullptr ? nullptr : smooth + (smooth_rows > 1 ? here.y * width : 0);
     if constexpr (ITERS > 0) {

@@ -427,6 +427,19 @@ __device__ __forceinline__ void bulk_load(void* smem_dst, const void* src, uint3
 // and the wait of that kernel for all of this one's work.
 __device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void wait_for_primary() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+// Reads what that kernel wrote, behind wait_for_primary().  A load through a const __restrict__ pointer may be taken for one of
+// read-only data: the compiler may move it in front of the wait, and the SM's L1 may answer it with what a neighbouring address
+// brought in before the wait.  These are neither moved nor answered by L1.
+__device__ __forceinline__ int32_t ld_of_primary(const int32_t* p) {
+  int32_t v;
+  asm volatile("ld.relaxed.gpu.global.s32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
+  return v;
+}
+__device__ __forceinline__ int2 ld_of_primary(const int2* p) {
+  int2 v;
+  asm volatile("ld.relaxed.gpu.global.v2.s32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p) : "memory");
+  return v;
+}
 
 // Named barrier among a subset of the CTA's warps (id 1..15; 0 is __syncthreads).
 __device__ __forceinline__ void named_barrier_sync(uint32_t id, uint32_t nthreads) {

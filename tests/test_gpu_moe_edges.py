@@ -1,0 +1,55 @@
+"""The mixture-of-experts block operators in places where memory, parameters or values lie at an edge: buffers that touch one
+another, parameters and values that are not finite, rows of no width."""
+import ctypes as C
+
+import pytest
+import torch
+
+from oracle import moe_oracle as oracle
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def npu():
+    import pytorch_b200  # noqa: F401
+    assert torch.cuda.is_available()
+    return torch.ops.npu
+
+
+@pytest.fixture(autouse=True)
+def no_device_error():
+    yield
+    from pytorch_b200 import _cabi
+    torch.cuda.synchronize()
+    assert _cabi.device_error() == 0
+
+
+@pytest.mark.parametrize("hidden", [20, 24, 30])
+@pytest.mark.parametrize("repeat", range(3))
+def test_rows_next_to_their_indices(npu, hidden, repeat):
+    """x ends and row_idx begins in one 32-byte sector.  The copy kernel loads x while the sort still runs and reads the rows
+    afterwards: they are the sort's, not what the sector held when x came in (-1, which would leave the row out)."""
+    from pytorch_b200 import _cabi as cabi
+    tokens, topk, experts = 3, 1024, 64
+    n = tokens * topk
+    g = torch.Generator().manual_seed(hidden + repeat)
+    idx = torch.randint(0, experts, (tokens, topk), generator=g, dtype=torch.int32)
+    x = torch.randn((tokens, hidden), generator=g).to(torch.bfloat16)
+    raw = x.view(torch.uint8).numel()
+    assert raw % 4 == 0
+    buf = torch.full((raw + 4 * n,), 0xFF, dtype=torch.uint8, device="cuda")
+    buf[:raw] = x.view(torch.uint8).reshape(-1).cuda()
+    ids, out = idx.cuda(), torch.zeros((n, hidden), dtype=torch.bfloat16, device="cuda")
+    ws = torch.empty(256, dtype=torch.uint8, device="cuda")
+    a = cabi.MoeRouteArgs()
+    a.x, a.x_dtype, a.expert_idx, a.idx_dtype = buf.data_ptr(), cabi.BF16, ids.data_ptr(), cabi.I32
+    a.tokens, a.topk, a.hidden, a.expert_begin, a.expert_end = tokens, topk, hidden, 0, experts
+    a.out, a.out_rows, a.row_idx = out.data_ptr(), n, buf.data_ptr() + raw
+    a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
+    torch.cuda.synchronize()
+    assert cabi.lib().b200q_moe_route(C.byref(a), torch.cuda.current_stream().cuda_stream) == cabi.OK
+    torch.cuda.synchronize()
+    row, src, _ = oracle.sorted_rows(idx, 0, experts)
+    assert torch.equal(buf[raw:].view(torch.int32).cpu(), row)
+    assert torch.equal(out.cpu(), oracle.gather_rows(x, src, topk))
