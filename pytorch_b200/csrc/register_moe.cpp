@@ -2,6 +2,7 @@
 // Meta implementations over the C ABI, and autograd functions whose backward passes are operators of their own
 // (npu_moe_token_permute_grad, npu_moe_token_unpermute_grad).  A call that needs no gradient goes straight to the
 // CUDA implementation.
+#include <torch/csrc/autograd/autograd_not_implemented_fallback.h>
 #include <torch/csrc/autograd/custom_function.h>
 
 #include "register_common.h"
@@ -627,6 +628,14 @@ NormOutputs norm_below(const Tensor& x, const Tensor& residual, const Tensor& ga
   return op.call(x, residual, gamma, post, gate, residual_scale, epsilon);
 }
 
+// A dual tensor's tangent (forward-mode differentiation) would be lost below autograd: it is refused, as PyTorch refuses it for an
+// autograd function without a jvp.
+void no_forward_mode(const char* op, std::initializer_list<const optional<Tensor>*> inputs) {
+  for (const optional<Tensor>* t : inputs)
+    TORCH_CHECK_NOT_IMPLEMENTED(!(t->has_value() && (*t)->defined() && (*t)->_fw_grad(/*level=*/0).defined()), op,
+                                ": forward-mode differentiation is not supported");
+}
+
 class PermuteFunction : public torch::autograd::Function<PermuteFunction> {
  public:
   static variable_list forward(AutogradContext* ctx, const Tensor& tokens, const Tensor& indices, optional<int64_t> num_out, bool padded_mode) {
@@ -653,6 +662,8 @@ class PermuteFunction : public torch::autograd::Function<PermuteFunction> {
 };
 
 std::tuple<Tensor, Tensor> permute_autograd(const Tensor& tokens, const Tensor& indices, optional<int64_t> num_out, bool padded_mode) {
+  const optional<Tensor> to(tokens);
+  no_forward_mode("npu_moe_token_permute", {&to});
   if (!(at::GradMode::is_enabled() && tokens.requires_grad())) {
     return permute_below(tokens, indices, num_out, padded_mode);
   }
@@ -683,6 +694,8 @@ class UnpermuteFunction : public torch::autograd::Function<UnpermuteFunction> {
 
 Tensor unpermute_autograd(const Tensor& rows, const Tensor& sorted, const optional<Tensor>& probs, bool padded_mode,
                           at::OptionalIntArrayRef restore_shape) {
+  const optional<Tensor> ro(rows);
+  no_forward_mode("npu_moe_token_unpermute", {&ro, &probs});
   if (!(at::GradMode::is_enabled() && (rows.requires_grad() || (probs.has_value() && probs->requires_grad())))) {
     return unpermute_below(rows, sorted, probs, padded_mode, restore_shape);
   }
@@ -722,6 +735,8 @@ class NormFunction : public torch::autograd::Function<NormFunction> {
 
 NormOutputs norm_autograd(const Tensor& x, const Tensor& residual, const Tensor& gamma, const optional<Tensor>& post, const optional<Tensor>& gate,
                           double residual_scale, double epsilon) {
+  const optional<Tensor> xo(x), ro(residual), go(gamma);
+  no_forward_mode("npu_gated_add_rms_norm", {&xo, &ro, &go, &post, &gate});
   const bool wanted = x.requires_grad() || residual.requires_grad() || gamma.requires_grad() || (post.has_value() && post->requires_grad()) ||
                       (gate.has_value() && gate->requires_grad());
   if (!(at::GradMode::is_enabled() && wanted)) {
@@ -773,6 +788,11 @@ TORCH_LIBRARY_IMPL(npu, AutogradCUDA, m) {
   m.impl("npu_moe_token_permute", TORCH_FN(permute_autograd));
   m.impl("npu_moe_token_unpermute", TORCH_FN(unpermute_autograd));
   m.impl("npu_gated_add_rms_norm", TORCH_FN(norm_autograd));
+  // No derivative of their own, in either mode, although some of their outputs are floats: asking for one is an error, where
+  // PyTorch's default for an operator without an autograd kernel is a warning in reverse mode and a lost tangent in forward mode.
+  for (const char* op : {"npu_moe_init_routing_v2", "npu_moe_token_permute_grad", "npu_moe_token_unpermute_grad", "npu_gated_add_rms_norm_grad",
+                         "npu_gated_add_rms_norm_dynamic_quant"})
+    m.impl(op, torch::autograd::autogradNotImplementedFallback());
 }
 
 TORCH_LIBRARY_IMPL(npu, Meta, m) {
