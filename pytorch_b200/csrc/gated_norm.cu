@@ -104,7 +104,8 @@ __device__ __forceinline__ void store8(T* __restrict__ row, int i, int width, co
   }
 }
 
-// Eight parameter values.  Past the width the last column's are read: they only ever meet zeros there.
+// Eight parameter values, zero past the width: a row's values are zero there too, and a parameter that is not finite must not make
+// them anything else.
 template <typename P, bool VEC>
 __device__ __forceinline__ void param8(const P* __restrict__ p, int i, int width, const Place& at, float2 (&f)[4]) {
   const int c = at.col<VEC>(i, 0);
@@ -112,8 +113,10 @@ __device__ __forceinline__ void param8(const P* __restrict__ p, int i, int width
     load_smooth8(p + c, f);
   } else {
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      f[j] = make_float2(to_f32<P>(p[min(c + 2 * j * at.threads, width - 1)]), to_f32<P>(p[min(c + (2 * j + 1) * at.threads, width - 1)]));
+    for (int j = 0; j < 4; ++j) {
+      const int c0 = c + 2 * j * at.threads, c1 = c0 + at.threads;
+      f[j] = make_float2(c0 < width ? to_f32<P>(p[c0]) : 0.0f, c1 < width ? to_f32<P>(p[c1]) : 0.0f);
+    }
   }
 }
 

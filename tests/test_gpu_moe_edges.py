@@ -53,3 +53,27 @@ def test_rows_next_to_their_indices(npu, hidden, repeat):
     row, src, _ = oracle.sorted_rows(idx, 0, experts)
     assert torch.equal(buf[raw:].view(torch.int32).cpu(), row)
     assert torch.equal(out.cpu(), oracle.gather_rows(x, src, topk))
+
+
+def norm_inputs(rows, width, g):
+    x, res = (torch.randn((rows, width), generator=g) + 4).to(torch.bfloat16), torch.randn((rows, width), generator=g).to(torch.bfloat16)
+    param = lambda: torch.rand(width, generator=g) + 0.5  # noqa: E731
+    return x, res, param(), param(), param()
+
+
+# Rows in full vectors; rows of other widths, a handful and many of them (which pass through shared memory).
+WIDTHS = [(3, 256), (3, 8), (5, 17), (4, 1111), (2, 4097), (1300, 1111), (1250, 520), (1300, 768)]
+
+
+@pytest.mark.parametrize("which", ["post_gamma", "gate"])
+@pytest.mark.parametrize("rows,width", WIDTHS)
+def test_an_infinite_parameter_in_the_last_column(npu, rows, width, which):
+    """h is infinite in that column, so the row's factor is 0: y is 0 in every other column, and 0 * infinity there.  Lanes behind
+    the row's end take no part."""
+    g = torch.Generator().manual_seed(width)
+    x, res, gamma, post, gate = norm_inputs(rows, width, g)
+    (post if which == "post_gamma" else gate)[-1] = float("inf")
+    y, rstd, h, post_rstd = npu.npu_gated_add_rms_norm(x.cuda(), res.cuda(), gamma.cuda(), post_gamma=post.cuda(), gate=gate.cuda())
+    assert float(rstd.abs().max()) == 0 and bool(torch.isfinite(post_rstd).all())
+    assert bool(torch.isinf(h[:, -1]).all()) and bool(torch.isfinite(h[:, :-1]).all())
+    assert float(y[:, :-1].abs().max()) == 0 and bool(torch.isnan(y[:, -1]).all())
