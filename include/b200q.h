@@ -313,7 +313,7 @@ int b200q_moe_combine_grad(const b200q_moe_combine_grad_args* args, void* stream
  *   h = residual_scale * residual + gate * z
  *   y = h * rsqrt(mean(h^2) + epsilon) * gamma
  * all in fp32, y and h rounded once.  With `scale` (the _dynamic_quant form) y is int8: y * smooth quantised per row as
- * b200q_dynamic_quant. */
+ * b200q_dynamic_quant.  A row with an infinity or a NaN gets a scale that is not finite. */
 typedef struct {
   const void* x;            /* [rows, width] bf16, f16 or f32; width at most 16384                          */
   const void* residual;     /* the same                                                                     */

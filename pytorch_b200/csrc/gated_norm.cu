@@ -182,6 +182,14 @@ __device__ __forceinline__ void row_sum16(float (&v)[N], float (*red)[32], const
   }
 }
 
+// The larger magnitude, NaN if either is NaN (fmaxf would pass over it, and a row that is all NaN would leave quantised as zeros with
+// scale 0).  Behind it NaN stays the largest: its bits are above infinity's.
+__device__ __forceinline__ float max_or_nan(float a, float b) {
+  float m;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(a), "f"(fabsf(b)));
+  return m;
+}
+
 // Maxima of N non-negative values over the threads of a row.
 template <int N>
 __device__ __forceinline__ void row_max(float (&v)[N], float (*red)[32], const Place& at, int barrier) {
@@ -426,7 +434,7 @@ gated_norm_kernel(const NormArgs a) {
         float2 y = __fmul2_rn(__fmul2_rn(h[i][j], splat(r2)), EARLY ? early_gamma[j] : w[j]);
         if (QUANT) {
           if (a.smooth != nullptr) y = __fmul2_rn(y, EARLY ? early_smooth[j] : sm[j]);
-          amax = fmaxf(amax, fmaxf(fabsf(y.x), fabsf(y.y)));
+          amax = max_or_nan(max_or_nan(amax, y.x), y.y);
         }
         h[i][j] = y;
       }
@@ -578,7 +586,7 @@ gated_norm_pipe_kernel(const NormArgs a, int threads_per_row, int stages) {
             float2 y = __fmul2_rn(__fmul2_rn(h[k][i][j], splat(r2[k])), w_gamma[j]);
             if (QUANT) {
               if (a.smooth != nullptr) y = __fmul2_rn(y, w_smooth[j]);
-              amax[k] = fmaxf(amax[k], fmaxf(fabsf(y.x), fabsf(y.y)));
+              amax[k] = max_or_nan(max_or_nan(amax[k], y.x), y.y);
             }
             h[k][i][j] = y;
           }

@@ -77,3 +77,25 @@ def test_an_infinite_parameter_in_the_last_column(npu, rows, width, which):
     assert float(rstd.abs().max()) == 0 and bool(torch.isfinite(post_rstd).all())
     assert bool(torch.isinf(h[:, -1]).all()) and bool(torch.isfinite(h[:, :-1]).all())
     assert float(y[:, :-1].abs().max()) == 0 and bool(torch.isnan(y[:, -1]).all())
+
+
+@pytest.mark.parametrize("post", [False, True])
+@pytest.mark.parametrize("rows,width", [(10, 256), (10, 64), (12, 8192), (1300, 1111), (1300, 512)])
+def test_rows_that_are_not_finite_keep_a_scale_that_is_not(npu, rows, width, post):
+    """int8 cannot hold what is not finite, so the row's scale says it: a row of y with an infinity or a NaN does not leave as zeros
+    with scale 0, which would look like a row of zeros.  The other rows keep their bits."""
+    g = torch.Generator().manual_seed(width + post)
+    x, res, gamma, pg, gate = norm_inputs(rows, width, g)
+    smooth = torch.rand(width, generator=g) + 0.5
+    bad = [1, 4, 5, rows - 1]
+    x[1, 2], res[4, width - 1], x[5, 0], res[rows - 1, 1] = float("inf"), float("-inf"), float("nan"), float("nan")
+    kw = dict(post_gamma=pg.cuda() if post else None, gate=gate.cuda())
+    for sm in (None, smooth.cuda()):
+        q, scale, h = npu.npu_gated_add_rms_norm_dynamic_quant(x.cuda(), res.cuda(), gamma.cuda(), smooth_scales=sm, **kw)
+        assert not bool(torch.isfinite(scale[bad]).any())
+        clean = torch.ones(rows, dtype=torch.bool)
+        clean[bad] = False
+        zeroed = [torch.where(clean[:, None], t, 0).cuda() for t in (x, res)]
+        q2, scale2, h2 = npu.npu_gated_add_rms_norm_dynamic_quant(*zeroed, gamma.cuda(), smooth_scales=sm, **kw)
+        assert torch.equal(q[clean.cuda()], q2[clean.cuda()]) and torch.equal(scale[clean.cuda()], scale2[clean.cuda()])
+        assert torch.equal(h[clean.cuda()], h2[clean.cuda()]) and bool((scale2[clean.cuda()] > 0).all())
