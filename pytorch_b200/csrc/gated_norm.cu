@@ -1337,9 +1337,11 @@ extern "C" int b200q_gated_norm(const b200q_gated_norm_args* a, void* stream) {
   B200Q_REQUIRE(quant || a->smooth == nullptr, B200Q_ERR_BAD_ARG, "%s: smooth scales belong to the quantised form (scale is NULL)", op);
   if (a->rows == 0) return B200Q_OK;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (a->width == 0) {
+  if (a->width == 0) {                                       // the mean over nothing is NaN (all bits set): the statistics are defined here too
     cudaError_t e = cudaSuccess;
     if (quant) e = cudaMemsetAsync(a->scale, 0, (size_t)a->rows * 4, st);
+    for (float* stat : {a->rstd, a->post_rstd})
+      if (e == cudaSuccess && stat != nullptr) e = cudaMemsetAsync(stat, 0xFF, (size_t)a->rows * 4, st);
     return e == cudaSuccess ? B200Q_OK : fail(B200Q_ERR_LAUNCH, "%s: %s", op, cudaGetErrorString(e));
   }
   B200Q_REQUIRE(a->x != nullptr && a->residual != nullptr && a->y != nullptr && a->h != nullptr && a->gamma != nullptr, B200Q_ERR_BAD_ARG,

@@ -340,7 +340,8 @@ b200q_gated_norm_args norm_args(const char* op, const Tensor& x, const Tensor& r
   a.residual_scale = static_cast<float>(residual_scale);
   a.epsilon = static_cast<float>(epsilon);
   a.width = x.size(-1);
-  a.rows = a.width ? x.numel() / a.width : 0;
+  a.rows = 1;
+  for (int64_t i = 0; i + 1 < x.dim(); ++i) a.rows *= x.size(i);   // rows without columns have statistics too
   return a;
 }
 

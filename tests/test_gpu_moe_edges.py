@@ -99,3 +99,16 @@ def test_rows_that_are_not_finite_keep_a_scale_that_is_not(npu, rows, width, pos
         q2, scale2, h2 = npu.npu_gated_add_rms_norm_dynamic_quant(*zeroed, gamma.cuda(), smooth_scales=sm, **kw)
         assert torch.equal(q[clean.cuda()], q2[clean.cuda()]) and torch.equal(scale[clean.cuda()], scale2[clean.cuda()])
         assert torch.equal(h[clean.cuda()], h2[clean.cuda()]) and bool((scale2[clean.cuda()] > 0).all())
+
+
+@pytest.mark.parametrize("shape", [(4, 0), (2, 3, 0)])
+def test_statistics_of_rows_without_columns(npu, shape):
+    """The mean over nothing is NaN, and so is its root's reciprocal: no statistic is left as the memory had it."""
+    w = torch.ones(0, device="cuda")
+    for dtype in (torch.float32, torch.bfloat16):
+        x = torch.zeros(shape, dtype=dtype, device="cuda")
+        for fill in (0.0, 1.0):
+            torch.full(shape[:-1], fill, device="cuda")                 # what the allocator hands out next
+            _, rstd, _, post_rstd = npu.npu_gated_add_rms_norm(x, x, w, post_gamma=w)
+            assert rstd.shape == post_rstd.shape == shape[:-1]
+            assert bool(torch.isnan(rstd).all()) and bool(torch.isnan(post_rstd).all())
