@@ -261,7 +261,7 @@ typedef struct {
   const void* expert_idx;   /* [tokens, topk] i32 or i64                                                    */
   int idx_dtype;
   int64_t tokens, topk, hidden;
-  int64_t expert_begin, expert_end;   /* at most 1024 experts                                               */
+  int64_t expert_begin, expert_end;   /* at most 1024 experts; not negative                                 */
   int quantise;
   const void* scale;        /* see above; may be NULL                                                       */
   int scale_dtype;

@@ -33,11 +33,12 @@ constexpr int kKeyShift = 12;             // (expert, assignment) in one word on
 static_assert(kDirectIds <= (1 << kKeyShift), "an assignment's number fits below the expert");
 constexpr int kNoExpert = -1;
 
-// Expert of assignment i relative to the range [begin, begin + experts), or kNoExpert.
+// Expert of assignment i relative to the range [begin, begin + experts), or kNoExpert.  begin is not negative, so that the difference
+// of an index behind it fits.
 template <typename IdT>
 __device__ __forceinline__ int expert_of(const IdT* __restrict__ ids, int64_t i, int64_t begin, int experts) {
-  const int64_t e = static_cast<int64_t>(ids[i]) - begin;
-  return (e >= 0 && e < experts) ? static_cast<int>(e) : kNoExpert;
+  const int64_t id = static_cast<int64_t>(ids[i]);
+  return (id >= begin && id - begin < experts) ? static_cast<int>(id - begin) : kNoExpert;
 }
 
 // ------------------------------------------------------------------------------------------------ sorting
@@ -56,7 +57,7 @@ static_assert(kMaxExperts < (1 << kExpertBits), "an expert's number and the one 
 
 template <typename IdT>
 __global__ void __launch_bounds__(kSortThreads, 1)
-moe_sort_kernel(const IdT* __restrict__ ids, int64_t n, int64_t begin, int experts, int strict_limit,
+moe_sort_kernel(const IdT* __restrict__ ids, int64_t n, int64_t begin, int experts, int64_t strict_limit,
                 int32_t* __restrict__ row_idx, int32_t* __restrict__ row_src, int64_t* __restrict__ expert_tokens,
                 int cumulative, int32_t* __restrict__ valid_rows, int2* __restrict__ row_info, int topk) {
   extern __shared__ int sort_smem[];
@@ -78,7 +79,7 @@ moe_sort_kernel(const IdT* __restrict__ ids, int64_t n, int64_t begin, int exper
       e[b] = kNoExpert;
       if (s + b < s1 && i < n) {
         const int64_t id = static_cast<int64_t>(ids[i]);
-        if (id - begin >= 0 && id - begin < experts) e[b] = static_cast<int>(id - begin);
+        if (id >= begin && id - begin < experts) e[b] = static_cast<int>(id - begin);
         else if (strict_limit && id >= strict_limit) record_device_error(kDevExpertRange);
       }
     }
@@ -224,7 +225,7 @@ __device__ __forceinline__ void direct_rows(const IdT* __restrict__ ids, int n, 
 
 // Rows of every expert (cumulative or not), by one CTA, for the direct path.
 template <typename IdT>
-__device__ __forceinline__ void direct_expert_tokens(const IdT* __restrict__ ids, int n, int64_t begin, int experts, int strict_limit,
+__device__ __forceinline__ void direct_expert_tokens(const IdT* __restrict__ ids, int n, int64_t begin, int experts, int64_t strict_limit,
                                                      int64_t* __restrict__ expert_tokens, int cumulative) {
   __shared__ int count[kMaxExperts];
   for (int e = threadIdx.x; e < experts; e += blockDim.x) count[e] = 0;
@@ -264,7 +265,7 @@ struct RouteIds {
   int64_t n;                 // tokens * topk
   int64_t begin;
   int experts, topk;
-  int strict_limit;          // indices from here on are an error (0: they are merely outside the range)
+  int64_t strict_limit;      // indices from here on are an error (0: they are merely outside the range)
 };
 
 // Copy, few assignments: one CTA a token finds the rows of its topk slots and copies the token there; one more CTA
@@ -1151,6 +1152,7 @@ extern "C" int b200q_moe_route(const b200q_moe_route_args* a, void* stream) {
   B200Q_REQUIRE(a->topk <= 1024 && a->tokens <= 0x7fffffffLL && a->tokens * a->topk < 0x7fffffffLL && a->hidden <= (1LL << 28),
                 B200Q_ERR_UNSUPPORTED, "moe_route: more than 2^31-2 assignments, 1024 slots or 2^28 columns");
   B200Q_REQUIRE(a->idx_dtype == B200Q_I32 || a->idx_dtype == B200Q_I64, B200Q_ERR_UNSUPPORTED, "moe_route: expert indices must be i32 or i64");
+  B200Q_REQUIRE(a->expert_begin >= 0, B200Q_ERR_BAD_ARG, "moe_route: negative expert_begin (a negative index is a padded token's)");
   B200Q_REQUIRE(a->expert_end > a->expert_begin && a->expert_end - a->expert_begin <= kMaxExperts, B200Q_ERR_UNSUPPORTED,
                 "moe_route: the expert range must hold 1 to %d experts", kMaxExperts);
   const int64_t n = a->tokens * a->topk;
@@ -1188,7 +1190,7 @@ extern "C" int b200q_moe_route(const b200q_moe_route_args* a, void* stream) {
                 "moe_route: needs %zu bytes of 256-byte aligned workspace, got %zu", need, a->workspace_bytes);
   int32_t* valid_rows = static_cast<int32_t*>(a->workspace);
   int2* row_info = a->quantise && need != 0 ? reinterpret_cast<int2*>(static_cast<uint8_t*>(a->workspace) + 256) : nullptr;
-  RouteIds r{a->expert_idx, n, a->expert_begin, (int)(a->expert_end - a->expert_begin), (int)a->topk, a->strict ? (int)a->expert_end : 0};
+  RouteIds r{a->expert_idx, n, a->expert_begin, (int)(a->expert_end - a->expert_begin), (int)a->topk, a->strict ? a->expert_end : 0};
   return a->idx_dtype == B200Q_I64 ? route<int64_t>(*a, r, row_info, valid_rows, st) : route<int32_t>(*a, r, row_info, valid_rows, st);
 }
 

@@ -112,3 +112,29 @@ def test_statistics_of_rows_without_columns(npu, shape):
             _, rstd, _, post_rstd = npu.npu_gated_add_rms_norm(x, x, w, post_gamma=w)
             assert rstd.shape == post_rstd.shape == shape[:-1]
             assert bool(torch.isnan(rstd).all()) and bool(torch.isnan(post_rstd).all())
+
+
+@pytest.mark.parametrize("tokens", [40, 3000])
+def test_a_strict_range_past_32_bits(npu, tokens):
+    """Experts numbered from 2^31 on: an index before the range has no row and is no error, also where the range's end does not fit into
+    32 bits."""
+    from pytorch_b200 import _cabi as cabi
+    begin, experts, h = 2 ** 31, 8, 16
+    g = torch.Generator().manual_seed(tokens)
+    local = torch.randint(-1, experts, (tokens, 1), generator=g)
+    idx = torch.where(local < 0, torch.full_like(local, 7), local + begin)
+    idx[3] = -2 ** 63
+    x = torch.randn((tokens, h), generator=g)
+    cx, ids, out = x.cuda(), idx.cuda(), torch.full((tokens, h), 7.0, device="cuda")
+    place, ends = torch.empty(tokens, dtype=torch.int32, device="cuda"), torch.empty(experts, dtype=torch.int64, device="cuda")
+    ws = torch.empty(256, dtype=torch.uint8, device="cuda")
+    a = cabi.MoeRouteArgs()
+    a.x, a.x_dtype, a.expert_idx, a.idx_dtype = cx.data_ptr(), cabi.F32, ids.data_ptr(), cabi.I64
+    a.tokens, a.topk, a.hidden, a.expert_begin, a.expert_end, a.strict = tokens, 1, h, begin, begin + experts, 1
+    a.out, a.out_rows, a.row_idx, a.expert_tokens = out.data_ptr(), tokens, place.data_ptr(), ends.data_ptr()
+    a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
+    assert cabi.lib().b200q_moe_route(C.byref(a), torch.cuda.current_stream().cuda_stream) == cabi.OK
+    torch.cuda.synchronize()
+    assert cabi.device_error() == 0
+    row, src, counts = oracle.sorted_rows(idx, begin, begin + experts)
+    assert torch.equal(place.cpu(), row) and torch.equal(ends.cpu(), counts) and torch.equal(out.cpu(), oracle.gather_rows(x, src, 1))
