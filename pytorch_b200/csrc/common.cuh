@@ -84,7 +84,7 @@ int resident_ctas(int threads) {
 }
 
 // Launches a kernel that may start before the kernel in front of it on the stream has finished (programmatic
-// dependent launch): it must not touch what that kernel writes before wait_for_primary() and reads it by ld_of_primary(), and the
+// dependent launch): it must not touch what that kernel writes before wait_for_primary() and reads it by ld_of_primary(_cached), and the
 // kernel in front must itself be an ordinary launch, so that everything before it is complete.
 template <typename... Params, typename... Args>
 int launch_dependent(void (*kern)(Params...), unsigned grid, int threads, cudaStream_t st, const char* what, Args&&... args) {

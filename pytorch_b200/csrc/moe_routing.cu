@@ -33,12 +33,15 @@ constexpr int kKeyShift = 12;             // (expert, assignment) in one word on
 static_assert(kDirectIds <= (1 << kKeyShift), "an assignment's number fits below the expert");
 constexpr int kNoExpert = -1;
 
-// Expert of assignment i relative to the range [begin, begin + experts), or kNoExpert.  begin is not negative, so that the difference
-// of an index behind it fits.
+// Expert relative to the range [begin, begin + experts), or kNoExpert.  begin is not negative, so as an unsigned number the
+// difference of an index before it, or of a negative one, is past any range.
+__device__ __forceinline__ int expert_in_range(int64_t id, int64_t begin, int experts) {
+  const uint64_t e = static_cast<uint64_t>(id) - static_cast<uint64_t>(begin);
+  return e < static_cast<uint64_t>(experts) ? static_cast<int>(e) : kNoExpert;
+}
 template <typename IdT>
 __device__ __forceinline__ int expert_of(const IdT* __restrict__ ids, int64_t i, int64_t begin, int experts) {
-  const int64_t id = static_cast<int64_t>(ids[i]);
-  return (id >= begin && id - begin < experts) ? static_cast<int>(id - begin) : kNoExpert;
+  return expert_in_range(static_cast<int64_t>(ids[i]), begin, experts);
 }
 
 // ------------------------------------------------------------------------------------------------ sorting
@@ -79,8 +82,8 @@ moe_sort_kernel(const IdT* __restrict__ ids, int64_t n, int64_t begin, int exper
       e[b] = kNoExpert;
       if (s + b < s1 && i < n) {
         const int64_t id = static_cast<int64_t>(ids[i]);
-        if (id >= begin && id - begin < experts) e[b] = static_cast<int>(id - begin);
-        else if (strict_limit && id >= strict_limit) record_device_error(kDevExpertRange);
+        e[b] = expert_in_range(id, begin, experts);
+        if (strict_limit && e[b] < 0 && id >= strict_limit) record_device_error(kDevExpertRange);
       }
     }
   };
@@ -490,10 +493,10 @@ moe_quant_kernel(int64_t n, const T* __restrict__ x, int64_t width, const ST* __
   // A row's token and expert are read two rows ahead, its x one row ahead.
   int2 here = make_int2(0, 0), after = make_int2(0, 0);
   if (r0 < r1) {
-    after = ld_of_primary(row_info + r0);
+    after = ld_of_primary_cached(row_info + r0);
     load(after.x);
   }
-  int2 later = r0 + 1 < r1 ? ld_of_primary(row_info + r0 + 1) : make_int2(0, 0);
+  int2 later = r0 + 1 < r1 ? ld_of_primary_cached(row_info + r0 + 1) : make_int2(0, 0);
   // This CTA's share of the rows that no assignment owns.
   const int64_t idle = n - valid;
   for (int64_t row = valid + idle * blockIdx.x / gridDim.x; row < valid + idle * (blockIdx.x + 1) / gridDim.x; ++row) {
@@ -513,7 +516,7 @@ moe_quant_kernel(int64_t n, const T* __restrict__ x, int64_t width, const ST* __
       for (int q = 0; q < ITERS; ++q) raw[q] = nxt[q];
       if (row + 1 < r1) load(after.x);
     }
-    if (row + 2 < r1) later = ld_of_primary(row_info + row + 2);
+    if (row + 2 < r1) later = ld_of_primary_cached(row_info + row + 2);
     par ^= 1;                                              // a buffer is written again only behind the other one's barrier
     const ST* sm = smooth == nullptr ? nullptr : smooth + (smooth_rows > 1 ? here.y * width : 0);
     if constexpr (ITERS > 0) {

@@ -429,15 +429,17 @@ __device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontr
 __device__ __forceinline__ void wait_for_primary() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 // Reads what that kernel wrote, behind wait_for_primary().  A load through a const __restrict__ pointer may be taken for one of
 // read-only data: the compiler may move it in front of the wait, and the SM's L1 may answer it with what a neighbouring address
-// brought in before the wait.  These are neither moved nor answered by L1.
+// brought in before the wait.  Neither of these moves in front of the wait.
+// For a kernel that loads other data before it waits: not answered by L1.
 __device__ __forceinline__ int32_t ld_of_primary(const int32_t* p) {
   int32_t v;
   asm volatile("ld.relaxed.gpu.global.s32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
   return v;
 }
-__device__ __forceinline__ int2 ld_of_primary(const int2* p) {
+// For a kernel that loads nothing before it waits, so that L1 holds nothing of it: L1 answers a CTA's other warps.
+__device__ __forceinline__ int2 ld_of_primary_cached(const int2* p) {
   int2 v;
-  asm volatile("ld.relaxed.gpu.global.v2.s32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p) : "memory");
+  asm volatile("ld.global.v2.s32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
   return v;
 }
 
