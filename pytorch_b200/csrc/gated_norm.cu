@@ -104,9 +104,11 @@ __device__ __forceinline__ void store8(T* __restrict__ row, int i, int width, co
   }
 }
 
-// Eight parameter values, zero past the width: a row's values are zero there too, and a parameter that is not finite must not make
-// them anything else.
-template <typename P, bool VEC>
+// Eight parameter values.  Past the width the last column's are read, and the row's values are zero there.  CLEAR: the parameter is
+// taken as zero too, so that an infinite one makes nothing there that reaches the other columns through a row's sum or maximum (in the
+// gradient the column itself does: every column of such a row is NaN by the formulas).  The value is loaded first and then chosen: loads
+// that wait for a predicate took up to 1.6 times as long for rows above 8192 columns.
+template <typename P, bool VEC, bool CLEAR>
 __device__ __forceinline__ void param8(const P* __restrict__ p, int i, int width, const Place& at, float2 (&f)[4]) {
   const int c = at.col<VEC>(i, 0);
   if constexpr (VEC) {
@@ -114,8 +116,8 @@ __device__ __forceinline__ void param8(const P* __restrict__ p, int i, int width
   } else {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const int c0 = c + 2 * j * at.threads, c1 = c0 + at.threads;
-      f[j] = make_float2(c0 < width ? to_f32<P>(p[c0]) : 0.0f, c1 < width ? to_f32<P>(p[c1]) : 0.0f);
+      f[j] = make_float2(to_f32<P>(p[min(c + 2 * j * at.threads, width - 1)]), to_f32<P>(p[min(c + (2 * j + 1) * at.threads, width - 1)]));
+      if constexpr (CLEAR) f[j] = make_float2(c + 2 * j * at.threads < width ? f[j].x : 0.0f, c + (2 * j + 1) * at.threads < width ? f[j].y : 0.0f);
     }
   }
 }
@@ -126,14 +128,14 @@ struct Gate {
   int per_row;
   int64_t rows_per;
 };
-template <typename P, bool VEC>
+template <typename P, bool VEC, bool CLEAR>
 __device__ __forceinline__ void gate8(const Gate& g, int64_t gate_row, int i, int width, const Place& at, float2 (&f)[4]) {
   if (g.p == nullptr || g.per_row) {
     const float v = g.p == nullptr ? 1.0f : to_f32<P>(static_cast<const P*>(g.p)[gate_row]);
 #pragma unroll
     for (int j = 0; j < 4; ++j) f[j] = make_float2(v, v);
   } else {
-    param8<P, VEC>(static_cast<const P*>(g.p) + gate_row * width, i, width, at, f);
+    param8<P, VEC, CLEAR>(static_cast<const P*>(g.p) + gate_row * width, i, width, at, f);
   }
 }
 
@@ -360,8 +362,8 @@ gated_norm_kernel(const NormArgs a) {
   const P* gamma = static_cast<const P*>(a.gamma);
   const P* post = static_cast<const P*>(a.post);
   auto smooth8 = [&](int i, float2(&f)[4]) {
-    if (a.smooth_f32) param8<float, VEC>(static_cast<const float*>(a.smooth), i, a.width, at, f);
-    else param8<T, VEC>(static_cast<const T*>(a.smooth), i, a.width, at, f);
+    if (a.smooth_f32) param8<float, VEC, true>(static_cast<const float*>(a.smooth), i, a.width, at, f);
+    else param8<T, VEC, true>(static_cast<const T*>(a.smooth), i, a.width, at, f);
   };
   Pack8<T> xr[ITERS], rr[ITERS];
   auto load_row = [&](int64_t row) {
@@ -374,15 +376,15 @@ gated_norm_kernel(const NormArgs a) {
   if ((int64_t)blockIdx.x < a.rows) load_row(blockIdx.x);
   float2 early_post[4], early_gamma[4], early_smooth[4];
   if constexpr (EARLY) {
-    if (post != nullptr) param8<P, VEC>(post, 0, a.width, at, early_post);
-    param8<P, VEC>(gamma, 0, a.width, at, early_gamma);
+    if (post != nullptr) param8<P, VEC, true>(post, 0, a.width, at, early_post);
+    param8<P, VEC, true>(gamma, 0, a.width, at, early_gamma);
     if (QUANT && a.smooth != nullptr) smooth8(0, early_smooth);
   }
   const float2 alpha = splat(a.alpha);
   for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
     const int64_t gate_row = a.gate.rows_per == 1 ? row : a.gate.rows_per >= a.rows ? 0 : row / a.gate.rows_per;
     float2 early_gate[4];
-    if constexpr (EARLY) gate8<P, VEC>(a.gate, gate_row, 0, a.width, at, early_gate);
+    if constexpr (EARLY) gate8<P, VEC, true>(a.gate, gate_row, 0, a.width, at, early_gate);
     float r1 = 1.0f;
     if (post != nullptr) {
       float2 s2 = splat(0.0f);
@@ -404,8 +406,8 @@ gated_norm_kernel(const NormArgs a) {
     for (int i = 0; i < ITERS; ++i) {
       float2 g[4], w[4];
       if constexpr (!EARLY) {
-        gate8<P, VEC>(a.gate, gate_row, i, a.width, at, g);
-        if (post != nullptr) param8<P, VEC>(post, i, a.width, at, w);
+        gate8<P, VEC, true>(a.gate, gate_row, i, a.width, at, g);
+        if (post != nullptr) param8<P, VEC, true>(post, i, a.width, at, w);
       }
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -426,7 +428,7 @@ gated_norm_kernel(const NormArgs a) {
     for (int i = 0; i < ITERS; ++i) {
       float2 w[4], sm[4];
       if constexpr (!EARLY) {
-        param8<P, VEC>(gamma, i, a.width, at, w);
+        param8<P, VEC, true>(gamma, i, a.width, at, w);
         if (QUANT && a.smooth != nullptr) smooth8(i, sm);
       }
 #pragma unroll
@@ -489,11 +491,11 @@ gated_norm_pipe_kernel(const NormArgs a, int threads_per_row, int stages) {
   const float2 alpha = splat(a.alpha);
   // A thread's columns stay the same: so do its parameters, but for the gate.
   float2 w_post[4], w_gamma[4], w_smooth[4], g[4];
-  if (post != nullptr) param8<P, VEC>(post, 0, a.width, at, w_post);
-  param8<P, VEC>(static_cast<const P*>(a.gamma), 0, a.width, at, w_gamma);
+  if (post != nullptr) param8<P, VEC, true>(post, 0, a.width, at, w_post);
+  param8<P, VEC, true>(static_cast<const P*>(a.gamma), 0, a.width, at, w_gamma);
   if (QUANT && a.smooth != nullptr) {
-    if (a.smooth_f32) param8<float, VEC>(static_cast<const float*>(a.smooth), 0, a.width, at, w_smooth);
-    else param8<T, VEC>(static_cast<const T*>(a.smooth), 0, a.width, at, w_smooth);
+    if (a.smooth_f32) param8<float, VEC, true>(static_cast<const float*>(a.smooth), 0, a.width, at, w_smooth);
+    else param8<T, VEC, true>(static_cast<const T*>(a.smooth), 0, a.width, at, w_smooth);
   }
   // The gate of the group's rows, walked along; rows_per 1: the row itself.
   const int rows_per = (int)min(a.gate.rows_per, a.rows);
@@ -554,7 +556,7 @@ gated_norm_pipe_kernel(const NormArgs a, int threads_per_row, int stages) {
       for (int i = 0; i < ITERS; ++i) {
 #pragma unroll
         for (int k = 0; k < ROWS; ++k) {
-          if (gate_row[k] != have_gate) gate8<P, VEC>(a.gate, gate_row[k], i, a.width, at, g);
+          if (gate_row[k] != have_gate) gate8<P, VEC, true>(a.gate, gate_row[k], i, a.width, at, g);
           have_gate = gate_row[k];
           const Pack8<T> rr = smem8<T, VEC>(rs[k], i, a.width, at);
 #pragma unroll
@@ -751,9 +753,9 @@ struct GlobalParams {
   const NormGradArgs& a;
   const Place& at;
   int64_t gate_row;
-  __device__ __forceinline__ void gate(int i, float2 (&f)[4]) const { gate8<P, VEC>(a.gate, gate_row, i, a.width, at, f); }
-  __device__ __forceinline__ void post(int i, float2 (&f)[4]) const { param8<P, VEC>(static_cast<const P*>(a.post), i, a.width, at, f); }
-  __device__ __forceinline__ void gamma(int i, float2 (&f)[4]) const { param8<P, VEC>(static_cast<const P*>(a.gamma), i, a.width, at, f); }
+  __device__ __forceinline__ void gate(int i, float2 (&f)[4]) const { gate8<P, VEC, false>(a.gate, gate_row, i, a.width, at, f); }
+  __device__ __forceinline__ void post(int i, float2 (&f)[4]) const { param8<P, VEC, false>(static_cast<const P*>(a.post), i, a.width, at, f); }
+  __device__ __forceinline__ void gamma(int i, float2 (&f)[4]) const { param8<P, VEC, false>(static_cast<const P*>(a.gamma), i, a.width, at, f); }
 };
 struct RegisterParams {
   float2 g[4], w1[4], w2[4];
@@ -925,13 +927,13 @@ gated_norm_grad_vector_kernel(const NormGradArgs a, int threads_per_row) {
     rs1 = a.post != nullptr ? a.post_rstd[row] : 1.0f;
   };
   RegisterParams params;
-  if (a.post != nullptr) param8<P, VEC>(static_cast<const P*>(a.post), 0, a.width, at, params.w1);
-  param8<P, VEC>(static_cast<const P*>(a.gamma), 0, a.width, at, params.w2);
+  if (a.post != nullptr) param8<P, VEC, false>(static_cast<const P*>(a.post), 0, a.width, at, params.w1);
+  param8<P, VEC, false>(static_cast<const P*>(a.gamma), 0, a.width, at, params.w2);
   const int64_t r0 = a.rows * blockIdx.x / gridDim.x, r1 = a.rows * (blockIdx.x + 1) / gridDim.x;
   for (int64_t seg = r0; seg < r1;) {
     const int64_t gate = SUM_GATE ? seg / a.gate.rows_per : 0;
     const int64_t seg_end = SUM_GATE ? min(r1, (gate + 1) * a.gate.rows_per) : r1;
-    if (SUM_GATE) gate8<P, VEC>(a.gate, gate, 0, a.width, at, params.g);
+    if (SUM_GATE) gate8<P, VEC, false>(a.gate, gate, 0, a.width, at, params.g);
     Pack8<T> kept[4], next[4];
     float rs1 = 1.0f, rs2 = 0.0f, next1 = 1.0f, next2 = 0.0f;
     if (AHEAD && seg + group < seg_end) fetch(seg + group, next, next1, next2);
@@ -953,7 +955,7 @@ gated_norm_grad_vector_kernel(const NormGradArgs a, int threads_per_row) {
         }
         fetch(row, kept, rs1, rs2);
       }
-      if (!SUM_GATE) gate8<P, VEC>(a.gate, row, 0, a.width, at, params.g);
+      if (!SUM_GATE) gate8<P, VEC, false>(a.gate, row, 0, a.width, at, params.g);
       auto load = [&](int q, int) { return kept[q]; };
       norm_grad_row<T, P, VEC, 1, SUM_GATE>(a, at, row, rs1, rs2, load, params, sums, red[0][group], red[1][group], 1 + group, true);
     }
@@ -1045,8 +1047,8 @@ gated_norm_grad_pipe_kernel(const NormGradArgs a, int threads_per_row, int stage
     look(r0, end);
     // A thread's columns stay the same: so do its parameters, but for the gate.
     RegisterParams params;
-    if (a.post != nullptr) param8<P, VEC>(static_cast<const P*>(a.post), 0, a.width, at, params.w1);
-    param8<P, VEC>(static_cast<const P*>(a.gamma), 0, a.width, at, params.w2);
+    if (a.post != nullptr) param8<P, VEC, false>(static_cast<const P*>(a.post), 0, a.width, at, params.w1);
+    param8<P, VEC, false>(static_cast<const P*>(a.gamma), 0, a.width, at, params.w2);
     int have_gate = -1;
     bool ok = true;
     for (int chunk = r0; chunk < r1;) {
@@ -1065,7 +1067,7 @@ gated_norm_grad_pipe_kernel(const NormGradArgs a, int threads_per_row, int stage
         for (int q = 0; q < 4; ++q)
           if (q < 3 || a.dh != nullptr) kept[q] = smem8<T, VEC>(pipe.slot(stage, q) + off, 0, a.width, at);
         auto load = [&](int q, int) { return kept[q]; };
-        if (row_gate != have_gate) gate8<P, VEC>(a.gate, row_gate, 0, a.width, at, params.g);
+        if (row_gate != have_gate) gate8<P, VEC, false>(a.gate, row_gate, 0, a.width, at, params.g);
         have_gate = row_gate;
         norm_grad_row<T, P, VEC, ITERS, SUM_GATE>(a, at, row, rs1, rs2, load, params, sums, red[0][group], red[1][group], 1 + group, ok);
       }
