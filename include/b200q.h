@@ -253,7 +253,8 @@ int b200q_trans_quant_param(const float* scale, int64_t scale_len, int64_t* out,
  * assignments by expert.  An expert outside [expert_begin, expert_end) (-1 for a padded token) has no row.
  *   quantise == 0: out[row] = x[i / topk] as it is (any dtype); a token's scale [tokens] f32 goes along to out_scale.
  *   quantise == 1: xs = x * smooth (smooth [scale_rows, hidden], one row or one for each expert, or NULL), then int8 and
- *                  out_scale as b200q_dynamic_quant.
+ *                  out_scale as b200q_dynamic_quant (as there, a row with an infinity or a NaN is not defined; it reaches no
+ *                  other row).
  * Rows past the last expert's are zero (their out_scale too). */
 typedef struct {
   const void* x;            /* [tokens, hidden] bf16, f16; without quantisation also f32, i32, i8           */
@@ -349,7 +350,7 @@ typedef struct {
 
 int b200q_gated_norm(const b200q_gated_norm_args* args, void* stream);
 /* Gradient; of args it reads x, residual, the parameters, residual_scale, rstd and post_rstd.  Sums over rows are added
- * in fp32 in a fixed order. */
+ * in fp32 in a fixed order.  At most 65533 gates that are shared by several rows. */
 size_t b200q_gated_norm_grad_workspace_bytes(const b200q_gated_norm_args* args);
 int b200q_gated_norm_grad(const b200q_gated_norm_args* args, const b200q_gated_norm_grads* grads, void* stream);
 

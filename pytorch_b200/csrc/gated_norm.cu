@@ -10,11 +10,13 @@
 //   dresidual = a * dh       dg = dh * z (summed to g's shape)            dz = dh * g
 //   dw1 = sum over rows of dz * xn      v = dz * w1      dx = r1 * (v - xn * mean(v * xn))
 //
-// Bound by HBM: the forward pass reads x and the residual and writes y and h, the gradient reads x, the residual and both
-// gradients and writes two, each once; a row stays in its CTA's registers between the reductions.  Everything between
-// loading and storing is fp32: h is not rounded before its norm, and the gradient computes it again from x and the
-// residual instead of reading the rounded one.  Sums over rows (dw1, dw2, a shared gate) are kept in shared memory or registers
-// by CTAs that take contiguous rows, written once per CTA as fp32 and added by a second kernel in a fixed order.
+// The forward pass reads x and the residual and writes y and h, the gradient reads x, the residual and both gradients and writes
+// two; a row stays in its CTA's registers between the reductions.  For rows of full vectors the forward pass is bound by HBM (0.86 of it)
+// and the gradient by the latency of its two reductions a row (0.66).  Rows of other widths pass value by value (0.2 to 0.36), and from
+// 4097 columns on their gradient reads each operand three times.  Everything between loading and storing is fp32: h is not rounded
+// before its norm, and the gradient computes it again from x and the residual instead of reading the rounded one.  Sums over rows (dw1,
+// dw2, a shared gate) are kept in shared memory or registers by CTAs that take contiguous rows, written once per CTA as fp32 and added
+// by a second kernel in a fixed order.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -1186,7 +1188,8 @@ inline RowPipePlan row_pipe_plan(int64_t width, int element, int arrays, int row
 // one vector a thread against two: 16 rows 6.1 / 8.2 us, 296 8.2 / 10.2, 600 10.2 / 10.2, 4096 32.8 / 30.7).  Many rows that are not
 // made of full vectors go through shared memory from a few hundred columns up to 4096 and from a 16-byte boundary on (f16, straight
 // from global memory against through shared memory: 600 rows of 1111 8.2 / 10.2 us, 6124 32.8 / 30.7, 3000 of 4000 51.2 / 45.1;
-// 6124 of 264 16.4 / 16.4, 20000 of 96 18.4 / 20.5).
+// 6124 of 264 16.4 / 16.4, 20000 of 96 18.4 / 20.5).  What a width off the grid of full vectors costs, bf16, forward: 16384 rows of 1152
+// 64 us and 6144 of 2880 68 (where 8192 of 4096 take 47), 2048 of 12296 266 (of 12288 47).
 template <typename T, typename P, bool VEC, bool QUANT>
 int launch_norm(const NormArgs& a, cudaStream_t st) {
   const bool many = a.rows > 2 * sm_count();
@@ -1227,7 +1230,8 @@ inline int grad_ctas(int64_t rows) { return (int)(rows < sm_count() ? rows : sm_
 // row sums' shuffles; two vectors a thread with the sums in shared memory took 121, rows through shared memory 176 to 203; 16384 rows of 1024
 // 45 against 61); above two (4096 rows of 8192: 125 us) or four vectors a thread.
 // Else through shared memory, up to 4096 columns and from a 16-byte boundary on (f16, read three times from global memory against
-// that: 100 rows of 1111 65 / 16 us, 6124 309 / 59, 3000 of 4000 342 / 84, 20000 of 96 364 / 47), and straight for what is left.
+// that: 100 rows of 1111 65 / 16 us, 6124 309 / 59, 3000 of 4000 342 / 84, 20000 of 96 364 / 47), and straight for what is left, with
+// spills of 1 to 1.4 KB a thread (bf16: 4096 rows of 5376 620 us, 2048 of 12296 687, where 2048 of 12288 take 172).
 template <typename T, typename P, bool VEC>
 int launch_norm_grad(const NormGradArgs& a, const NormSumArgs& s, bool sum_gate, cudaStream_t st) {
 #define B200Q_NORM_GRAD(I, MAX, MIN, SUM)                                                                                \

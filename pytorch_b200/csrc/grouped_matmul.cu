@@ -17,14 +17,12 @@
 //   warp 1      MMA issuer; accumulators in TMEM, two buffers, so that one tile's epilogue overlaps the next one's products
 //   warps 2-9   epilogue: a lane owns a channel; neighbouring lanes exchange tokens so that a lane stores two channels
 // Three instantiations: CTA pairs and single CTAs with up to 256 tokens a tile (bound by the tensor cores), and single CTAs
-// with up to 64 and a deeper ring (few rows an expert: bound by reading the weights).  128 rows over 64 weights of 4096 x 4096 take
-// 139 us (6.7 TB/s of weights); 16384 rows over 8 weights of 4096 x 22016 1058 us in a burst (2790 TOP/s) and 1230 under the
+// with up to 64 and a deeper ring (few rows an expert: bound by reading the weights).  Two rows for each of 64 weights of 4096 x 4096
+// take 159 us (6.75 TB/s of weights); 16384 rows over 8 weights of 4096 x 22016 1058 us in a burst (2790 TOP/s) and 1230 under the
 // power cap; 1531 very unequal rows over 24 weights of 5120 x 1416 46 us (up to 128 tokens a tile and six stages: 44 there, but
 // 270 against 245 with 64 groups of 128 rows and 60 against 51 with 8 of 256).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
-
-#include <mutex>
 
 #include "common.cuh"
 #include "ptx.cuh"
@@ -446,7 +444,9 @@ grouped_matmul_kernel(const __grid_constant__ GroupedMaps<MAX_TOKENS> maps, cons
   grouped_matmul_body<1, MAX_TOKENS, STAGES, MAX_TOKENS <= 64>(maps, a);
 }
 
-// Any k, strides and alignment: one thread an output element.
+// Any k, strides and alignment: one thread an output element, which walks k byte by byte.  It is here so that every layout has an
+// answer, not for speed: 128 rows over 64 contiguous [k, n] weights of 4096 x 4096 take 1664 us where the transposed views of [n, k] take
+// 159, 2048 rows over eight of them 12570 against 41.
 __global__ void __launch_bounds__(256)
 grouped_matmul_simt_kernel(const int8_t* __restrict__ x, const int8_t* __restrict__ w, int64_t w_stride_g, int64_t w_stride_k, int64_t w_stride_n,
                            const GroupedArgs a) {

@@ -13,7 +13,9 @@ using namespace b200q_torch;
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
 
-constexpr int64_t kPermuteExperts = 1024;      // npu_moe_token_permute takes indices below this
+// npu_moe_token_permute takes indices below this and sorts for all of them, as it is not told how many experts there are: the routing of
+// 8192 x 8 indices, which is told, takes 19.8 us for 8 experts and 21.0 for 1024.
+constexpr int64_t kPermuteExperts = 1024;
 
 bool is_float_type(at::ScalarType t) { return t == at::kBFloat16 || t == at::kHalf || t == at::kFloat; }
 
