@@ -2,7 +2,6 @@
 // Meta implementations over the C ABI, and autograd functions whose backward passes are operators of their own
 // (npu_moe_token_permute_grad, npu_moe_token_unpermute_grad).  A call that needs no gradient goes straight to the
 // CUDA implementation.
-#include <torch/csrc/autograd/autograd_not_implemented_fallback.h>
 #include <torch/csrc/autograd/custom_function.h>
 
 #include "register_common.h"
@@ -749,6 +748,18 @@ NormOutputs norm_autograd(const Tensor& x, const Tensor& residual, const Tensor&
   return {o[0], o[1], o[2], o[3]};
 }
 
+// The same for the operators without an autograd kernel, below PyTorch's default one for them.
+void no_forward_mode_boxed(const c10::OperatorHandle& op, c10::DispatchKeySet keys, torch::jit::Stack* stack) {
+  const char* name = op.schema().name().c_str();
+  auto check = [&](const optional<Tensor>& t) { no_forward_mode(name, {&t}); };
+  for (const c10::IValue& v : torch::jit::last(*stack, op.schema().arguments().size())) {
+    if (v.isTensor()) check(v.toTensor());
+    else if (v.isTensorList())
+      for (const Tensor& t : v.toTensorVector()) check(t);
+  }
+  op.redispatchBoxed(keys & c10::after_ADInplaceOrView_keyset, stack);
+}
+
 }  // namespace
 
 TORCH_LIBRARY_FRAGMENT(npu, m) {
@@ -791,11 +802,14 @@ TORCH_LIBRARY_IMPL(npu, AutogradCUDA, m) {
   m.impl("npu_moe_token_permute", TORCH_FN(permute_autograd));
   m.impl("npu_moe_token_unpermute", TORCH_FN(unpermute_autograd));
   m.impl("npu_gated_add_rms_norm", TORCH_FN(norm_autograd));
-  // No derivative of their own, in either mode, although some of their outputs are floats: asking for one is an error, where
-  // PyTorch's default for an operator without an autograd kernel is a warning in reverse mode and a lost tangent in forward mode.
+}
+
+// No derivative of their own, although some of their outputs are floats.  PyTorch's default autograd kernel warns of that in a backward
+// pass, but loses a tangent without a word.
+TORCH_LIBRARY_IMPL(npu, ADInplaceOrView, m) {
   for (const char* op : {"npu_moe_init_routing_v2", "npu_moe_token_permute_grad", "npu_moe_token_unpermute_grad", "npu_gated_add_rms_norm_grad",
-                         "npu_gated_add_rms_norm_dynamic_quant"})
-    m.impl(op, torch::autograd::autogradNotImplementedFallback());
+                         "npu_gated_add_rms_norm_dynamic_quant", "npu_grouped_matmul"})
+    m.impl(op, torch::CppFunction::makeFromBoxedFunction<&no_forward_mode_boxed>());
 }
 
 TORCH_LIBRARY_IMPL(npu, Meta, m) {

@@ -138,3 +138,22 @@ def test_a_strict_range_past_32_bits(npu, tokens):
     assert cabi.device_error() == 0
     row, src, counts = oracle.sorted_rows(idx, begin, begin + experts)
     assert torch.equal(place.cpu(), row) and torch.equal(ends.cpu(), counts) and torch.equal(out.cpu(), oracle.gather_rows(x, src, 1))
+
+
+def test_router_weights_learn_through_the_quantised_block(npu):
+    """The quantised part of the block has no gradient.  A backward pass through the whole gives the router's weights theirs, with and
+    without a gradient asked for x (then behind a warning)."""
+    import pytorch_b200.contrib.function as function
+    g = torch.Generator().manual_seed(1)
+    t, k, e, h, f = 40, 2, 4, 64, 32
+    x, idx = torch.randn((t, h), generator=g).to(torch.bfloat16).cuda(), torch.topk(torch.rand((t, e), generator=g), k).indices.int().cuda()
+    w_in, w_out = (torch.randint(-127, 128, s, generator=g).to(torch.int8).cuda() for s in ((e, 2 * f, h), (e, h, f)))
+    s_in, s_out = (torch.rand(s, generator=g).cuda() * 1e-3 for s in ((e, 2 * f), (e, h)))
+    probs, dy = torch.rand((t, k), generator=g).cuda(), torch.randn((t, h), generator=g).to(torch.bfloat16).cuda()
+    grads = []
+    for asked in (False, True):
+        a, p = x.clone().requires_grad_(asked), probs.clone().requires_grad_()
+        function.w8a8_swiglu_moe(a, idx, p, None, w_in, s_in, None, w_out, s_out).backward(dy)
+        assert a.grad is None
+        grads.append(p.grad)
+    assert torch.equal(grads[0], grads[1]) and float(grads[0].abs().min()) > 0
